@@ -7,8 +7,8 @@
  * the reference lines (relative to the reference root) it replaces.
  *
  * Conventions
- *   - all tensors are fp32, row-major (batch, feature), resident in device memory and
- *     owned by the caller; the library never allocates or frees device memory;
+ *   - all tensors are fp32 (the tensor operators also take bf16 and fp16), row-major (batch, feature),
+ *     resident in device memory and owned by the caller; the library never allocates or frees device memory;
  *   - nn.Linear.weight is (out, in); a model's parameters travel as ONE flat fp32 arena
  *     in `parameters()` order: for each MLP in [logl (iVAE only), f, g, logv], for each
  *     layer: weight (out*in) then bias (out)           (models/nets.py:422-430, 99-106);
@@ -27,7 +27,10 @@
 extern "C" {
 #endif
 
-enum { IVAE_ACT_NONE = 0, IVAE_ACT_LRELU = 1, IVAE_ACT_XTANH = 2, IVAE_ACT_SIGMOID = 3 };
+enum { IVAE_ACT_NONE = 0, IVAE_ACT_LRELU = 1, IVAE_ACT_XTANH = 2, IVAE_ACT_SIGMOID = 3,
+       IVAE_ACT_GELU = 4, IVAE_ACT_SILU = 5 };      /* the last two: ivae_linear only */
+
+enum { IVAE_F32 = 0, IVAE_BF16 = 1, IVAE_F16 = 2 }; /* element types of the tensor operators */
 
 enum {
     IVAE_OK = 0,
@@ -36,7 +39,8 @@ enum {
     IVAE_E_NULLPTR = -3,      /* a required pointer is NULL */
     IVAE_E_TOOLARGE = -4,     /* shape exceeds what the kernels' LDS tiling supports */
     IVAE_E_HIP = -5,          /* a HIP call failed; see ivae_last_hip_error() */
-    IVAE_E_WORKSPACE = -6     /* workspace smaller than ivae_workspace_bytes() */
+    IVAE_E_WORKSPACE = -6,    /* workspace smaller than ivae_workspace_bytes() */
+    IVAE_E_BADTYPE = -7       /* unknown element type (IVAE_F32 / IVAE_BF16 / IVAE_F16) */
 };
 
 /* Shape of one model and of one call.  Mirrors the constructor arguments at
@@ -232,6 +236,60 @@ int ivae_corr_static(const float* x, const float* y, int64_t n, int32_t d, doubl
  * x, y (n_blocks, n, d) fp32; cc_out (n_blocks, d, d) float64.  One launch, no workspace. */
 int ivae_corr_batched(const float* x, const float* y, int64_t n_blocks, int64_t n, int32_t d,
                       double* cc_out, void* stream);
+
+/* ---- tensor operators of a residual MLP block ---------------------------------------------
+ * What a wider or deeper MLP than those of models/nets.py:65-121 is built from: y = h + dropout(W2 act(W1 norm(h) + b1) + b2)
+ * is the three operators below and nothing else, forward and backward.  NO COUNTERPART IN THE REFERENCE.
+ * A tensor is a matrix of `rows` rows; inputs may have a row stride (ld*, in elements, >= 0; 0 repeats one row), weights and
+ * outputs are dense.  No alignment beyond an element's is asked for.  rows = 0 is a valid call (parameter gradients become 0).
+ * Outputs may not overlap inputs.  Sums are in 32 bits and in a fixed order: equal calls give equal bits. */
+
+/* y = act(x w^T + b) + residual;  x (rows, in_features), w (out_features, in_features), b (out_features) or NULL,
+ * residual (rows, out_features) or NULL, y (rows, out_features).
+ * saved: NULL, or (rows, out_features) values that the backward pass of an activation other than IVAE_ACT_NONE needs: the
+ * pre-activation in fp32, or for IVAE_BF16 in fp16 (clamped to fp16's range, its sign kept).
+ * ivae_linear_backward: dy (rows, out_features) -> dx (rows, in_features), dw (like w), db (out_features); any of them may be
+ * NULL.  The gradient of the residual is dy itself.  In large products act'(s) dy is rounded to the element type first.
+ * Limits: in_features, out_features <= 2^24, rows <= 2^40: IVAE_E_TOOLARGE. */
+typedef struct IvaeLinear {
+    int64_t rows;
+    int32_t in_features, out_features;
+    int32_t dtype;              /* IVAE_F32 | IVAE_BF16 | IVAE_F16, of every tensor but `saved` */
+    int32_t activation;         /* IVAE_ACT_* */
+    float   slope;              /* lrelu negative slope / xtanh linear term */
+    int64_t ldx, ld_residual, lddy;
+} IvaeLinear;
+int ivae_linear_workspace_bytes(const IvaeLinear* lin, int32_t backward, size_t* out);
+int ivae_linear(const IvaeLinear* lin, const void* x, const void* w, const void* b, const void* residual, void* y, void* saved,
+                void* workspace, size_t workspace_bytes, void* stream);
+int ivae_linear_backward(const IvaeLinear* lin, const void* dy, const void* x, const void* w, const void* saved,
+                         void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension (var: the mean of squares about the mean); weight,
+ * bias (width) or NULL, in x's type or, with weight_f32 != 0, in fp32.  stats: NULL, or (2, rows) fp32: each row's mean and
+ * 1 / sqrt(var + eps), for the backward pass.
+ * ivae_layer_norm_backward: dx (rows, width) [+ residual (rows, width), the gradient that arrives past the norm, or NULL],
+ * dweight and dbias (width, in the weight's type); any of the three may be NULL.  Limits: width <= 2^24, rows <= 2^40. */
+typedef struct IvaeNorm {
+    int64_t rows;
+    int32_t width;
+    int32_t dtype;
+    int32_t weight_f32;
+    float   eps;
+    int64_t ldx, lddy, ld_residual;
+} IvaeNorm;
+int ivae_layer_norm_workspace_bytes(const IvaeNorm* norm, size_t* out);        /* of the backward pass */
+int ivae_layer_norm(const IvaeNorm* norm, const void* x, const void* weight, const void* bias, void* y, float* stats, void* stream);
+int ivae_layer_norm_backward(const IvaeNorm* norm, const void* dy, const void* x, const float* stats, const void* weight,
+                             const void* residual, void* dx, void* dweight, void* dbias,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* y_e = residual_e + (keep_e ? x_e / (1 - p) : 0) over n dense elements; residual may be NULL.  keep_e: word e % 4 of
+ * Philox4x32-10 (Salmon et al. 2011) with counter (e / 4, offset) and key `seed` is at least floor(p 2^32).  No mask is stored:
+ * the backward pass is the same call on dy (without residual).  offset_device: NULL, or an int64 in device memory that is
+ * added to `offset` when the kernel runs, so that a captured graph draws a new mask at every replay.  0 <= p <= 1. */
+int ivae_dropout(int32_t dtype, int64_t n, const void* x, const void* residual, void* y, double p, uint64_t seed,
+                 uint64_t offset, const int64_t* offset_device, void* stream);
 
 /* ---- diagnostics ---------------------------------------------------------------------- */
 const char* ivae_last_hip_error(void);   /* text of the last failing HIP call (thread-local) */

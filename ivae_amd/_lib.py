@@ -12,9 +12,11 @@ LIB_PATH = os.environ.get("IVAE_AMD_LIB") or os.path.join(_HERE, "libivae_amd.so
 
 ACT_IDS = {"none": 0, "lrelu": 1, "xtanh": 2, "sigmoid": 3}
 
+LINEAR_ACT_IDS = dict(ACT_IDS, gelu=4, silu=5)     # what ivae_linear takes
+
 ERRORS = {
     -1: "bad dimensions", -2: "unknown activation", -3: "null pointer", -4: "shape too large for the kernels",
-    -5: "HIP error", -6: "workspace too small",
+    -5: "HIP error", -6: "workspace too small", -7: "unknown element type",
 }
 
 
@@ -35,8 +37,20 @@ class IvaeWsLayout(C.Structure):
                                          "rz", "cg", "cv", "lse_s", "lse_k")]
 
 
+class IvaeLinear(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("in_features", C.c_int32), ("out_features", C.c_int32), ("dtype", C.c_int32),
+                ("activation", C.c_int32), ("slope", C.c_float), ("ldx", C.c_int64), ("ld_residual", C.c_int64), ("lddy", C.c_int64)]
+
+
+class IvaeNorm(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("width", C.c_int32), ("dtype", C.c_int32), ("weight_f32", C.c_int32), ("eps", C.c_float),
+                ("ldx", C.c_int64), ("lddy", C.c_int64), ("ld_residual", C.c_int64)]
+
+
 EXPORTS = ["ivae_param_count", "ivae_workspace_bytes", "ivae_workspace_layout", "ivae_elbo_fwd_bwd", "ivae_forward",
            "ivae_pairwise", "ivae_pairwise_workspace_bytes", "ivae_backward", "ivae_adam_step", "ivae_elbo_adam_steps", "ivae_train_steps", "ivae_train_steps_supported", "ivae_corr_workspace_bytes", "ivae_corr", "ivae_corr_static", "ivae_corr_batched",
+           "ivae_linear_workspace_bytes", "ivae_linear", "ivae_linear_backward", "ivae_layer_norm_workspace_bytes", "ivae_layer_norm",
+           "ivae_layer_norm_backward", "ivae_dropout",
            "ivae_last_hip_error", "ivae_version", "ivae_debug_fault_inject", "ivae_debug_launch_events"]
 
 _lib = None
@@ -72,6 +86,14 @@ def lib():
     L.ivae_corr.argtypes = [vp, vp, C.c_int64, C.c_int32, vp, vp, C.c_size_t, vp]
     L.ivae_corr_static.argtypes = [vp, vp, C.c_int64, C.c_int32, vp, vp]
     L.ivae_corr_batched.argtypes = [vp, vp, C.c_int64, C.c_int64, C.c_int32, vp, vp]
+    pl, pn = C.POINTER(IvaeLinear), C.POINTER(IvaeNorm)
+    L.ivae_linear_workspace_bytes.argtypes = [pl, C.c_int32, C.POINTER(C.c_size_t)]
+    L.ivae_linear.argtypes = [pl, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+    L.ivae_linear_backward.argtypes = [pl, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+    L.ivae_layer_norm_workspace_bytes.argtypes = [pn, C.POINTER(C.c_size_t)]
+    L.ivae_layer_norm.argtypes = [pn, vp, vp, vp, vp, vp, vp]
+    L.ivae_layer_norm_backward.argtypes = [pn, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+    L.ivae_dropout.argtypes = [C.c_int32, C.c_int64, vp, vp, vp, f64, C.c_uint64, C.c_uint64, vp, vp]
     L.ivae_last_hip_error.restype = C.c_char_p
     L.ivae_version.restype = C.c_char_p
     for n in EXPORTS:

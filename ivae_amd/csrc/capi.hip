@@ -323,4 +323,99 @@ int ivae_corr_batched(const float* x, const float* y, int64_t n_blocks, int64_t 
     return e == hipSuccess ? IVAE_OK : hip_fail(e, "ivae_corr_batched");
 }
 
+// ---- tensor operators
+#define IVAE_OP_MAX_WIDTH (1 << 24)
+#define IVAE_OP_MAX_ROWS (1ll << 40)
+static int check_linear(const IvaeLinear* l) {
+    if (!l) return IVAE_E_NULLPTR;
+    if (l->dtype < IVAE_F32 || l->dtype > IVAE_F16) return IVAE_E_BADTYPE;
+    if (l->activation < IVAE_ACT_NONE || l->activation > IVAE_ACT_SILU) return IVAE_E_BADACT;
+    if (l->rows < 0 || l->in_features <= 0 || l->out_features <= 0 || l->ldx < 0 || l->ld_residual < 0 || l->lddy < 0) return IVAE_E_BADDIMS;
+    if (l->in_features > IVAE_OP_MAX_WIDTH || l->out_features > IVAE_OP_MAX_WIDTH || l->rows > IVAE_OP_MAX_ROWS) return IVAE_E_TOOLARGE;
+    return IVAE_OK;
+}
+
+int ivae_linear_workspace_bytes(const IvaeLinear* lin, int32_t backward, size_t* out) {
+    if (!out) return IVAE_E_NULLPTR;
+    const int rc = check_linear(lin);
+    if (rc) return rc;
+    *out = linear_ws_bytes(*lin, backward != 0);
+    return IVAE_OK;
+}
+
+int ivae_linear(const IvaeLinear* lin, const void* x, const void* w, const void* b, const void* residual, void* y, void* saved,
+                void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check_linear(lin);
+    if (rc) return rc;
+    if (lin->rows == 0) return IVAE_OK;
+    if (!x || !w || !y) return IVAE_E_NULLPTR;
+    const size_t need = linear_ws_bytes(*lin, false);
+    if (need && !workspace) return IVAE_E_NULLPTR;
+    if (workspace_bytes < need) return IVAE_E_WORKSPACE;
+    hipError_t e = launch_linear(*lin, x, w, b, residual, y, saved, workspace, (hipStream_t)stream);
+    return e == hipSuccess ? IVAE_OK : hip_fail(e, "ivae_linear");
+}
+
+int ivae_linear_backward(const IvaeLinear* lin, const void* dy, const void* x, const void* w, const void* saved, void* dx, void* dw,
+                         void* db, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check_linear(lin);
+    if (rc) return rc;
+    if (lin->rows > 0 && (!dy || (dw && !x) || (dx && !w) || (lin->activation != IVAE_ACT_NONE && !saved))) return IVAE_E_NULLPTR;
+    const size_t need = linear_ws_bytes(*lin, true);
+    if (need && !workspace) return IVAE_E_NULLPTR;
+    if (workspace_bytes < need) return IVAE_E_WORKSPACE;
+    if (!dx && !dw && !db) return IVAE_OK;
+    hipError_t e = launch_linear_backward(*lin, dy, x, w, saved, dx, dw, db, workspace, (hipStream_t)stream);
+    return e == hipSuccess ? IVAE_OK : hip_fail(e, "ivae_linear_backward");
+}
+
+static int check_norm(const IvaeNorm* n) {
+    if (!n) return IVAE_E_NULLPTR;
+    if (n->dtype < IVAE_F32 || n->dtype > IVAE_F16) return IVAE_E_BADTYPE;
+    if (n->rows < 0 || n->width <= 0 || n->ldx < 0 || n->lddy < 0 || n->ld_residual < 0 || !(n->eps >= 0.f)) return IVAE_E_BADDIMS;
+    if (n->width > IVAE_OP_MAX_WIDTH || n->rows > IVAE_OP_MAX_ROWS) return IVAE_E_TOOLARGE;
+    return IVAE_OK;
+}
+
+int ivae_layer_norm_workspace_bytes(const IvaeNorm* norm, size_t* out) {
+    if (!out) return IVAE_E_NULLPTR;
+    const int rc = check_norm(norm);
+    if (rc) return rc;
+    *out = norm_ws_bytes(norm->rows, norm->width);
+    return IVAE_OK;
+}
+
+int ivae_layer_norm(const IvaeNorm* norm, const void* x, const void* weight, const void* bias, void* y, float* stats, void* stream) {
+    const int rc = check_norm(norm);
+    if (rc) return rc;
+    if (norm->rows == 0) return IVAE_OK;
+    if (!x || !y) return IVAE_E_NULLPTR;
+    hipError_t e = launch_layer_norm(*norm, x, weight, bias, y, stats, (hipStream_t)stream);
+    return e == hipSuccess ? IVAE_OK : hip_fail(e, "ivae_layer_norm");
+}
+
+int ivae_layer_norm_backward(const IvaeNorm* norm, const void* dy, const void* x, const float* stats, const void* weight,
+                             const void* residual, void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+    const int rc = check_norm(norm);
+    if (rc) return rc;
+    if (norm->rows > 0 && (!dy || !x || !stats)) return IVAE_E_NULLPTR;
+    const size_t need = dweight || dbias ? norm_ws_bytes(norm->rows, norm->width) : 0;
+    if (need && !workspace) return IVAE_E_NULLPTR;
+    if (workspace_bytes < need) return IVAE_E_WORKSPACE;
+    if (!dx && !dweight && !dbias) return IVAE_OK;
+    hipError_t e = launch_layer_norm_backward(*norm, dy, x, stats, weight, residual, dx, dweight, dbias, (float*)workspace, (hipStream_t)stream);
+    return e == hipSuccess ? IVAE_OK : hip_fail(e, "ivae_layer_norm_backward");
+}
+
+int ivae_dropout(int32_t dtype, int64_t n, const void* x, const void* residual, void* y, double p, uint64_t seed, uint64_t offset,
+                 const int64_t* offset_device, void* stream) {
+    if (dtype < IVAE_F32 || dtype > IVAE_F16) return IVAE_E_BADTYPE;
+    if (n < 0 || !(p >= 0. && p <= 1.)) return IVAE_E_BADDIMS;
+    if (n == 0) return IVAE_OK;
+    if (!x || !y) return IVAE_E_NULLPTR;
+    hipError_t e = launch_dropout(dtype, n, x, residual, y, p, seed, offset, offset_device, (hipStream_t)stream);
+    return e == hipSuccess ? IVAE_OK : hip_fail(e, "ivae_dropout");
+}
+
 }  // extern "C"

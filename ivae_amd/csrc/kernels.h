@@ -46,6 +46,17 @@ size_t corr_ws_bytes(int64_t n, int d);
 hipError_t launch_corr_batched(const float* x, const float* y, int64_t n_blocks, int64_t n, int d, double* cc, hipStream_t st);
 hipError_t launch_corr_static(const float* x, const float* y, int64_t n, int d, double* cc, hipStream_t st);
 #define CORR_STATIC_MAX_D 40
+size_t linear_ws_bytes(const IvaeLinear& L, bool backward);
+hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, const void* b, const void* residual, void* y, void* saved,
+                         void* ws, hipStream_t st);
+hipError_t launch_linear_backward(const IvaeLinear& L, const void* dy, const void* x, const void* w, const void* saved, void* dx, void* dw,
+                                  void* db, void* ws, hipStream_t st);
+size_t norm_ws_bytes(int64_t rows, int width);
+hipError_t launch_layer_norm(const IvaeNorm& N, const void* x, const void* w, const void* b, void* y, float* stats, hipStream_t st);
+hipError_t launch_layer_norm_backward(const IvaeNorm& N, const void* dy, const void* x, const float* stats, const void* w, const void* residual,
+                                      void* dx, void* dw, void* db, float* ws, hipStream_t st);
+hipError_t launch_dropout(int dtype, int64_t n, const void* x, const void* residual, void* y, double p, uint64_t seed, uint64_t offset,
+                          const int64_t* offset_dev, hipStream_t st);
 
 // Dynamic LDS above 64 KB needs the function attribute.  hipFuncSetAttribute SETS the limit (it does not take a maximum),
 // and host threads may launch the same kernel with different sizes at the same moment (sweep.py trains one pack per

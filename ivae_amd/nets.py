@@ -13,6 +13,7 @@ from numbers import Number
 import numpy as np
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
 from . import ops
@@ -45,13 +46,96 @@ class Normal:
         return lpdf.sum(dim=-1) if reduce else lpdf
 
 
+def _no_capture(*tensors):
+    """The autograd engine synchronises the streams of a graph's leaves by itself, which a capture on another stream does not
+    survive: gradients under capture are the business of ``ops`` (``linear_backward`` and its siblings capture like any launch)."""
+    if any(t is not None and t.is_cuda for t in tensors) and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError('autograd through MLP operators cannot be captured into a graph: capture ivae_amd.ops calls instead')
+
+
+class _LinearFn(torch.autograd.Function):
+    """ops.linear with its gradients."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, activation, slope, residual):
+        save = any(ctx.needs_input_grad[:3])
+        if not save:
+            return ops.linear(x, weight, bias, activation, slope, residual)
+        _no_capture(x)
+        y, pre = ops.linear(x, weight, bias, activation, slope, residual, save=True)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.act = activation, slope
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _no_capture(dy)
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if any(need[:3]):
+            x, weight, pre = ctx.saved_tensors
+            dx, dw, db = ops.linear_backward(dy, x, weight, pre, *ctx.act, need=need[:3])
+        return dx, dw, db, None, None, dy if need[5] else None
+
+
+class _LayerNormFn(torch.autograd.Function):
+    """ops.layer_norm with its gradients."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        if not any(ctx.needs_input_grad[:3]):
+            return ops.layer_norm(x, weight, bias, eps)
+        _no_capture(x)
+        y, stats = ops.layer_norm(x, weight, bias, eps, save=True)
+        ctx.save_for_backward(x, weight, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _no_capture(dy)
+        x, weight, stats = ctx.saved_tensors
+        return (*ops.layer_norm_backward(dy, x, stats, weight, need=ctx.needs_input_grad[:3]), None)
+
+
+class _DropoutFn(torch.autograd.Function):
+    """ops.dropout with its gradients; the mask is drawn again in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, residual):
+        if any(ctx.needs_input_grad):
+            _no_capture(x)
+        ctx.draw = p, seed, offset
+        return ops.dropout(x, p, seed, offset, residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _no_capture(dy)
+        need = ctx.needs_input_grad
+        return ops.dropout_backward(dy, *ctx.draw) if need[0] else None, None, None, None, dy if need[4] else None
+
+
 class MLP(nn.Module):
     """Container with the reference's constructor and ``fc`` ModuleList (nets.py:66-107).
     Inside the fused models only its parameters are used; its own ``forward`` (plain torch
-    ops) exists for callers that evaluate a sub-network by itself."""
+    ops) exists for callers that evaluate a sub-network by itself.
 
-    def __init__(self, input_dim, output_dim, hidden_dim, n_layers, activation='none', slope=.1, device='cpu'):
+    ``layer_norm``, ``residual`` and ``dropout`` (no counterpart in the reference) turn the hidden layers into residual blocks,
+    ``h + dropout(act(fc(norm(h))))``: every layer but the first normalises its input (``norm.<layer - 1>``), the sum is taken where a
+    hidden layer's two widths agree, and dropout acts in training mode, its seed drawn from torch's CPU generator.  With any of
+    them the forward and backward passes run in the library's kernels (``ops.linear``, ``ops.layer_norm``, ``ops.dropout``) and need
+    a ROCm device; fp32, bf16 and fp16 parameters, and the activations 'gelu' and 'silu' besides the others."""
+
+    def __init__(self, input_dim, output_dim, hidden_dim, n_layers, activation='none', slope=.1, device='cpu', layer_norm=False,
+                 residual=False, dropout=0.):
         super().__init__()
+        if not 0. <= dropout <= 1.:
+            raise ValueError('dropout must be between 0 and 1: {}'.format(dropout))
+        self.residual = bool(residual)
+        self.dropout = float(dropout)
+        self.operators = bool(layer_norm or residual or dropout)
         self.input_dim = input_dim
         self.output_dim = output_dim
         self.n_layers = n_layers
@@ -70,10 +154,11 @@ class MLP(nn.Module):
         else:
             raise ValueError('Wrong argument type for activation: {}'.format(activation))
         for act in self.activation:
-            if act not in ops.ACT_IDS:
+            if act not in (ops.LINEAR_ACT_IDS if self.operators else ops.ACT_IDS):
                 raise ValueError('Incorrect activation: {}'.format(act))
         dims = [self.input_dim] + list(self.hidden_dim[:self.n_layers - 1]) + [self.output_dim]
         self.fc = nn.ModuleList([nn.Linear(dims[i], dims[i + 1]) for i in range(self.n_layers)])
+        self.norm = nn.ModuleList([nn.LayerNorm(d) for d in dims[1:-1]]) if layer_norm else None
         self.to(self.device)
 
     @staticmethod
@@ -89,7 +174,38 @@ class MLP(nn.Module):
             return torch.sigmoid(h)
         return h
 
+    def _forward_operators(self, x):
+        if not x.is_cuda:
+            raise RuntimeError('x must live on a ROCm device: ivae_amd has no CPU path')
+        drop = self.dropout if self.training else 0.
+        seed = 0
+        if drop:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('a captured MLP would draw the same dropout mask at every replay: call eval() first')
+            seed = int(torch.randint(2 ** 63 - 1, ()))
+        # (inside a Function the grad mode of its caller is not to be seen: without one nothing needs to be saved)
+        grad = torch.is_grad_enabled()
+        linear, layer_norm, drop_out = ((_LinearFn.apply, _LayerNormFn.apply, _DropoutFn.apply) if grad else
+                                        (ops.linear, ops.layer_norm, ops.dropout))
+        h = x
+        for c, fc in enumerate(self.fc):
+            t = h
+            if self.norm is not None and c:
+                n = self.norm[c - 1]
+                t = layer_norm(t, n.weight, n.bias, n.eps)
+            if c == self.n_layers - 1:
+                return linear(t, fc.weight, fc.bias, 'none', self.slope, None)
+            add = h if self.residual and fc.in_features == fc.out_features else None
+            if drop:
+                t = linear(t, fc.weight, fc.bias, self.activation[c], self.slope, None)
+                h = drop_out(t, drop, seed, c, add)
+            else:
+                h = linear(t, fc.weight, fc.bias, self.activation[c], self.slope, add)
+        return h
+
     def forward(self, x):
+        if self.operators:
+            return self._forward_operators(x)
         h = x
         for c in range(self.n_layers):
             h = self.fc[c](h)

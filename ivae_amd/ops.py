@@ -2,13 +2,14 @@
 stream; every computation below happens in libivae_amd.so's HIP kernels."""
 import contextlib
 import ctypes as C
+import functools
 import math
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import ACT_IDS, IvaeCoef, IvaeDims, IvaeWsLayout, check
+from ._lib import ACT_IDS, LINEAR_ACT_IDS, IvaeCoef, IvaeDims, IvaeLinear, IvaeNorm, IvaeWsLayout, check
 
 
 # Tuning of the shape-generic kernels (IvaeDims.tile_rows / waves / wgrad_rows); 0 = the library picks.  Host-side default
@@ -378,3 +379,222 @@ def train_steps(shape, coef, params, exp_avg, exp_avg_sq, x_data, u_data, batch_
                                           float(adam_eps), _ptr(loss), _ptr(z), _ptr(zs), _stream(dev)),
               "ivae_train_steps")
     return loss, (zs if want_z_steps else z)
+
+
+# ---- tensor operators of a residual MLP block -------------------------------------------------------------------------
+# linear, layer_norm and dropout with their backward passes, over (..., width) tensors of fp32, bf16 or fp16.  Like every call
+# above they run on the current stream of the inputs' device, record no autograd graph (ivae_amd.nets has the autograd side),
+# allocate their outputs, and raise on anything they do not serve.  All of them can be captured into a graph.
+
+DTYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_SAVED = (torch.float32, torch.float16, torch.float32)       # of linear's pre-activation, by type id
+
+
+def _dtype_id(t, name):
+    dt = DTYPE_IDS.get(t.dtype)
+    if dt is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on a ROCm device: ivae_amd has no CPU path")
+    return dt
+
+
+def _like(t, ref, name, shape=None, dtype=None):
+    """t, checked to have ref's type (or `dtype`) and device and the given shape."""
+    if t.dtype != (dtype or ref.dtype):
+        raise TypeError(f"{name} must be {dtype or ref.dtype}, got {t.dtype}")
+    if t.device != ref.device:
+        raise RuntimeError(f"{name} must live on {ref.device}, got {t.device}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _matrix(t):
+    """(t, row stride) of a (..., width) tensor as a matrix with unit column stride; copied only where its strides do not make one."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1):
+        return t, t.stride(0)
+    return t.contiguous(), t.shape[-1]
+
+
+def _call(dev, fn, what, *args):
+    """fn(*args, stream) with `dev` current."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        check(rc, what)
+
+
+def _opt(t):
+    return None if t is None else t.data_ptr()
+
+
+def _scratch(nbytes, dev):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_plan(rows, k, n, dt, act, slope, ldx, ldr, lddy, backward):
+    """(argument struct, workspace bytes) of a call: functions of the sizes alone."""
+    lin = IvaeLinear(rows, k, n, dt, act, slope, ldx, ldr, lddy)
+    nb = C.c_size_t()
+    check(_lib.lib().ivae_linear_workspace_bytes(C.byref(lin), backward, C.byref(nb)), "ivae_linear_workspace_bytes")
+    return lin, nb.value
+
+
+def _linear_shapes(x, weight, activation):
+    dt = _dtype_id(x, "x")
+    act = LINEAR_ACT_IDS.get(activation)
+    if act is None:
+        raise ValueError("Incorrect activation: {}".format(activation))
+    _like(weight, x, "weight")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x (..., in) and weight (out, in) do not fit: {tuple(x.shape)} and {tuple(weight.shape)}")
+    n, k = weight.shape
+    if n == 0 or k == 0:
+        raise ValueError("linear needs at least one input and one output feature")
+    return dt, act, x.numel() // k, k, n
+
+
+def linear(x, weight, bias=None, activation="none", slope=.1, residual=None, save=False):
+    """ivae_linear: act(x weight^T + bias) + residual, for x (..., in), weight (out, in), bias (out,), residual (..., out) of one
+    type; activation: none, lrelu (slope), xtanh (tanh(s) + slope s), sigmoid, gelu (the erf form), silu.
+    -> y, or with save=True (y, saved): saved is what linear_backward needs of the pre-activation, None for 'none'."""
+    dt, act, rows, k, n = _linear_shapes(x, weight, activation)
+    out = x.shape[:-1] + (n,)
+    if bias is not None:
+        bias = _like(bias, x, "bias", (n,)).contiguous()
+    x, ldx = _matrix(x)
+    weight = weight.contiguous()
+    ldr = 0
+    if residual is not None:
+        residual, ldr = _matrix(_like(residual, x, "residual", out))
+    dev = x.device
+    lin, nb = _linear_plan(rows, k, n, dt, act, float(slope), ldx, ldr, 0, 0)
+    y = torch.empty(out, dtype=x.dtype, device=dev)
+    saved = torch.empty(out, dtype=_SAVED[dt], device=dev) if save and act else None
+    ws = _scratch(nb, dev)
+    _call(dev, _lib.lib().ivae_linear, "ivae_linear", lin, x.data_ptr(), weight.data_ptr(), _opt(bias), _opt(residual), y.data_ptr(), _opt(saved),
+          _opt(ws), nb)
+    return (y, saved) if save else y
+
+
+def linear_backward(dy, x, weight, saved=None, activation="none", slope=.1, need=(True, True, True)):
+    """ivae_linear_backward: -> (dx, dweight, dbias), None where `need` says no.  `saved`: linear's, of the same x, weight and
+    activation.  The gradient of the residual is dy itself."""
+    dt, act, rows, k, n = _linear_shapes(x, weight, activation)
+    out = x.shape[:-1] + (n,)
+    _like(dy, x, "dy", out)
+    if act:
+        if saved is None:
+            raise ValueError("the backward pass of an activation needs linear's `saved` (save=True)")
+        saved = _like(saved, x, "saved", out, _SAVED[dt]).contiguous()
+    else:
+        saved = None
+    shape = x.shape
+    x, ldx = _matrix(x)
+    dy, lddy = _matrix(dy)
+    weight = weight.contiguous()
+    dev = x.device
+    lin, nb = _linear_plan(rows, k, n, dt, act, float(slope), ldx, 0, lddy, 1)
+    dx = torch.empty(shape, dtype=x.dtype, device=dev) if need[0] else None
+    dw = torch.empty((n, k), dtype=x.dtype, device=dev) if need[1] else None
+    db = torch.empty((n,), dtype=x.dtype, device=dev) if need[2] else None
+    ws = _scratch(nb, dev)
+    _call(dev, _lib.lib().ivae_linear_backward, "ivae_linear_backward", lin, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _opt(saved),
+          _opt(dx), _opt(dw), _opt(db), _opt(ws), nb)
+    return dx, dw, db
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_plan(rows, width, dt, weight_f32, eps, ldx, lddy, ldr):
+    norm = IvaeNorm(rows, width, dt, weight_f32, eps, ldx, lddy, ldr)
+    nb = C.c_size_t()
+    check(_lib.lib().ivae_layer_norm_workspace_bytes(C.byref(norm), C.byref(nb)), "ivae_layer_norm_workspace_bytes")
+    return norm, nb.value
+
+
+def _norm_shapes(x, weight, bias):
+    dt = _dtype_id(x, "x")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("layer_norm needs a last dimension of at least one element")
+    d = x.shape[-1]
+    wt = next((w.dtype for w in (weight, bias) if w is not None), x.dtype)
+    if wt not in (x.dtype, torch.float32):
+        raise TypeError(f"weight and bias must be {x.dtype} or float32, got {wt}")
+    if weight is not None:
+        weight = _like(weight, x, "weight", (d,), wt).contiguous()
+    if bias is not None:
+        bias = _like(bias, x, "bias", (d,), wt).contiguous()
+    return dt, x.numel() // d, d, wt, weight, bias
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, save=False):
+    """ivae_layer_norm over the last dimension; weight and bias (width,) in x's type or float32, or None.
+    -> y, or with save=True (y, stats): stats (2, rows) fp32 is what layer_norm_backward needs."""
+    dt, rows, d, wt, weight, bias = _norm_shapes(x, weight, bias)
+    shape = x.shape
+    x, ldx = _matrix(x)
+    dev = x.device
+    norm, _ = _norm_plan(rows, d, dt, int(wt == torch.float32), float(eps), ldx, 0, 0)
+    y = torch.empty(shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=dev) if save else None
+    _call(dev, _lib.lib().ivae_layer_norm, "ivae_layer_norm", norm, x.data_ptr(), _opt(weight), _opt(bias), y.data_ptr(), _opt(stats))
+    return (y, stats) if save else y
+
+
+def layer_norm_backward(dy, x, stats, weight=None, residual=None, need=(True, True, True)):
+    """ivae_layer_norm_backward: -> (dx [+ residual], dweight, dbias), None where `need` says no; dweight and dbias in the weight's
+    type (x's without a weight).  residual (like x): the gradient that arrives past the norm in a block x + f(norm(x))."""
+    dt, rows, d, wt, weight, _ = _norm_shapes(x, weight, None)
+    shape = x.shape
+    _like(dy, x, "dy", shape)
+    stats = _like(stats, x, "stats", (2, rows), torch.float32).contiguous()
+    x, ldx = _matrix(x)
+    dy, lddy = _matrix(dy)
+    ldr = 0
+    if residual is not None:
+        residual, ldr = _matrix(_like(residual, x, "residual", shape))
+    dev = x.device
+    norm, nb = _norm_plan(rows, d, dt, int(wt == torch.float32), 0., ldx, lddy, ldr)
+    dx = torch.empty(shape, dtype=x.dtype, device=dev) if need[0] else None
+    dw = torch.empty((d,), dtype=wt, device=dev) if need[1] else None
+    db = torch.empty((d,), dtype=wt, device=dev) if need[2] else None
+    ws = _scratch(nb, dev) if need[1] or need[2] else None
+    _call(dev, _lib.lib().ivae_layer_norm_backward, "ivae_layer_norm_backward", norm, dy.data_ptr(), x.data_ptr(), stats.data_ptr(), _opt(weight),
+          _opt(residual), _opt(dx), _opt(dw), _opt(db), _opt(ws), nb if ws is not None else 0)
+    return dx, dw, db
+
+
+def dropout(x, p, seed, offset=0, residual=None):
+    """ivae_dropout: x / (1 - p) where kept, 0 elsewhere, plus residual (like x).  The mask is a function of (seed, offset, element
+    number) and is not stored; give every call of a step another offset.  offset: an int, or an int64 tensor of one element on
+    x's device, read when the kernel runs (a captured graph then draws a new mask at every replay, if the graph or its owner
+    advances the tensor)."""
+    dt = _dtype_id(x, "x")
+    p = float(p)
+    if not 0. <= p <= 1.:
+        raise ValueError(f"p must be between 0 and 1, got {p}")
+    if residual is not None:
+        residual = _like(residual, x, "residual", x.shape).contiguous()
+    offset_dev = None
+    if isinstance(offset, torch.Tensor):
+        offset_dev = _like(offset, x, "offset", None, torch.int64)
+        if offset.numel() != 1:
+            raise ValueError("offset must be one number")
+        offset = 0
+    x = x.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _call(x.device, _lib.lib().ivae_dropout, "ivae_dropout", dt, x.numel(), x.data_ptr(), _opt(residual), y.data_ptr(), p,
+          int(seed) & (2 ** 64 - 1), int(offset) & (2 ** 64 - 1), _opt(offset_dev))
+    return y
+
+
+def dropout_backward(dy, p, seed, offset=0):
+    """The gradient of dropout's x: the same mask drawn again over dy.  (The gradient of the residual is dy itself.)"""
+    return dropout(dy, p, seed, offset)
