@@ -31,24 +31,45 @@ __device__ __forceinline__ f16_t pre_pack(float s, f16_t) {
     return s > 0.f && h == (f16_t)0.f ? (f16_t)5.9604645e-8f : h;
 }
 
+// Activations of 16-bit results from the hardware's exp2 and reciprocal (1 unit in the last place of 32 bits each): their errors are
+// at most 2e-7 next to steps of 2^-11 and more, and an epilogue of 128 values a lane costs a third of what the exact forms do.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ float fast_sigmoid(float s) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-s)); }
+__device__ __forceinline__ float fast_tanh(float s) {
+    const float a = fabsf(s), q = s * s;
+    const float near = s * (1.f + q * (-1.f / 3.f + q * (2.f / 15.f - q * (17.f / 315.f))));          // Taylor: 2e-10 at 0.1
+    const float far = copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(1.f + fast_exp(2.f * a)), s);
+    return a < 0.1f ? near : far;
+}
+// 1 + erf(x / sqrt 2) (twice the normal distribution): Abramowitz and Stegun 7.1.26, |error| <= 1.5e-7
+__device__ __forceinline__ float fast_cdf2(float s) {
+    const float a = fabsf(s) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * a);
+    const float tail = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * fast_exp(-a * a);
+    return s < 0.f ? tail : 2.f - tail;
+}
+template <typename T>
 __device__ __forceinline__ float lin_act(int act, float slope, float s) {
+    constexpr bool fast = sizeof(T) == 2;
     switch (act) {
         case IVAE_ACT_LRELU: return s > 0.f ? s : slope * s;
-        case IVAE_ACT_XTANH: return tanhf(s) + slope * s;
-        case IVAE_ACT_SIGMOID: return 1.f / (1.f + expf(-s));
-        case IVAE_ACT_GELU: return 0.5f * s * (1.f + erff(s * 0.70710678118654752f));
-        case IVAE_ACT_SILU: return s / (1.f + expf(-s));
+        case IVAE_ACT_XTANH: return (fast ? fast_tanh(s) : tanhf(s)) + slope * s;
+        case IVAE_ACT_SIGMOID: return fast ? fast_sigmoid(s) : 1.f / (1.f + expf(-s));
+        case IVAE_ACT_GELU: return 0.5f * s * (fast ? fast_cdf2(s) : 1.f + erff(s * 0.70710678118654752f));
+        case IVAE_ACT_SILU: return fast ? s * fast_sigmoid(s) : s / (1.f + expf(-s));
         default: return s;
     }
 }
+template <typename T>
 __device__ __forceinline__ float lin_act_slope(int act, float slope, float s) {
+    constexpr bool fast = sizeof(T) == 2;
     switch (act) {
         case IVAE_ACT_LRELU: return s > 0.f ? 1.f : slope;
-        case IVAE_ACT_XTANH: { const float t = tanhf(s); return (1.f - t * t) + slope; }
-        case IVAE_ACT_SIGMOID: { const float t = 1.f / (1.f + expf(-s)); return t * (1.f - t); }
+        case IVAE_ACT_XTANH: { const float t = fast ? fast_tanh(s) : tanhf(s); return (1.f - t * t) + slope; }
+        case IVAE_ACT_SIGMOID: { const float t = fast ? fast_sigmoid(s) : 1.f / (1.f + expf(-s)); return t * (1.f - t); }
         case IVAE_ACT_GELU:
-            return 0.5f * (1.f + erff(s * 0.70710678118654752f)) + s * expf(-0.5f * s * s) * 0.39894228040143268f;
-        case IVAE_ACT_SILU: { const float t = 1.f / (1.f + expf(-s)); return t * (1.f + s * (1.f - t)); }
+            return 0.5f * (fast ? fast_cdf2(s) : 1.f + erff(s * 0.70710678118654752f)) +
+                   s * (fast ? fast_exp(-0.5f * s * s) : expf(-0.5f * s * s)) * 0.39894228040143268f;
+        case IVAE_ACT_SILU: { const float t = fast ? fast_sigmoid(s) : 1.f / (1.f + expf(-s)); return t * (1.f + s * (1.f - t)); }
         default: return 1.f;
     }
 }
@@ -56,3 +77,12 @@ __device__ __forceinline__ float lin_act_slope(int act, float slope, float s) {
 hipError_t linear_small_forward(const LinArgs& A, int dtype, hipStream_t st);
 hipError_t linear_small_backward(const LinArgs& A, int dtype, hipStream_t st);
 size_t linear_small_ws(const LinArgs& A, bool backward);
+
+// sums of split parts: kx, kw of them where there are two or more, kb where there is one (db is not written before the join)
+struct LinParts { const float* x; const float* w; const float* b; int kx, kw, kb; };
+hipError_t linear_join_forward(const LinArgs& A, int splits, int dtype, hipStream_t st);
+hipError_t linear_join_backward(const LinArgs& A, const LinParts& J, int dtype, hipStream_t st);
+// fp32 tiles whose flag is set in any of the `splits` runs of flags, computed again from the tensors themselves
+struct LinMarks { const int* flags; int tile_p, tile_q, splits; };
+hipError_t linear_mend_forward(const LinArgs& A, const LinMarks& y, hipStream_t st);
+hipError_t linear_mend_backward(const LinArgs& A, const LinMarks& x, const LinMarks& w, hipStream_t st);

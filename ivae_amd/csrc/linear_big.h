@@ -1,0 +1,31 @@
+// Interface of the large-product kernels (linear_big.hip).
+#pragma once
+#include "linear.h"
+
+// One operand of a product C[p][q] = sum_r P(p, r) Q(q, r), in memory as a row-major 16-bit matrix.
+//   along = true:  (extent, R): the summed index runs along a row;   along = false: (R, extent): it runs down the rows
+// Rows start at multiples of 16 bytes and hold whole 16-byte groups; `limit` is the end of the stored values along R (a multiple
+// of 8 where `along`; values between R and limit are 0).  Split fp32: of every second 32 along R, Q has its sign turned.  `plane`: elements between the three parts of split fp32 values.
+struct BigOperand {
+    const void* base;
+    int64_t ld, extent, limit, plane;
+    bool along;
+};
+
+enum { EPI_FWD, EPI_STORE };
+
+struct BigProduct {
+    BigOperand P, Q;
+    int64_t p_end, q_end, R;    // size of C and of the sum
+    int epi;
+    void* out;                  // EPI_STORE: (p_end, q_end) of the output type
+    float* part;                // split sums: (splits, p_end, q_end)
+    int* nan_seen;              // split fp32: one flag a tile and split: 1 where a sum came out as NaN
+    int tile_p, tile_q;         // 16-bit types: 256 x 256 or 128 x 128; fp32: 256 x 128 or 128 x 128
+    int splits;
+    int64_t len;                // R of a split, a multiple of 64
+};
+
+int64_t big_tiles(const BigProduct& B);
+// T: type of the tensors (float: operands are split bf16)
+hipError_t big_launch(const BigProduct& B, const LinArgs& A, int dtype, hipStream_t st);

@@ -1,0 +1,424 @@
+// Large products of the linear operator on the matrix cores.
+//
+// Operands go from memory straight into LDS (buffer_load ... lds, 16 bytes a lane) in two buffers: the loads of a step are issued when
+// the step before begins to be multiplied, so that one barrier a step is enough.  An operand whose summed index runs along its rows
+// is read from LDS 16 bytes a lane; one whose summed index runs down its rows (the weight in dx, both operands of dw) is read with
+// ds_read_b64_tr_b16, which transposes 4 x 16 values on the way into the registers: no operand is ever transposed in memory.
+// LDS rows cannot be padded (a load fills them in lane order), so the 16-byte groups of a row are permuted instead, by an XOR with
+// bits of the row number that puts every 16 lanes (along) or every 8 groups of 32 bytes (down) on distinct banks.
+//
+// fp32 (k_big_split): x = x0 + x1 + x2 with bf16 parts cut off after 8 bits each (exact), and x y = x0 y0 + x0 y1 + x1 y0 + x1 y1 + x0 y2 +
+// x2 y0 up to 2^-23 |x y|: six products at 16 times the rate of the fp32 matrix instructions.  The bf16 matrix instructions round their
+// running sum downwards, by little but always the same way, and a column sum over such results would add that up; so every 32 of
+// the summed index start from zero, smallest products first, and are added to the sum by fp32 additions that round to nearest.
+// An infinity times a part that is 0 makes a NaN that fp32 would not: a tile with a NaN in it is marked, and computed again in
+// fp32 by the small kernel.
+#include "kernels.h"
+#include "linear_big.h"
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char* lds_ptr;
+
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+template <typename E> struct E8;
+template <> struct E8<bf16_t> { typedef bf16x8 t; };
+template <> struct E8<f16_t> { typedef f16x8 t; };
+
+__device__ const uint4 g_zeros = {0, 0, 0, 0};          // where lanes beyond the sum read
+
+// One operand's tile of B rows (along) or B columns (down) and BR (64 or 32) of the summed index.  THREADS x 16 bytes a load.
+template <int B, int BR, bool ALONG, int THREADS>
+struct Stage {
+    static constexpr int BYTES = B * BR * 2, LOADS = BYTES / (THREADS * 16), PER_ROW = (ALONG ? BR : B) / 8;
+    static_assert(BYTES % (THREADS * 16) == 0 && THREADS % PER_ROW == 0, "whole loads");
+    uint32_t voff[LOADS];       // bytes from the tile's corner
+    int row, col;               // of load 0, in elements; load j is j * (THREADS / PER_ROW) rows further
+    const char* corner;
+    int64_t step;               // bytes from one BR to the next
+
+    static __device__ __forceinline__ int swizzle(int row) {
+        if (ALONG) return BR == 64 ? row >> 1 & 7 : row >> 2 & 3;
+        return ((row & 3) | (row >> 1 & 4)) << 1 & (PER_ROW - 1);          // (row >> 1 & 4 is bit 3 of the row, moved to bit 2)
+    }
+
+    __device__ __forceinline__ void init(const BigOperand& O, int64_t e0, int64_t r0) {
+        const int t = threadIdx.x;
+        row = t / PER_ROW;
+        col = (t % PER_ROW ^ swizzle(row)) * 8;
+        if (ALONG) {
+            corner = (const char*)O.base + (e0 * O.ld + r0) * 2;
+            step = BR * 2;
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                int64_t e = row + j * (THREADS / PER_ROW);
+                if (e0 + e >= O.extent) e = O.extent - 1 - e0;             // rows past the end repeat the last one; their results are not stored
+                voff[j] = (uint32_t)((e * O.ld + col) * 2);
+            }
+        } else {
+            corner = (const char*)O.base + (r0 * O.ld + e0) * 2;
+            step = (int64_t)BR * O.ld * 2;
+            int64_t c = col;
+            if (e0 + c >= O.extent) c = O.extent - 8 - e0;
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) voff[j] = (uint32_t)(((row + j * (THREADS / PER_ROW)) * O.ld + c) * 2);
+        }
+    }
+    // all of BR lies inside the operand
+    __device__ __forceinline__ void load_full(uint32_t lds, int64_t advance) const {
+        const uint64_t a = (uint64_t)(corner + advance);
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        u32x4 rsrc;
+        rsrc.x = __builtin_amdgcn_readfirstlane((uint32_t)a);
+        rsrc.y = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) & 0xffffu;
+        rsrc.z = 0xffffffffu;
+        rsrc.w = 0x00020000u;
+        const uint32_t base = __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(base + j * THREADS * 16), "v"(voff[j]), "s"(rsrc)
+                         : "memory");
+    }
+    // `left` of the summed index remain: what lies beyond reads zeros
+    __device__ __forceinline__ void load_part(uint32_t lds, int64_t advance, int64_t left) const {
+        const uint32_t base = __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const bool in = ALONG ? col < left : row + j * (THREADS / PER_ROW) < left;
+            const char* p = in ? corner + advance + voff[j] : (const char*)&g_zeros;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base + j * THREADS * 16), "v"(p) : "memory");
+        }
+    }
+    // lane's address of fragment 0 of the 16 rows / columns from `base`, half k (32 of the summed index each)
+    static __device__ __forceinline__ int frag(int base, int k) {
+        const int l = threadIdx.x % 64, i = l % 16, g = l / 16;
+        if (ALONG) {
+            const int r = base + i;
+            return r * (BR * 2) + (((k * 4 + g) ^ swizzle(r)) << 4);
+        }
+        const int r = k * 32 + g * 8 + i / 4, c = base + i % 4 * 4;        // the first four of a lane group's eight rows
+        return r * (B * 2) + (((c >> 3) ^ swizzle(r)) << 4) + (c & 4) * 2;
+    }
+};
+
+template <typename E, int B, bool ALONG, int THREADS>
+__device__ __forceinline__ typename E8<E>::t read_frag(uint32_t lds, int off) {
+    if constexpr (ALONG) return *(const __attribute__((address_space(3))) typename E8<E>::t*)(uintptr_t)(lds + off);
+    else {
+        // rows +4: bit 2 of the row is in no swizzle, so the address is B * 8 bytes further
+        typedef __attribute__((address_space(3))) s16x4* p4;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(uintptr_t)(lds + off));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(uintptr_t)(lds + off + B * 8));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(typename E8<E>::t, v);
+    }
+}
+
+// 8 neighbouring values, `n` of them inside the matrix
+template <typename T> __device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+    constexpr int N = Wide<T>::N;
+#pragma unroll
+    for (int h = 0; h < 8 / N; ++h) {
+        float u[N];
+        load_some<T>(p + h * N, n - h * N, u);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[h * N + j] = u[j];
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
+    constexpr int N = Wide<T>::N;
+#pragma unroll
+    for (int h = 0; h < 8 / N; ++h) {
+        float u[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) u[j] = v[h * N + j];
+        store_some<T>(p + h * N, n - h * N, u);
+    }
+}
+// LDS of a block: two buffers of a step, and in the end 128 rows of sums (4 words of padding keep a column off one bank)
+static constexpr int big_lds(int step_bytes, int btq) { return 2 * step_bytes > 128 * (btq + 4) * 4 ? 2 * step_bytes : 128 * (btq + 4) * 4; }
+
+// Tiles in bands of 8 rows of tiles, neighbours in a band one after the other, and a contiguous run of them for each of the 8 dies
+// (blocks go to the dies in turn): a die's cache then serves the few operand strips that its run shares.
+struct Place { int64_t p0, q0, ra, rb; int split, tile; };
+template <int BTP, int BTQ> __device__ __forceinline__ Place place(const BigProduct& G) {
+    const int tp = (int)((G.p_end + BTP - 1) / BTP), tq = (int)((G.q_end + BTQ - 1) / BTQ), tiles = tp * tq, blocks = tiles * G.splits;
+    int b = blockIdx.x;
+    const int per = blocks / 8, extra = blocks % 8, die = b % 8;
+    b = die * per + (die < extra ? die : extra) + b / 8;
+    Place r;
+    r.split = b / tiles;
+    b -= r.split * tiles;
+    const int band = b / (8 * tq), in_band = b - band * 8 * tq, rows = tp - band * 8 < 8 ? tp - band * 8 : 8;
+    const int ip = band * 8 + in_band % rows, iq = in_band / rows;
+    r.tile = ip * tq + iq;
+    r.p0 = (int64_t)ip * BTP;
+    r.q0 = (int64_t)iq * BTQ;
+    r.ra = r.split * G.len;
+    r.rb = r.ra + G.len < G.R ? r.ra + G.len : G.R;
+    return r;
+}
+
+// The sums go through LDS, 128 rows of the tile at a time, so that what follows runs along whole rows: 16-byte loads of the residual
+// and stores of the results, side by side, and one copy of the code for them.
+template <typename T, int BTP, int BTQ, int WP, int WQ, int EPI, int FP, int FQ>
+__device__ __forceinline__ void finish(const BigProduct& G, const LinArgs& A, const Place& at0, const f32x4 (&acc)[FP][FQ], float* sums) {
+    constexpr int THREADS = WP * WQ * 64, HALVES = BTP / 128, LD = BTQ + 4, RW = 16 * FP / HALVES;      // RW rows of each row of waves
+    static_assert(WP * RW == 128 && FP % HALVES == 0, "128 rows a pass");
+    const int wave = threadIdx.x / 64, l = threadIdx.x % 64, wq = wave % WQ * (BTQ / WQ);
+    const int64_t Q = G.q_end;
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < FP / HALVES; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+                *(f32x4*)(sums + (wave / WQ * RW + i * 16 + l % 16) * LD + wq + j * 16 + l / 16 * 4) = acc[h * (FP / HALVES) + i][j];
+        __syncthreads();
+#pragma unroll 1
+        for (int c = threadIdx.x; c < 128 * (BTQ / 8); c += THREADS) {
+            const int row = c / (BTQ / 8), col = c % (BTQ / 8) * 8;
+            const int64_t p = at0.p0 + row / RW * (BTP / WP) + h * RW + row % RW, q = at0.q0 + col;
+            if (p >= G.p_end || q >= Q) continue;
+            const int n = Q - q < 8 ? (int)(Q - q) : 8;
+            float v[8];
+            load8(sums + row * LD + col, 8, v);
+            const int64_t at = p * Q + q;
+            if (G.splits > 1) {
+                store8(G.part + (int64_t)at0.split * G.p_end * Q + at, n, v);
+            } else if (EPI == EPI_FWD) {
+                typedef typename Pre<T>::t pre_t;
+                float u[8];
+                if (A.b) {
+                    load8((const T*)A.b + q, n, u);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += u[e];
+                }
+                if (A.pre) {
+                    struct __attribute__((packed, aligned(sizeof(pre_t)))) { pre_t e[8]; } s;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s.e[e] = pre_pack(v[e], pre_t());
+                    pre_t* to = (pre_t*)A.pre + at;
+                    if (n == 8) *(decltype(s)*)to = s;
+                    else
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (e < n) to[e] = s.e[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = lin_act<T>(A.act, A.slope, v[e]);
+                if (A.res) {
+                    load8((const T*)A.res + p * A.ldr + q, n, u);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += u[e];
+                }
+                store8((T*)A.y + at, n, v);
+            } else store8((T*)G.out + at, n, v);
+        }
+    }
+}
+
+// 16-bit types.  BT x BT tiles, WP x WQ waves, 64 of the summed index a step.
+template <typename T, int BT, int WP, int WQ, bool PA, bool QA, int EPI>
+__global__ __launch_bounds__(WP * WQ * 64, 2) void k_big(BigProduct G, LinArgs A) {
+    constexpr int THREADS = WP * WQ * 64, FP = BT / WP / 16, FQ = BT / WQ / 16, BR = 64;
+    typedef Stage<BT, BR, PA, THREADS> SP;
+    typedef Stage<BT, BR, QA, THREADS> SQ;
+    typedef typename E8<T>::t v8;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)smem;
+    constexpr int BUF = SP::BYTES + SQ::BYTES;
+    const Place at0 = place<BT, BT>(G);
+
+    SP sp;
+    SQ sq;
+    sp.init(G.P, at0.p0, at0.ra);
+    sq.init(G.Q, at0.q0, at0.ra);
+    const int wave = threadIdx.x / 64;
+    const int wp = wave / WQ * (BT / WP), wq = wave % WQ * (BT / WQ);
+    // the lane's fragment addresses: 16 rows (along) are 16 * BR * 2 bytes apart and keep the swizzle; 16 columns (down) are two
+    // 16-byte groups apart, which the swizzle permutes, so each has its own
+    int op[PA ? 1 : FP][2], oq[QA ? 1 : FQ][2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int i = 0; i < (PA ? 1 : FP); ++i) op[i][k] = SP::frag(wp + i * 16, k);
+#pragma unroll
+        for (int i = 0; i < (QA ? 1 : FQ); ++i) oq[i][k] = SP::BYTES + SQ::frag(wq + i * 16, k);
+    }
+
+    const int64_t steps = (at0.rb - at0.ra + BR - 1) / BR;
+    auto load = [&](int64_t s) {
+        const uint32_t at = lds0 + (int)(s & 1) * BUF;
+        const int64_t r = at0.ra + s * BR, end = at0.rb;
+        // a split ends at a multiple of BR or at R, so only R itself cuts a step short
+        const int64_t lp = (end < G.R ? end : PA ? G.P.limit : G.R) - r, lq = (end < G.R ? end : QA ? G.Q.limit : G.R) - r;
+        if (lp >= BR) sp.load_full(at, s * sp.step);
+        else sp.load_part(at, s * sp.step, lp);
+        if (lq >= BR) sq.load_full(at + SP::BYTES, s * sq.step);
+        else sq.load_part(at + SP::BYTES, s * sq.step, lq);
+    };
+
+    f32x4 acc[FP][FQ];
+#pragma unroll
+    for (int i = 0; i < FP; ++i)
+#pragma unroll
+        for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (steps > 0) load(0);
+    for (int64_t s = 0; s < steps; ++s) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                        // this step's operands are in LDS, and the other buffer has been read by all
+        if (s + 1 < steps) load(s + 1);
+        const uint32_t at = lds0 + (int)(s & 1) * BUF;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            v8 p[FP], q[FQ];
+#pragma unroll
+            for (int j = 0; j < FQ; ++j) q[j] = read_frag<T, BT, QA, THREADS>(at, QA ? oq[0][k] + j * 16 * BR * 2 : oq[QA ? 0 : j][k]);
+#pragma unroll
+            for (int i = 0; i < FP; ++i) p[i] = read_frag<T, BT, PA, THREADS>(at, PA ? op[0][k] + i * 16 * BR * 2 : op[PA ? 0 : i][k]);
+#pragma unroll
+            for (int i = 0; i < FP; ++i)
+#pragma unroll
+                for (int j = 0; j < FQ; ++j) acc[i][j] = mma(q[j], p[i], acc[i][j]);
+        }
+    }
+    finish<T, BT, BT, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
+}
+
+// fp32 in three bf16 parts.  BTP x BTQ tiles, 64 x 64 a wave, 32 of the summed index a step, all three parts of both operands in LDS:
+// six products for each pair of fragments that is read.
+template <int BTP, int BTQ, bool PA, bool QA, int EPI>
+__global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_big_split(BigProduct G, LinArgs A) {
+    constexpr int WP = BTP / 64, WQ = BTQ / 64, THREADS = WP * WQ * 64, BR = 32;
+    typedef Stage<BTP, BR, PA, THREADS> SP;
+    typedef Stage<BTQ, BR, QA, THREADS> SQ;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)smem;
+    constexpr int BUF = 3 * (SP::BYTES + SQ::BYTES);
+    const Place at0 = place<BTP, BTQ>(G);
+
+    SP sp;
+    SQ sq;
+    sp.init(G.P, at0.p0, at0.ra);
+    sq.init(G.Q, at0.q0, at0.ra);
+    const int wave = threadIdx.x / 64, wp = wave / WQ * 64, wq = wave % WQ * 64;
+    int op[PA ? 1 : 4], oq[QA ? 1 : 4];
+#pragma unroll
+    for (int i = 0; i < (PA ? 1 : 4); ++i) op[i] = SP::frag(wp + i * 16, 0);
+#pragma unroll
+    for (int i = 0; i < (QA ? 1 : 4); ++i) oq[i] = 3 * SP::BYTES + SQ::frag(wq + i * 16, 0);
+
+    const int64_t steps = (at0.rb - at0.ra + BR - 1) / BR;
+    auto load = [&](int64_t s) {
+        const uint32_t at = lds0 + (int)(s & 1) * BUF;
+        const int64_t r = at0.ra + s * BR, end = at0.rb;
+        const int64_t lp = (end < G.R ? end : PA ? G.P.limit : G.R) - r, lq = (end < G.R ? end : QA ? G.Q.limit : G.R) - r;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const int64_t ap = k * G.P.plane * 2 + s * sp.step, aq = k * G.Q.plane * 2 + s * sq.step;
+            if (lp >= BR) sp.load_full(at + k * SP::BYTES, ap);
+            else sp.load_part(at + k * SP::BYTES, ap, lp);
+            if (lq >= BR) sq.load_full(at + 3 * SP::BYTES + k * SQ::BYTES, aq);
+            else sq.load_part(at + 3 * SP::BYTES + k * SQ::BYTES, aq, lq);
+        }
+    };
+
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (steps > 0) load(0);
+    for (int64_t s = 0; s < steps; ++s) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (s + 1 < steps) load(s + 1);
+        const uint32_t at = lds0 + (int)(s & 1) * BUF;
+        const float sign = s & 1 ? -1.f : 1.f;                  // (a split starts at a multiple of 64)
+        bf16x8 p[3][4];
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                p[k][i] = read_frag<bf16_t, BTP, PA, THREADS>(at + k * SP::BYTES, PA ? op[0] + i * 16 * BR * 2 : op[PA ? 0 : i]);
+#pragma unroll
+        for (int jj = 0; jj < 4; jj += 2) {
+            bf16x8 q[3][2];
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    q[k][j] = read_frag<bf16_t, BTQ, QA, THREADS>(at + k * SQ::BYTES, QA ? oq[0] + (jj + j) * 16 * BR * 2 : oq[QA ? 0 : jj + j]);
+            f32x4 c[4][2];
+            constexpr int TP[6] = {0, 2, 1, 0, 1, 0}, TQ[6] = {2, 0, 1, 1, 0, 0};      // parts of the six products, smallest first
+#pragma unroll
+            for (int t = 0; t < 6; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) c[i][j] = mma(q[TQ[t]][j], p[TP[t]][i], t ? c[i][j] : f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][jj + j][e] = __fmaf_rn(c[i][j][e], sign, acc[i][jj + j][e]);
+        }
+    }
+
+    int nan = 0;                                // is there a NaN in what will be stored?
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) nan |= acc[i][j][e] != acc[i][j][e];
+    nan = __syncthreads_or(nan);
+    if (threadIdx.x == 0) {
+        const int64_t tiles = ((G.p_end + BTP - 1) / BTP) * ((G.q_end + BTQ - 1) / BTQ);
+        G.nan_seen[at0.split * tiles + at0.tile] = nan;
+    }
+    finish<float, BTP, BTQ, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
+}
+
+int64_t big_tiles(const BigProduct& B) { return ((B.p_end + B.tile_p - 1) / B.tile_p) * ((B.q_end + B.tile_q - 1) / B.tile_q); }
+
+template <typename F>
+static hipError_t go(F fn, int bytes, int threads, SmemCache& cache, const BigProduct& B, const LinArgs& A, hipStream_t st) {
+    const hipError_t e = set_smem((const void*)fn, bytes, cache);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(fn, dim3((unsigned)(big_tiles(B) * B.splits)), dim3(threads), bytes, st, B, A);
+    return hipGetLastError();
+}
+template <typename T, int BT, int WP, int WQ, bool PA, bool QA, int EPI>
+static hipError_t go16(const BigProduct& B, const LinArgs& A, hipStream_t st) {
+    static SmemCache cache;
+    return go(k_big<T, BT, WP, WQ, PA, QA, EPI>, big_lds(2 * BT * 64 * 2, BT), WP * WQ * 64, cache, B, A, st);
+}
+template <int BTP, int BTQ, bool PA, bool QA, int EPI>
+static hipError_t go32(const BigProduct& B, const LinArgs& A, hipStream_t st) {
+    static SmemCache cache;
+    return go(k_big_split<BTP, BTQ, PA, QA, EPI>, big_lds(3 * (BTP + BTQ) * 32 * 2, BTQ), BTP * BTQ / 64, cache, B, A, st);
+}
+template <typename T, int BT, int WP, int WQ>
+static hipError_t forms16(const BigProduct& B, const LinArgs& A, hipStream_t st) {
+    if (B.epi == EPI_FWD) return go16<T, BT, WP, WQ, true, true, EPI_FWD>(B, A, st);      // forward
+    if (B.P.along) return go16<T, BT, WP, WQ, true, false, EPI_STORE>(B, A, st);          // dx
+    return go16<T, BT, WP, WQ, false, false, EPI_STORE>(B, A, st);                        // dw
+}
+template <int BTP, int BTQ>
+static hipError_t forms32(const BigProduct& B, const LinArgs& A, hipStream_t st) {
+    if (B.epi == EPI_FWD) return go32<BTP, BTQ, true, true, EPI_FWD>(B, A, st);
+    if (B.P.along) return go32<BTP, BTQ, true, false, EPI_STORE>(B, A, st);
+    return go32<BTP, BTQ, false, false, EPI_STORE>(B, A, st);
+}
+hipError_t big_launch(const BigProduct& B, const LinArgs& A, int dtype, hipStream_t st) {
+    if (dtype == IVAE_F32) return B.tile_p == 256 ? forms32<256, 128>(B, A, st) : forms32<128, 128>(B, A, st);
+    if (dtype == IVAE_BF16) return B.tile_p == 256 ? forms16<bf16_t, 256, 2, 4>(B, A, st) : forms16<bf16_t, 128, 2, 2>(B, A, st);
+    return B.tile_p == 256 ? forms16<f16_t, 256, 2, 4>(B, A, st) : forms16<f16_t, 128, 2, 2>(B, A, st);
+}

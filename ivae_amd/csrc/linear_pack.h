@@ -1,0 +1,20 @@
+// Interface of linear_pack.hip.
+#pragma once
+#include "linear.h"
+
+enum { FLIP_NONE, FLIP_ROWS, FLIP_COLS };
+
+struct PackArgs {
+    const void* src;            // (rows, cols), row stride ld
+    const void* pre;            // or null: (rows, cols) saved pre-activations; the values become act'(pre) src
+    void* out;                  // or null: (rows, ldo) of the same type, or for fp32 three bf16 matrices `plane` elements apart
+    float* colsum;              // or null: (row blocks, cols) sums over the rows
+    int64_t rows, ld, ldo, plane;
+    int cols;
+    int act;
+    float slope;
+    int flip;                   // fp32: every second run of 32 rows (FLIP_ROWS) or columns (FLIP_COLS) with its sign turned
+    int group;                  // set by the launcher
+};
+int pack_row_blocks(int64_t rows, int64_t width);       // of a launch with ldo = width: rows of colsum
+hipError_t launch_pack(const PackArgs& P, int dtype, hipStream_t st);

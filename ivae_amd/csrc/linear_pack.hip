@@ -1,0 +1,111 @@
+// What a large product needs done to a matrix before it can be loaded 16 bytes at a time: rows brought to 16-byte boundaries,
+// fp32 cut into three bf16 parts, and in the backward pass the gradient of the pre-activation, ds = act'(s) dy, with its column
+// sums (db) taken on the way.  One read and one write of the matrix; a thread takes 8 neighbouring values of every row that its
+// group walks.
+#include "kernels.h"
+#include "linear_pack.h"
+
+// x = x0 + x1 + x2, 8 bits each, cut off rather than rounded: every part has x's sign and the first never overflows.  Infinities and
+// NaN are whole in the first part.
+__device__ __forceinline__ void cut(float x, bf16_t (&o)[3]) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const bool finite = (u & 0x7f800000u) != 0x7f800000u;
+    const uint32_t h0 = finite || (u & 0x007fffffu) == 0 ? u & 0xffff0000u : u | 0x00400000u;
+    const float r1 = finite ? x - __builtin_bit_cast(float, h0 & 0xffff0000u) : 0.f;
+    const uint32_t u1 = __builtin_bit_cast(uint32_t, r1) & 0xffff0000u;
+    const float r2 = r1 - __builtin_bit_cast(float, u1);
+    o[0] = __builtin_bit_cast(bf16_t, (uint16_t)(h0 >> 16));
+    o[1] = __builtin_bit_cast(bf16_t, (uint16_t)(u1 >> 16));
+    o[2] = __builtin_bit_cast(bf16_t, (uint16_t)(__builtin_bit_cast(uint32_t, r2) >> 16));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack(PackArgs A) {
+    typedef typename Pre<T>::t pre_t;
+    const int group = A.group;                          // threads that share a row of 8 * group values
+    const int col = (blockIdx.x * group + threadIdx.x % group) * 8, sub = threadIdx.x / group, subs = 256 / group;
+    float sum[8] = {};
+    const int left = A.cols - col;                      // <= 0: beyond the last value (the padding is zeros)
+    for (int64_t r = (int64_t)blockIdx.y * subs + sub; r < A.rows && col < A.ldo; r += (int64_t)gridDim.y * subs) {
+        float v[8], s[8];
+        const T* p = (const T*)A.src + r * A.ld + col;
+        constexpr int N = Wide<T>::N;
+#pragma unroll
+        for (int h = 0; h < 8 / N; ++h) {
+            float u[N];
+            if (left - h * N >= N) load_wide<T>(p + h * N, u);
+            else load_part<T>(p + h * N, left - h * N, u);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[h * N + j] = u[j];
+        }
+        if (A.pre) {
+            const pre_t* q = (const pre_t*)A.pre + r * A.cols + col;
+            constexpr int NP = Wide<pre_t>::N;
+#pragma unroll
+            for (int h = 0; h < 8 / NP; ++h) {
+                float u[NP];
+                if (left - h * NP >= NP) load_wide<pre_t>(q + h * NP, u);
+                else load_part<pre_t>(q + h * NP, left - h * NP, u);
+#pragma unroll
+                for (int j = 0; j < NP; ++j) s[h * NP + j] = u[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= lin_act_slope<T>(A.act, A.slope, s[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += v[j];
+        if (!A.out) continue;
+        const int64_t at = r * A.ldo + col;
+        if constexpr (sizeof(T) == 2) {
+            store_wide<T>((T*)A.out + at, v);
+        } else {
+            if (A.flip != FLIP_NONE && ((A.flip == FLIP_ROWS ? (int)(r >> 5) : col >> 5) & 1))
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = -v[j];
+            struct __attribute__((aligned(16))) V { bf16_t e[8]; } part[3];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                bf16_t o[3];
+                cut(v[j], o);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) part[k].e[j] = o[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 3; ++k) *(V*)((bf16_t*)A.out + k * A.plane + at) = part[k];
+        }
+    }
+    if (!A.colsum) return;
+    __shared__ float fold[256][9];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) fold[threadIdx.x][j] = sum[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < group * 8; i += 256) {
+        float s = 0.f;
+        for (int k = 0; k < subs; ++k) s += fold[k * group + i / 8][i % 8];
+        const int c = blockIdx.x * group * 8 + i;
+        if (c < A.cols) A.colsum[(int64_t)blockIdx.y * A.cols + c] = s;
+    }
+}
+
+static int group_of(int64_t width) {                    // a power of two: 8 * group values cover a row, or 512 of it
+    int g = 1;
+    while (g < 64 && g * 8 < width) g *= 2;
+    return g;
+}
+// blocks along the rows: about 2048 blocks in all, 8 rows a thread at least
+int pack_row_blocks(int64_t rows, int64_t width) {
+    const int g = group_of(width);
+    const int64_t strips = (width + g * 8 - 1) / (g * 8), subs = 256 / g;
+    int64_t y = (rows + subs * 8 - 1) / (subs * 8), most = 2048 / strips;
+    if (y > most) y = most;
+    return (int)(y < 1 ? 1 : y);
+}
+hipError_t launch_pack(const PackArgs& P, int dtype, hipStream_t st) {
+    PackArgs A = P;
+    A.group = group_of(A.ldo);
+    const dim3 g((unsigned)((A.ldo + A.group * 8 - 1) / (A.group * 8)), (unsigned)pack_row_blocks(A.rows, A.ldo)), b(256);
+    if (dtype == IVAE_F32) hipLaunchKernelGGL(k_pack<float>, g, b, 0, st, A);
+    else if (dtype == IVAE_BF16) hipLaunchKernelGGL(k_pack<bf16_t>, g, b, 0, st, A);
+    else hipLaunchKernelGGL(k_pack<f16_t>, g, b, 0, st, A);
+    return hipGetLastError();
+}

@@ -116,7 +116,7 @@ template <typename T>
 __device__ __forceinline__ void forward_store(const LinArgs& A, int64_t m, int n, float s) {
     if (A.b) s += to_f(((const T*)A.b)[n]);
     if (A.pre) ((typename Pre<T>::t*)A.pre)[m * A.N + n] = pre_pack(s, typename Pre<T>::t());
-    s = lin_act(A.act, A.slope, s);
+    s = lin_act<T>(A.act, A.slope, s);
     if (A.res) s += to_f(((const T*)A.res)[m * A.ldr + n]);
     ((T*)A.y)[m * A.N + n] = from_f<T>(s);
 }
@@ -147,7 +147,7 @@ __device__ __forceinline__ void tile_product(const LinArgs& A, const LinSplit& S
                 float s[8];
                 fetch_tile<pre_t, RC>(pre, A.N, p0, P, r0, rb, s);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) vp[j] *= lin_act_slope(A.act, A.slope, s[j]);
+                for (int j = 0; j < 8; ++j) vp[j] *= lin_act_slope<T>(A.act, A.slope, s[j]);
             }
             if (MODE == MODE_DW)
 #pragma unroll
@@ -229,14 +229,61 @@ __global__ __launch_bounds__(256) void k_linear_join_fwd(LinArgs A, int splits) 
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
         forward_store<T>(A, i / A.N, (int)(i % A.N), join(A.part, splits, n, i));
 }
-template <typename T>
-__global__ __launch_bounds__(256) void k_linear_join_bwd(LinArgs A, int sx, int sw, const float* part_w, const float* part_b) {
-    const int64_t nx = sx > 1 ? A.M * A.K : 0, nw = sw > 1 && A.dw ? (int64_t)A.N * A.K : 0, nb = sw > 1 && A.db ? A.N : 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nx + nw + nb; i += (int64_t)gridDim.x * 256) {
-        if (i < nx) ((T*)A.dx)[i] = from_f<T>(join(A.part, sx, nx, i));
-        else if (i < nx + nw) ((T*)A.dw)[i - nx] = from_f<T>(join(part_w, sw, nw, i - nx));
-        else ((T*)A.db)[i - nx - nw] = from_f<T>(join(part_b, sw, nb, i - nx - nw));
+// db is a sum over up to hundreds of parts of a few thousand columns: its blocks (the first ones) take 64 columns each, four walks
+// over the parts side by side, eight loads in flight
+__device__ __forceinline__ float join_walk(const float* part, int k, int64_t n, int64_t i, int w) {
+    float s = 0.f;
+    int j = w;
+    for (; j + 28 < k; j += 32) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = part[(j + e * 4) * n + i];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += v[e];
     }
+    for (; j < k; j += 4) s += part[j * n + i];
+    return s;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_join_bwd(LinArgs A, LinParts J) {
+    const int64_t nx = J.kx > 1 ? A.M * A.K : 0, nw = J.kw > 1 ? (int64_t)A.N * A.K : 0, nb = J.kb > 0 ? (A.N + 63) / 64 : 0;
+    if (blockIdx.x < nb) {
+        __shared__ float fold[4][64];
+        const int l = threadIdx.x % 64, w = threadIdx.x / 64;
+        const int64_t i = (int64_t)blockIdx.x * 64 + l;
+        fold[w][l] = i < A.N ? join_walk(J.b, J.kb, A.N, i, w) : 0.f;
+        __syncthreads();
+        if (w == 0 && i < A.N) ((T*)A.db)[i] = from_f<T>((fold[0][l] + fold[1][l]) + (fold[2][l] + fold[3][l]));
+        return;
+    }
+    for (int64_t i = (int64_t)(blockIdx.x - nb) * 256 + threadIdx.x; i < nx + nw; i += (int64_t)(gridDim.x - nb) * 256) {
+        if (i < nx) ((T*)A.dx)[i] = from_f<T>(join(J.x, J.kx, nx, i));
+        else ((T*)A.dw)[i - nx] = from_f<T>(join(J.w, J.kw, nw, i - nx));
+    }
+}
+
+// The marked tiles of a large fp32 product: a block takes one of them in 64 x 64 parts.
+template <int MODE>
+__device__ __forceinline__ void mend(const LinArgs& A, const LinMarks& K, int64_t P, int64_t Q, int64_t R, int64_t b, float* lp, float* lq) {
+    const int64_t tp = (P + K.tile_p - 1) / K.tile_p, tq = (Q + K.tile_q - 1) / K.tile_q;
+    int marked = 0;
+    for (int k = 0; k < K.splits; ++k) marked |= K.flags[k * tp * tq + b];
+    if (!marked) return;
+    const LinSplit S = {(P + TP - 1) / TP, (Q + TQ - 1) / TQ, 1, (R + TR - 1) / TR * TR};
+    const int64_t i0 = b / tq * (K.tile_p / TP), j0 = b % tq * (K.tile_q / TQ);
+    for (int64_t i = i0; i < i0 + K.tile_p / TP && i < S.tp; ++i)
+        for (int64_t j = j0; j < j0 + K.tile_q / TQ && j < S.tq; ++j) tile_product<float, MODE>(A, S, i * S.tq + j, nullptr, nullptr, lp, lq, nullptr, nullptr);
+}
+__global__ __launch_bounds__(256) void k_linear_mend_fwd(LinArgs A, LinMarks y) {
+    __shared__ __attribute__((aligned(16))) float lp[TP * Lds<float>::LD];
+    __shared__ __attribute__((aligned(16))) float lq[TQ * Lds<float>::LD];
+    mend<MODE_FWD>(A, y, A.M, A.N, A.K, blockIdx.x, lp, lq);
+}
+__global__ __launch_bounds__(256) void k_linear_mend_bwd(LinArgs A, LinMarks x, int64_t nx, LinMarks w) {
+    __shared__ __attribute__((aligned(16))) float lp[TP * Lds<float>::LD];
+    __shared__ __attribute__((aligned(16))) float lq[TQ * Lds<float>::LD];
+    if (blockIdx.x < nx) mend<MODE_DX>(A, x, A.M, A.K, A.N, blockIdx.x, lp, lq);
+    else mend<MODE_DW>(A, w, A.N, A.K, A.M, blockIdx.x - nx, lp, lq);
 }
 
 static LinSplit split_of(int64_t P, int64_t Q, int64_t R) {
@@ -277,31 +324,64 @@ size_t linear_small_ws(const LinArgs& A, bool backward) {
 
 static unsigned cap(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20); }
 
+hipError_t linear_join_forward(const LinArgs& A, int splits, int dtype, hipStream_t st) {
+    if (splits < 2) return hipSuccess;
+    const dim3 g(cap((A.M * A.N + 255) / 256)), b(256);
+    if (dtype == IVAE_F32) hipLaunchKernelGGL(k_linear_join_fwd<float>, g, b, 0, st, A, splits);
+    else if (dtype == IVAE_BF16) hipLaunchKernelGGL(k_linear_join_fwd<bf16_t>, g, b, 0, st, A, splits);
+    else hipLaunchKernelGGL(k_linear_join_fwd<f16_t>, g, b, 0, st, A, splits);
+    return hipGetLastError();
+}
+hipError_t linear_join_backward(const LinArgs& A, const LinParts& J0, int dtype, hipStream_t st) {
+    LinParts J = J0;
+    if (!A.dx) J.kx = 0;
+    if (!A.dw) J.kw = 0;
+    if (!A.db) J.kb = 0;
+    const int64_t n = (J.kx > 1 ? A.M * A.K : 0) + (J.kw > 1 ? (int64_t)A.N * A.K : 0);
+    const unsigned blocks = cap((n + 255) / 256) + (J.kb > 0 ? (unsigned)((A.N + 63) / 64) : 0);
+    if (blocks == 0) return hipSuccess;
+    const dim3 g(blocks), b(256);
+    if (dtype == IVAE_F32) hipLaunchKernelGGL(k_linear_join_bwd<float>, g, b, 0, st, A, J);
+    else if (dtype == IVAE_BF16) hipLaunchKernelGGL(k_linear_join_bwd<bf16_t>, g, b, 0, st, A, J);
+    else hipLaunchKernelGGL(k_linear_join_bwd<f16_t>, g, b, 0, st, A, J);
+    return hipGetLastError();
+}
+static int64_t mend_tiles(int64_t P, int64_t Q, const LinMarks& K) { return ((P + K.tile_p - 1) / K.tile_p) * ((Q + K.tile_q - 1) / K.tile_q); }
+hipError_t linear_mend_forward(const LinArgs& A, const LinMarks& y, hipStream_t st) {
+    hipLaunchKernelGGL(k_linear_mend_fwd, dim3((unsigned)mend_tiles(A.M, A.N, y)), dim3(256), 0, st, A, y);
+    return hipGetLastError();
+}
+hipError_t linear_mend_backward(const LinArgs& A, const LinMarks& x, const LinMarks& w, hipStream_t st) {
+    const int64_t nx = A.dx ? mend_tiles(A.M, A.K, x) : 0, nw = A.dw ? mend_tiles(A.N, A.K, w) : 0;
+    LinArgs B = A;
+    B.db = nullptr;                                             // (its sums are fp32 already)
+    if (nx + nw) hipLaunchKernelGGL(k_linear_mend_bwd, dim3((unsigned)(nx + nw)), dim3(256), 0, st, B, x, nx, w);
+    return hipGetLastError();
+}
+
 template <typename T> static void fwd(const LinArgs& A, hipStream_t st) {
     const LinSplit S = split_of(A.M, A.N, A.K);
     hipLaunchKernelGGL(k_linear_fwd<T>, dim3(cap(S.tp * S.tq * S.splits)), dim3(256), 0, st, A, S);
-    if (S.splits > 1) hipLaunchKernelGGL(k_linear_join_fwd<T>, dim3(cap((A.M * A.N + 255) / 256)), dim3(256), 0, st, A, S.splits);
 }
 hipError_t linear_small_forward(const LinArgs& A, int dtype, hipStream_t st) {
     if (dtype == IVAE_F32) fwd<float>(A, st);
     else if (dtype == IVAE_BF16) fwd<bf16_t>(A, st);
     else fwd<f16_t>(A, st);
-    return hipGetLastError();
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : linear_join_forward(A, split_of(A.M, A.N, A.K).splits, dtype, st);
 }
-template <typename T> static void bwd(const LinArgs& A, hipStream_t st) {
+template <typename T> static void bwd(const LinArgs& A, const BwdPlan& p, float* pw, float* pb, hipStream_t st) {
+    const int64_t tiles = p.X.tp * p.X.tq * p.X.splits + p.W.tp * p.W.tq * p.W.splits;
+    if (tiles) hipLaunchKernelGGL(k_linear_bwd<T>, dim3(cap(tiles)), dim3(256), 0, st, A, p.X, p.W, pw, pb);
+}
+hipError_t linear_small_backward(const LinArgs& A, int dtype, hipStream_t st) {
     const BwdPlan p = plan_bwd(A);
     float* pw = A.part ? A.part + p.off_w : nullptr;
     float* pb = A.part ? A.part + p.off_b : nullptr;
-    const int64_t tiles = p.X.tp * p.X.tq * p.X.splits + p.W.tp * p.W.tq * p.W.splits;
-    if (tiles == 0) return;
-    hipLaunchKernelGGL(k_linear_bwd<T>, dim3(cap(tiles)), dim3(256), 0, st, A, p.X, p.W, pw, pb);
-    const int sx = A.dx ? p.X.splits : 1, sw = p.W.tq ? p.W.splits : 1;
-    const int64_t n = (sx > 1 ? A.M * A.K : 0) + (sw > 1 ? (int64_t)A.N * A.K + A.N : 0);
-    if (n) hipLaunchKernelGGL(k_linear_join_bwd<T>, dim3(cap((n + 255) / 256)), dim3(256), 0, st, A, sx, sw, pw, pb);
-}
-hipError_t linear_small_backward(const LinArgs& A, int dtype, hipStream_t st) {
-    if (dtype == IVAE_F32) bwd<float>(A, st);
-    else if (dtype == IVAE_BF16) bwd<bf16_t>(A, st);
-    else bwd<f16_t>(A, st);
-    return hipGetLastError();
+    if (dtype == IVAE_F32) bwd<float>(A, p, pw, pb, st);
+    else if (dtype == IVAE_BF16) bwd<bf16_t>(A, p, pw, pb, st);
+    else bwd<f16_t>(A, p, pw, pb, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    return linear_join_backward(A, {A.part, pw, pb, p.X.splits, p.W.splits, p.W.splits > 1 ? p.W.splits : 0}, dtype, st);
 }

@@ -277,20 +277,33 @@ __global__ __launch_bounds__(256) void k_norm_cols_wide(NormArgs A) {
     if (w < 2 && i < A.D) A.part[((int64_t)blockIdx.y * 2 + w) * A.D + i] = fold[w][0][l] + fold[w][1][l] + fold[w][2][l] + fold[w][3][l];
 }
 
-// dg, dc from the blocks' sums: 64 columns a block, four interleaved walks over the blocks, joined in a fixed order
+// dg, dc from the blocks' sums: 32 columns a block, 32 interleaved walks over the blocks with eight loads in flight, joined in a fixed order
 template <typename T>
-__global__ __launch_bounds__(256) void k_norm_join(const float* part, int blocks, int D, int w_f32, void* dg, void* dc) {
-    __shared__ float fold[4][64];
-    const int l = threadIdx.x % 64, w = threadIdx.x / 64, i = blockIdx.x * 64 + l;
+__global__ __launch_bounds__(1024) void k_norm_join(const float* part, int blocks, int D, int w_f32, void* dg, void* dc) {
+    __shared__ float fold[32][33];
+    const int l = threadIdx.x % 32, w = threadIdx.x / 32, i = blockIdx.x * 32 + l;
     void* out = blockIdx.y ? dc : dg;
     if (!out) return;
     float s = 0.f;
-    if (i < D)
-        for (int b = w; b < blocks; b += 4) s += part[((int64_t)b * 2 + blockIdx.y) * D + i];
+    if (i < D) {
+        const float* p = part + (int64_t)blockIdx.y * D + i;
+        int b = w;
+        for (; b + 7 * 32 < blocks; b += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = p[(int64_t)(b + e * 32) * 2 * D];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += v[e];
+        }
+        for (; b < blocks; b += 32) s += p[(int64_t)b * 2 * D];
+    }
     fold[w][l] = s;
     __syncthreads();
-    if (w || i >= D) return;
-    s = fold[0][l] + fold[1][l] + fold[2][l] + fold[3][l];
+    if (w >= 1) return;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) s += fold[k][l];
+    if (i >= D) return;
     if (w_f32) ((float*)out)[i] = s;
     else ((T*)out)[i] = from_f<T>(s);
 }
@@ -346,7 +359,7 @@ static void norm_bwd(const NormArgs& A, int blocks, void* dg, void* dc, hipStrea
         else if (tpr == 256) hipLaunchKernelGGL((k_norm_bwd<T, 256>), g, dim3(256), 0, st, A);
         else hipLaunchKernelGGL((k_norm_bwd<T, 1024>), g, dim3(1024), 0, st, A);
     }
-    if (dg || dc) hipLaunchKernelGGL(k_norm_join<T>, dim3((A.D + 63) / 64, 2), dim3(256), 0, st, A.part, blocks, A.D, A.w_f32, dg, dc);
+    if (dg || dc) hipLaunchKernelGGL(k_norm_join<T>, dim3((A.D + 31) / 32, 2), dim3(1024), 0, st, A.part, blocks, A.D, A.w_f32, dg, dc);
 }
 hipError_t launch_layer_norm_backward(const IvaeNorm& N, const void* dy, const void* x, const float* stats, const void* w, const void* residual,
                                       void* dx, void* dg, void* dc, float* ws, hipStream_t st) {

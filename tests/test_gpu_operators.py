@@ -96,6 +96,82 @@ def test_linear_long_sums(dt, m, k, n):
     run_linear(dt, m, k, n, "gelu", seed=m)
 
 
+# large products: whole tiles, ragged in every direction, summed dimensions that end inside a step, few tiles with long sums
+BIG = [(1024, 512, 512), (520, 768, 648), (777, 1001, 531), (64, 4104, 1000), (4100, 64, 1024), (1030, 1024, 264), (70, 72, 60000), (70, 60000, 72), (2050, 520, 1100)]
+
+
+@pytest.mark.parametrize("m,k,n", BIG)
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_linear_large(dt, m, k, n):
+    run_linear(dt, m, k, n, "gelu", seed=m + 1)
+
+
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_linear_large_forms(dt):
+    run_linear(dt, 640, 704, 648, "none", res=False, bias=False, seed=1)
+    run_linear(dt, 640, 704, 648, "lrelu", layout="strided", seed=2)
+    run_linear(dt, 640, 700, 650, "none", layout="transposed", seed=3)
+    full = run_linear(dt, 640, 704, 648, "xtanh", seed=4)
+    for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True)):
+        part = run_linear(dt, 640, 704, 648, "xtanh", seed=4, need=need)
+        assert all(b is None or torch.equal(a, b) for a, b in zip(full[-1], part[-1]))
+
+
+def test_linear_large_rows_past_the_last_are_left_alone():
+    """Results are written to (rows, out) exactly: what lies behind them in the same allocation keeps its values."""
+    from ivae_amd import _lib
+    m, k, n = 515, 1024, 513
+    x, w = torch.randn(m, k, device=dev()), torch.randn(n, k, device=dev())
+    for dt, code in ((F32, 0), (BF16, 1)):
+        X, W = x.to(dt), w.to(dt)
+        buf = torch.full((m * n + 4096,), 7.0, device=dev(), dtype=dt)
+        lin, nb = ops._linear_plan(m, k, n, code, 0, .1, k, 0, 0, 0)
+        ws = torch.empty(nb + 256, dtype=torch.uint8, device=dev())
+        ws[nb:] = 7
+        assert _lib.lib().ivae_linear(lin, X.data_ptr(), W.data_ptr(), None, None, buf.data_ptr(), None, ws.data_ptr(), nb,
+                                      torch.cuda.current_stream().cuda_stream) == 0
+        assert bool((buf[m * n:] == 7).all()) and bool((ws[nb:] == 7).all())
+        R.close(buf[:m * n].view(m, n), R.linear64(X.cpu(), W.cpu(), None, "none", None)["y"], "y")
+
+
+@pytest.mark.parametrize("dt", R.DTYPES)
+@pytest.mark.parametrize("m,k,n", [(600, 1024, 520), (64, 8192, 520)])
+def test_linear_large_keeps_nan_and_infinities(dt, m, k, n):
+    g = torch.Generator().manual_seed(12)
+    x, w, b, dy = normal(g, m, k, dtype=dt), normal(g, n, k, scale=.03, dtype=dt), normal(g, n, dtype=dt), normal(g, m, n, dtype=dt)
+    want = R.linear64(x, w, b, "none", None, dy)
+    x[1, 3], x[2, 0], w[4, 7], dy[5, 6] = float("nan"), float("inf"), float("inf"), -float("inf")
+    y = ops.linear(on(x), on(w), on(b)).cpu()
+    rows, cols = torch.tensor([i for i in range(m) if i not in (1, 2)]), torch.tensor([j for j in range(n) if j != 4])
+    R.close(y[rows][:, cols], tuple(v[rows][:, cols] for v in want["y"]), "finite part")
+    assert torch.isnan(y[1]).all()
+    s = torch.where(w[:, 0].double() > 0, float("inf"), -float("inf"))
+    assert torch.equal(y[2, cols].double(), s[cols])
+    inf4 = torch.where(x[rows, 7].double() > 0, float("inf"), -float("inf"))
+    assert torch.equal(y[rows, 4].double(), inf4)
+    dx, dw, db = (t.cpu() for t in ops.linear_backward(on(dy), on(x), on(w)))
+    rows2 = torch.tensor([i for i in range(m) if i != 5])
+    ok = torch.tensor([j for j in range(k) if j != 7])                     # (column 7 meets the weight's infinity)
+    R.close(dx[rows2][:, ok], tuple(v[rows2][:, ok] for v in want["dx"]), "dx")
+    s = torch.where(w[6].double() > 0, -float("inf"), float("inf"))
+    assert torch.equal(dx[5, ok].double(), s[ok])
+    okw = torch.tensor([j for j in range(k) if j not in (0, 3)])
+    rw = torch.tensor([j for j in range(n) if j != 6])
+    R.close(dw[rw][:, okw], tuple(v[rw][:, okw] for v in want["dw"]), "dw")
+    assert torch.isnan(dw[:, 3]).all() and not torch.isfinite(dw[6]).any()
+    assert float(db[6]) == -float("inf")
+
+
+def test_linear_fp32_range():
+    """The three parts of a value keep its range: products near both ends of fp32's."""
+    g = torch.Generator().manual_seed(13)
+    x, w = normal(g, 512, 1024), normal(g, 512, 1024)
+    for sx, sw in ((2.0 ** 100, 2.0 ** -100), (2.0 ** -60, 2.0 ** -40), (2.0 ** 60, 2.0 ** 50)):
+        y = ops.linear(on(x * sx), on(w * sw))
+        v, bound = R.linear64(x * sx, w * sw, None, "none", None)["y"]
+        R.close(y, (v, bound), (sx, sw))
+
+
 def test_linear_leading_dimensions_and_empty():
     g = torch.Generator().manual_seed(8)
     x, w, b = normal(g, 2, 3, 5, 24), normal(g, 10, 24), normal(g, 10)
