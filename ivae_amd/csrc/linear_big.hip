@@ -38,7 +38,7 @@ struct Stage {
     int64_t step;               // bytes from one BR to the next
 
     static __device__ __forceinline__ int swizzle(int row) {
-        if (ALONG) return BR == 64 ? row >> 1 & 7 : row >> 2 & 3;
+        if (ALONG) return BR == 64 ? row >> 1 & 7 : -(row >> 2) & 3;
         return ((row & 3) | (row >> 1 & 4)) << 1 & (PER_ROW - 1);          // (row >> 1 & 4 is bit 3 of the row, moved to bit 2)
     }
 
@@ -89,15 +89,17 @@ struct Stage {
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base + j * THREADS * 16), "v"(p) : "memory");
         }
     }
-    // lane's address of fragment 0 of the 16 rows / columns from `base`, half k (32 of the summed index each)
-    static __device__ __forceinline__ int frag(int base, int k) {
+    // lane's address in the fragment of the 16 rows / columns from `base` (a multiple of 64) in the first 32 of the summed index
+    static __device__ __forceinline__ int frag(int base) {
         const int l = threadIdx.x % 64, i = l % 16, g = l / 16;
-        if (ALONG) {
-            const int r = base + i;
-            return r * (BR * 2) + (((k * 4 + g) ^ swizzle(r)) << 4);
-        }
-        const int r = k * 32 + g * 8 + i / 4, c = base + i % 4 * 4;        // the first four of a lane group's eight rows
+        if (ALONG) return (base + i) * (BR * 2) + ((g ^ swizzle(i)) << 4);
+        const int r = g * 8 + i / 4, c = base + i % 4 * 4;                 // the first four of a lane group's eight rows
         return r * (B * 2) + (((c >> 3) ^ swizzle(r)) << 4) + (c & 4) * 2;
+    }
+    // ... of the i-th 16 from there on (i * 16 < 128), in the k-th 32.  Along: 16 rows keep the swizzle, k flips bit 2 of the group.  Down:
+    // 16 columns are 2 groups, and i flips bits of the group like the swizzle does; 32 rows keep it.
+    static __device__ __forceinline__ int frag(int first, int i, int k) {
+        return ALONG ? (first ^ k << 6) + i * 16 * BR * 2 : (first ^ i << 5) + k * 32 * B * 2;
     }
 };
 
@@ -237,17 +239,7 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void k_big(BigProduct G, LinArgs A
     sp.init(G.P, at0.p0, at0.ra);
     sq.init(G.Q, at0.q0, at0.ra);
     const int wave = threadIdx.x / 64;
-    const int wp = wave / WQ * (BT / WP), wq = wave % WQ * (BT / WQ);
-    // the lane's fragment addresses: 16 rows (along) are 16 * BR * 2 bytes apart and keep the swizzle; 16 columns (down) are two
-    // 16-byte groups apart, which the swizzle permutes, so each has its own
-    int op[PA ? 1 : FP][2], oq[QA ? 1 : FQ][2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int i = 0; i < (PA ? 1 : FP); ++i) op[i][k] = SP::frag(wp + i * 16, k);
-#pragma unroll
-        for (int i = 0; i < (QA ? 1 : FQ); ++i) oq[i][k] = SP::BYTES + SQ::frag(wq + i * 16, k);
-    }
+    const int op = SP::frag(wave / WQ * (BT / WP)), oq = SQ::frag(wave % WQ * (BT / WQ));
 
     const int64_t steps = (at0.rb - at0.ra + BR - 1) / BR;
     auto load = [&](int64_t s) {
@@ -260,31 +252,59 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void k_big(BigProduct G, LinArgs A
         if (lq >= BR) sq.load_full(at + SP::BYTES, s * sq.step);
         else sq.load_part(at + SP::BYTES, s * sq.step, lq);
     };
-
+    v8 p0[FP], q0[FQ], p1[FP], q1[FQ];          // fragments of the first and the second 32 of a step
+    auto read = [&](v8 (&p)[FP], v8 (&q)[FQ], int64_t s, int k) {
+        const uint32_t at = lds0 + (int)(s & 1) * BUF;
+#pragma unroll
+        for (int j = 0; j < FQ; ++j) q[j] = read_frag<T, BT, QA, THREADS>(at + SP::BYTES, SQ::frag(oq, j, k));
+#pragma unroll
+        for (int i = 0; i < FP; ++i) p[i] = read_frag<T, BT, PA, THREADS>(at, SP::frag(op, i, k));
+    };
     f32x4 acc[FP][FQ];
 #pragma unroll
     for (int i = 0; i < FP; ++i)
 #pragma unroll
         for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    if (steps > 0) load(0);
-    for (int64_t s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                        // this step's operands are in LDS, and the other buffer has been read by all
-        if (s + 1 < steps) load(s + 1);
-        const uint32_t at = lds0 + (int)(s & 1) * BUF;
+    auto multiply = [&](const v8 (&p)[FP], const v8 (&q)[FQ]) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            v8 p[FP], q[FQ];
+        for (int i = 0; i < FP; ++i)
 #pragma unroll
-            for (int j = 0; j < FQ; ++j) q[j] = read_frag<T, BT, QA, THREADS>(at, QA ? oq[0][k] + j * 16 * BR * 2 : oq[QA ? 0 : j][k]);
+            for (int j = 0; j < FQ; ++j) acc[i][j] = mma(q[j], p[i], acc[i][j]);
+    };
+    // the reads of one half between the products of the other: the matrix cores wait for neither LDS nor its queue
+    auto interleave = [&] {
+        constexpr int READS = FP * (PA ? 1 : 2) + FQ * (QA ? 1 : 2), PER = FP * FQ / READS, REST = FP * FQ - READS * PER;
 #pragma unroll
-            for (int i = 0; i < FP; ++i) p[i] = read_frag<T, BT, PA, THREADS>(at, PA ? op[0][k] + i * 16 * BR * 2 : op[PA ? 0 : i][k]);
-#pragma unroll
-            for (int i = 0; i < FP; ++i)
-#pragma unroll
-                for (int j = 0; j < FQ; ++j) acc[i][j] = mma(q[j], p[i], acc[i][j]);
+        for (int i = 0; i < READS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(0x008, REST, 0);
+    };
+
+    if (steps > 0) {
+        load(0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (steps > 1) load(1);
+        read(p0, q0, 0, 0);
+        for (int64_t s = 0; s + 1 < steps; ++s) {
+            read(p1, q1, s, 1);
+            multiply(p0, q0);
+            interleave();
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();       // the next step's operands are in LDS, and all of this one's have been read
+            asm volatile("" ::: "memory");
+            if (s + 2 < steps) load(s + 2);
+            read(p0, q0, s + 1, 0);
+            multiply(p1, q1);
+            interleave();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        read(p1, q1, steps - 1, 1);
+        multiply(p0, q0);
+        multiply(p1, q1);
     }
     finish<T, BT, BT, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
 }
@@ -305,12 +325,7 @@ __global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_big_split(BigProduct G, L
     SQ sq;
     sp.init(G.P, at0.p0, at0.ra);
     sq.init(G.Q, at0.q0, at0.ra);
-    const int wave = threadIdx.x / 64, wp = wave / WQ * 64, wq = wave % WQ * 64;
-    int op[PA ? 1 : 4], oq[QA ? 1 : 4];
-#pragma unroll
-    for (int i = 0; i < (PA ? 1 : 4); ++i) op[i] = SP::frag(wp + i * 16, 0);
-#pragma unroll
-    for (int i = 0; i < (QA ? 1 : 4); ++i) oq[i] = 3 * SP::BYTES + SQ::frag(wq + i * 16, 0);
+    const int wave = threadIdx.x / 64, op = SP::frag(wave / WQ * 64), oq = 3 * SP::BYTES + SQ::frag(wave % WQ * 64);
 
     const int64_t steps = (at0.rb - at0.ra + BR - 1) / BR;
     auto load = [&](int64_t s) {
@@ -332,43 +347,70 @@ __global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_big_split(BigProduct G, L
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    if (steps > 0) load(0);
-    for (int64_t s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (s + 1 < steps) load(s + 1);
+    bf16x8 p[3][4], q[2][3][2];                 // parts of the P fragments; parts of the Q fragments, two columns of tiles at a time
+    auto read_p = [&](int64_t s, int k) {
+        const uint32_t at = lds0 + (int)(s & 1) * BUF + k * SP::BYTES;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[k][i] = read_frag<bf16_t, BTP, PA, THREADS>(at, SP::frag(op, i, 0));
+    };
+    auto read_q = [&](int64_t s, int half) {
         const uint32_t at = lds0 + (int)(s & 1) * BUF;
-        const float sign = s & 1 ? -1.f : 1.f;                  // (a split starts at a multiple of 64)
-        bf16x8 p[3][4];
 #pragma unroll
         for (int k = 0; k < 3; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                p[k][i] = read_frag<bf16_t, BTP, PA, THREADS>(at + k * SP::BYTES, PA ? op[0] + i * 16 * BR * 2 : op[PA ? 0 : i]);
+            for (int j = 0; j < 2; ++j) q[half][k][j] = read_frag<bf16_t, BTQ, QA, THREADS>(at + k * SQ::BYTES, SQ::frag(oq, half * 2 + j, 0));
+    };
+    f32x4 c[4][2];
+    auto product = [&](int half, int kp, int kq, bool first) {
 #pragma unroll
-        for (int jj = 0; jj < 4; jj += 2) {
-            bf16x8 q[3][2];
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int k = 0; k < 3; ++k)
+            for (int j = 0; j < 2; ++j) c[i][j] = mma(q[half][kq][j], p[kp][i], first ? f32x4{0.f, 0.f, 0.f, 0.f} : c[i][j]);
+    };
+    auto add = [&](int half, float sign) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    q[k][j] = read_frag<bf16_t, BTQ, QA, THREADS>(at + k * SQ::BYTES, QA ? oq[0] + (jj + j) * 16 * BR * 2 : oq[QA ? 0 : jj + j]);
-            f32x4 c[4][2];
-            constexpr int TP[6] = {0, 2, 1, 0, 1, 0}, TQ[6] = {2, 0, 1, 1, 0, 0};      // parts of the six products, smallest first
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int t = 0; t < 6; ++t)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) c[i][j] = mma(q[TQ[t]][j], p[TP[t]][i], t ? c[i][j] : f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][jj + j][e] = __fmaf_rn(c[i][j][e], sign, acc[i][jj + j][e]);
+                for (int e = 0; e < 4; ++e) acc[i][half * 2 + j][e] = __fmaf_rn(c[i][j][e], sign, acc[i][half * 2 + j][e]);
+    };
+    if (steps > 0) {
+        load(0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (steps > 1) load(1);
+        read_p(0, 0), read_p(0, 1), read_p(0, 2), read_q(0, 0);
+        auto first_half = [&](int64_t s, float sign) {
+            read_q(s, 1);
+            product(0, 0, 2, true), product(0, 2, 0, false), product(0, 1, 1, false), product(0, 0, 1, false), product(0, 1, 0, false), product(0, 0, 0, false);
+            add(0, sign);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        float sign = 1.f;                       // (a split starts at a multiple of 64)
+        for (int64_t s = 0; s + 1 < steps; ++s) {
+            first_half(s, sign);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();       // the next step's operands are in LDS, and all of this one's have been read
+            asm volatile("" ::: "memory");
+            if (s + 2 < steps) load(s + 2);
+            read_q(s + 1, 0);
+            // the next step's P takes each part's registers as soon as its last product is issued
+            product(1, 0, 2, true), product(1, 2, 0, false);
+            __builtin_amdgcn_sched_barrier(0);
+            read_p(s + 1, 2);
+            product(1, 1, 1, false), product(1, 1, 0, false);
+            __builtin_amdgcn_sched_barrier(0);
+            read_p(s + 1, 1);
+            product(1, 0, 1, false), product(1, 0, 0, false);
+            __builtin_amdgcn_sched_barrier(0);
+            read_p(s + 1, 0);
+            add(1, sign);
+            sign = -sign;
         }
+        first_half(steps - 1, sign);
+        product(1, 0, 2, true), product(1, 2, 0, false), product(1, 1, 1, false), product(1, 0, 1, false), product(1, 1, 0, false), product(1, 0, 0, false);
+        add(1, sign);
     }
 
     int nan = 0;                                // is there a NaN in what will be stored?
