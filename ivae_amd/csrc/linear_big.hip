@@ -31,7 +31,7 @@ __device__ const uint4 g_zeros = {0, 0, 0, 0};          // where lanes beyond th
 template <int B, int BR, bool ALONG, int THREADS>
 struct Stage {
     static constexpr int BYTES = B * BR * 2, LOADS = BYTES / (THREADS * 16), PER_ROW = (ALONG ? BR : B) / 8;
-    static_assert(BYTES % (THREADS * 16) == 0 && THREADS % PER_ROW == 0, "whole loads");
+    static_assert(BYTES % (THREADS * 16) == 0 && THREADS / PER_ROW % 16 == 0, "whole loads; the rows of one thread share a swizzle");
     uint32_t voff[LOADS];       // bytes from the tile's corner
     int row, col;               // of load 0, in elements; load j is j * (THREADS / PER_ROW) rows further
     const char* corner;

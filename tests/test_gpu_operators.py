@@ -106,6 +106,26 @@ def test_linear_large(dt, m, k, n):
     run_linear(dt, m, k, n, "gelu", seed=m + 1)
 
 
+@pytest.mark.parametrize("m,k,n", SIZES + BIG + [(64, 60000, 256), (4096, 200, 264), (8200, 1032, 136)])
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_linear_integers_are_exact(dt, m, k, n):
+    """Small whole numbers: every product and sum is one too, below 2^24, so each result is the exact one, rounded once to its type."""
+    g = torch.Generator().manual_seed(m + k + n)
+    x, w, dy, r = (torch.randint(-3, 4, s, generator=g).to(dt).to(dev()) for s in ((m, k), (n, k), (m, n), (m, n)))
+    b = torch.randint(-9, 10, (n,), generator=g).to(dt).to(dev())
+    X, W, D = x.double(), w.double(), dy.double()
+    assert torch.equal(ops.linear(x, w, b, residual=r), (X @ W.t() + b.double() + r.double()).to(dt))
+    for got, want in zip(ops.linear_backward(dy, x, w), (D @ W, D.t() @ X, D.sum(0))):
+        assert torch.equal(got, want.to(dt))
+    # with an activation whose slope is 1 or 2: ds stays whole, and its sums exact
+    y, saved = ops.linear(x, w, b, "lrelu", 2.0, save=True)
+    s = X @ W.t() + b.double()
+    assert torch.equal(y, torch.where(s > 0, s, 2 * s).to(dt))
+    ds = D * torch.where(s > 0, 1.0, 2.0)
+    for got, want in zip(ops.linear_backward(dy, x, w, saved, "lrelu", 2.0), (ds @ W, ds.t() @ X, ds.sum(0))):
+        assert torch.equal(got, want.to(dt))
+
+
 @pytest.mark.parametrize("dt", R.DTYPES)
 def test_linear_large_forms(dt):
     run_linear(dt, 640, 704, 648, "none", res=False, bias=False, seed=1)
