@@ -74,6 +74,16 @@ __device__ __forceinline__ float lin_act_slope(int act, float slope, float s) {
     }
 }
 
+// what follows the sum of one result of the forward pass
+template <typename T>
+__device__ __forceinline__ void forward_store(const LinArgs& A, int64_t m, int n, float s) {
+    if (A.b) s += to_f(((const T*)A.b)[n]);
+    if (A.pre) ((typename Pre<T>::t*)A.pre)[m * A.N + n] = pre_pack(s, typename Pre<T>::t());
+    s = lin_act<T>(A.act, A.slope, s);
+    if (A.res) s += to_f(((const T*)A.res)[m * A.ldr + n]);
+    ((T*)A.y)[m * A.N + n] = from_f<T>(s);
+}
+
 hipError_t linear_small_forward(const LinArgs& A, int dtype, hipStream_t st);
 hipError_t linear_small_backward(const LinArgs& A, int dtype, hipStream_t st);
 size_t linear_small_ws(const LinArgs& A, bool backward);

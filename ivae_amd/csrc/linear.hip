@@ -2,6 +2,7 @@
 #include "kernels.h"
 #include "linear_big.h"
 #include "linear_pack.h"
+#include "linear_rows.h"
 
 static LinArgs lin_args(const IvaeLinear& L) {
     LinArgs A = {};
@@ -166,6 +167,7 @@ static bool big_in_place(const void* p, int64_t cols, int64_t ld, int dtype) { r
 size_t linear_ws_bytes(const IvaeLinear& L, bool backward) {
     LinArgs A = lin_args(L);
     A.dx = A.dw = A.db = &A;           // the size serves a call that asks for all of them
+    if (!backward && A.M <= ROWS_MAX) return rows_ws(A);
     size_t n = linear_small_ws(A, backward);
     if (big_by_size(A, backward)) {
         const size_t big = backward ? plan_big_backward(A, L.dtype, nullptr).bytes : plan_big_forward(A, L.dtype, nullptr).bytes;
@@ -177,6 +179,7 @@ hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, cons
                          void* ws, hipStream_t st) {
     LinArgs A = lin_args(L);
     A.x = x; A.w = w; A.b = b; A.res = residual; A.y = y; A.pre = saved; A.part = (float*)ws;
+    if (A.M <= ROWS_MAX) return linear_rows_forward(A, L.dtype, st);
     if (big_by_size(A, false) && big_in_place(x, A.K, A.ldx, L.dtype) && big_in_place(w, A.K, A.K, L.dtype) && aligned(ws))
         return big_forward(A, L.dtype, ws, st);
     return linear_small_forward(A, L.dtype, st);

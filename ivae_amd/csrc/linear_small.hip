@@ -112,15 +112,6 @@ __device__ __forceinline__ void tile_mma<float>(const float* lp, const float* lq
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void forward_store(const LinArgs& A, int64_t m, int n, float s) {
-    if (A.b) s += to_f(((const T*)A.b)[n]);
-    if (A.pre) ((typename Pre<T>::t*)A.pre)[m * A.N + n] = pre_pack(s, typename Pre<T>::t());
-    s = lin_act<T>(A.act, A.slope, s);
-    if (A.res) s += to_f(((const T*)A.res)[m * A.ldr + n]);
-    ((T*)A.y)[m * A.N + n] = from_f<T>(s);
-}
-
 template <typename T, int MODE>
 __device__ __forceinline__ void tile_product(const LinArgs& A, const LinSplit& S, int64_t tile, float* part, float* part_db, T* lp, T* lq, T* le, float* lsum) {
     const int64_t split = tile / (S.tp * S.tq);

@@ -52,60 +52,106 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* lds) {
     }
 }
 
-template <typename T, int TPR>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs A) {
-    constexpr int N = Wide<T>::N, C = EPT / N, BLOCK = TPR > 256 ? TPR : 256;
-    __shared__ float lds[BLOCK / 64];
-    const int t = threadIdx.x % TPR;
-    for (int64_t r0 = (int64_t)blockIdx.x * (BLOCK / TPR); r0 < A.rows; r0 += (int64_t)gridDim.x * (BLOCK / TPR)) {
-        const int64_t row = r0 + threadIdx.x / TPR;
-        const bool live = row < A.rows;
-        const T* x = (const T*)A.x + (live ? row : 0) * A.ldx;
-        float v[C][N];
-        float s[1] = {0.f};
+// The thread's 16 elements of a row as they lie in memory: C groups of 16 bytes, the c-th at element (c TPR + t) N.  A group that the row
+// ends in is loaded by elements (TAIL: the width is no multiple of N); what lies beyond the row is 0.
+template <typename T, int TPR, bool TAIL> struct Row {
+    static constexpr int N = Wide<T>::N, C = EPT / N;
+    Vec<T> v[C];
+    __device__ __forceinline__ void load(const T* row, int t, int D, bool live) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int e = (c * TPR + t) * N;
-            if (live && e < A.D) load_some<T>(x + e, A.D - e, v[c]);
+            if (live && (TAIL ? e + N <= D : e < D)) v[c] = *(const Vec<T>*)(row + e);
             else
 #pragma unroll
-                for (int j = 0; j < N; ++j) v[c][j] = 0.f;
-#pragma unroll
-            for (int j = 0; j < N; ++j) s[0] += v[c][j];
+                for (int j = 0; j < N; ++j) v[c].e[j] = TAIL && live && e + j < D ? row[e + j] : (T)0.f;
         }
+    }
+};
+template <typename T, int TPR, bool TAIL, int C, int N> __device__ __forceinline__ void store_row(T* row, int t, int D, const float (&o)[C][N]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int e = (c * TPR + t) * N;
+        if (TAIL ? e + N <= D : e < D) store_wide<T>(row + e, o[c]);
+        else if (TAIL && e < D) store_part<T>(row + e, D - e, o[c]);
+    }
+}
+// the thread's elements of the weight or the bias (null: `none`)
+template <typename T, int TPR, bool TAIL, int C, int N>
+__device__ __forceinline__ void load_weight(const void* w, int w_f32, int t, int D, float none, float (&o)[C][N]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int e = (c * TPR + t) * N;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[c][j] = e + j < D ? none : 0.f;
+        if (!w || e >= D) continue;
+        if (TAIL && e + N > D) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (e + j < D) o[c][j] = w_f32 ? ((const float*)w)[e + j] : to_f(((const T*)w)[e + j]);
+        } else if (w_f32) {
+#pragma unroll
+            for (int h = 0; h < N; h += 4) {
+                float u[4];
+                load_wide<float>((const float*)w + e + h, u);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[c][h + j] = u[j];
+            }
+        } else {
+            load_wide<T>((const T*)w + e, o[c]);
+        }
+    }
+}
+
+// A block walks rows; the next row's loads are under way while a row is summed.
+template <typename T, int TPR, bool TAIL>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs A) {
+    constexpr int N = Wide<T>::N, C = EPT / N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+    __shared__ float lds[BLOCK / 64];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t r0 = (int64_t)blockIdx.x * RPB;
+    Row<T, TPR, TAIL> now, next;
+    now.load((const T*)A.x + (r0 + sub < A.rows ? r0 + sub : 0) * A.ldx, t, A.D, r0 + sub < A.rows);
+    float g[C][N], b[C][N];
+    load_weight<T, TPR, TAIL>(A.w, A.w_f32, t, A.D, 1.f, g);
+    load_weight<T, TPR, TAIL>(A.b, A.w_f32, t, A.D, 0.f, b);
+    for (; r0 < A.rows; r0 += step) {
+        const int64_t row = r0 + sub, ahead = row + step;
+        const bool live = row < A.rows;
+        if (r0 + step < A.rows) next.load((const T*)A.x + (ahead < A.rows ? ahead : 0) * A.ldx, t, A.D, ahead < A.rows);
+        float v[C][N];
+        float s[1] = {0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                v[c][j] = to_f(now.v[c].e[j]);
+                s[0] += v[c][j];
+            }
         row_sum<TPR, 1, BLOCK>(s, lds);
         const float mean = s[0] / (float)A.D;
         float q[1] = {0.f};
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int e = (c * TPR + t) * N;
+        for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 v[c][j] -= mean;
-                if (e + j < A.D) q[0] += v[c][j] * v[c][j];
+                if ((c * TPR + t) * N + (TAIL ? j : 0) < A.D) q[0] += v[c][j] * v[c][j];
             }
-        }
         row_sum<TPR, 1, BLOCK>(q, lds);
         const float r = 1.f / sqrtf(q[0] / (float)A.D + A.eps);
+        now = next;
         if (!live) continue;                    // (after the row's last barrier)
         if (A.stats && t == 0) {
             A.stats[row] = mean;
             A.stats[A.rows + row] = r;
         }
-        T* y = (T*)A.y + row * A.D;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int e = (c * TPR + t) * N;
-            if (e >= A.D) break;
-            float o[N];
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int i = e + j < A.D ? e + j : A.D - 1;
-                const float g = A.w ? wload(A.w, A.w_f32, i, IsBf16<T>::v) : 1.f, b = A.b ? wload(A.b, A.w_f32, i, IsBf16<T>::v) : 0.f;
-                o[j] = v[c][j] * r * g + b;
-            }
-            store_some<T>(y + e, A.D - e, o);
-        }
+            for (int j = 0; j < N; ++j) v[c][j] = v[c][j] * r * g[c][j] + b[c][j];
+        store_row<T, TPR, TAIL>((T*)A.y + row * A.D, t, A.D, v);
     }
 }
 
@@ -138,69 +184,69 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_wide(NormArgs A) {
     }
 }
 
-// dx, and each block's sums of dy xh and dy over the rows it walks (block, block + grid, ...)
-template <typename T, int TPR>
+// dx, and each block's sums of dy xh and dy over the rows it walks (block, block + grid, ...).  (1024 threads have 128 registers each:
+// no room for the next row.)
+template <typename T, int TPR, bool TAIL>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs A) {
     constexpr int N = Wide<T>::N, C = EPT / N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+    constexpr bool AHEAD = TPR < 1024;
     __shared__ float lds[BLOCK / 64 * 2];
     __shared__ float fold[RPB > 1 ? TPR * EPT * 2 : 1];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const float inv = 1.f / (float)A.D;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t r0 = (int64_t)blockIdx.x * RPB;
+    Row<T, TPR, TAIL> x, dy, xn, dyn;
+    float mean = 0.f, r = 0.f, mean_n = 0.f, r_n = 0.f;
+    auto load = [&](Row<T, TPR, TAIL>& a, Row<T, TPR, TAIL>& b, float& m, float& rs, int64_t row) {
+        const bool live = row < A.rows;
+        const int64_t at = live ? row : 0;
+        a.load((const T*)A.x + at * A.ldx, t, A.D, live);
+        b.load((const T*)A.dy + at * A.lddy, t, A.D, live);
+        m = live ? A.cstats[row] : 0.f;
+        rs = live ? A.cstats[A.rows + row] : 0.f;
+    };
+    if (AHEAD) load(x, dy, mean, r, r0 + sub);
     float g[C][N], dg[C][N], dc[C][N];
+    load_weight<T, TPR, TAIL>(A.w, A.w_f32, t, A.D, 1.f, g);
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int i = (c * TPR + t) * N + j;
-            g[c][j] = i < A.D ? (A.w ? wload(A.w, A.w_f32, i, IsBf16<T>::v) : 1.f) : 0.f;
-            dg[c][j] = dc[c][j] = 0.f;
-        }
-    const float inv = 1.f / (float)A.D;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < A.rows; r0 += (int64_t)gridDim.x * RPB) {
+        for (int j = 0; j < N; ++j) dg[c][j] = dc[c][j] = 0.f;
+    for (; r0 < A.rows; r0 += step) {
         const int64_t row = r0 + sub;
         const bool live = row < A.rows;
-        const T* x = (const T*)A.x + (live ? row : 0) * A.ldx;
-        const T* dy = (const T*)A.dy + (live ? row : 0) * A.lddy;
-        const float mean = live ? A.cstats[row] : 0.f, r = live ? A.cstats[A.rows + row] : 0.f;
+        if (!AHEAD) load(x, dy, mean, r, row);
+        else if (r0 + step < A.rows) load(xn, dyn, mean_n, r_n, row + step);
+        Row<T, TPR, TAIL> add;
+        if (A.residual) add.load((const T*)A.residual + (live ? row : 0) * A.ldr, t, A.D, live);
         float xh[C][N], d[C][N];
         float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int e = (c * TPR + t) * N;
-            if (live && e < A.D) {
-                load_some<T>(x + e, A.D - e, xh[c]);
-                load_some<T>(dy + e, A.D - e, d[c]);
-            } else
-#pragma unroll
-                for (int j = 0; j < N; ++j) xh[c][j] = d[c][j] = 0.f;
+        for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                xh[c][j] = live && e + j < A.D ? (xh[c][j] - mean) * r : 0.f;
-                dg[c][j] += d[c][j] * xh[c][j];
-                dc[c][j] += d[c][j];
-                d[c][j] *= g[c][j];
+                const bool in = live && (c * TPR + t) * N + (TAIL ? j : 0) < A.D;
+                const float dv = to_f(dy.v[c].e[j]);
+                xh[c][j] = in ? (to_f(x.v[c].e[j]) - mean) * r : 0.f;
+                dg[c][j] += dv * xh[c][j];
+                dc[c][j] += dv;
+                d[c][j] = dv * g[c][j];
                 s[0] += d[c][j];
                 s[1] += d[c][j] * xh[c][j];
             }
-        }
         row_sum<TPR, 2, BLOCK>(s, lds);
-        if (live && A.y) {
-            const float m1 = s[0] * inv, m2 = s[1] * inv;
-            T* dx = (T*)A.y + row * A.D;
-            const T* add = A.residual ? (const T*)A.residual + row * A.ldr : nullptr;
+        const float m1 = s[0] * inv, m2 = s[1] * inv, rr = r;
+        if (AHEAD) x = xn, dy = dyn, mean = mean_n, r = r_n;
+        if (!live || !A.y) continue;
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int e = (c * TPR + t) * N;
-                if (e >= A.D) break;
-                float o[N], q[N];
-                if (add) load_some<T>(add + e, A.D - e, q);
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    o[j] = r * (d[c][j] - m1 - xh[c][j] * m2);
-                    if (add) o[j] += q[j];
-                }
-                store_some<T>(dx + e, A.D - e, o);
+            for (int j = 0; j < N; ++j) {
+                d[c][j] = rr * (d[c][j] - m1 - xh[c][j] * m2);
+                if (A.residual) d[c][j] += to_f(add.v[c].e[j]);
             }
-        }
+        store_row<T, TPR, TAIL>((T*)A.y + row * A.D, t, A.D, d);
     }
     if (!A.part) return;
     float* part = A.part + (int64_t)blockIdx.x * 2 * A.D;
@@ -309,31 +355,45 @@ __global__ __launch_bounds__(1024) void k_norm_join(const float* part, int block
 }
 
 static unsigned wide_blocks(int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
-static int tpr_of(int D) { return D <= 16 * EPT ? 16 : D <= 64 * EPT ? 64 : D <= 256 * EPT ? 256 : 1024; }
-
+// threads that share a row: the fewest whose registers hold it
+static int tpr_of(int D) {
+    for (int t : {16, 64, 128, 256, 512})
+        if (D <= t * EPT) return t;
+    return 1024;
+}
+static int64_t groups_of(int64_t rows, int D, int64_t most) {       // blocks of RPB rows each, at most `most`
+    const int tpr = tpr_of(D), rpb = tpr < 256 ? 256 / tpr : 1;
+    const int64_t need = (rows + rpb - 1) / rpb;
+    return need < most ? need : most;
+}
+// about as many blocks as the chip holds: each keeps the weight in registers, and in the backward pass its sums
+static int fwd_blocks(int64_t rows, int D) { return (int)groups_of(rows, D, tpr_of(D) <= 256 ? 1280 : tpr_of(D) == 512 ? 640 : 320); }
 // blocks of the backward pass = rows of `part`
 static int norm_blocks(int64_t rows, int D) {
     if (rows == 0) return 0;
     if (D > NORM_MAX_D) return (int)(rows < 256 ? (rows + 3) / 4 : 64);
-    const int tpr = tpr_of(D), block = tpr > 256 ? tpr : 256, rpb = block / tpr;
-    const int64_t need = (rows + rpb - 1) / rpb, most = 512;
-    return (int)(need < most ? need : most);
+    return (int)groups_of(rows, D, tpr_of(D) <= 256 ? 768 : tpr_of(D) == 512 ? 512 : 256);
 }
 size_t norm_ws_bytes(int64_t rows, int D) { return (size_t)norm_blocks(rows, D) * 2 * D * sizeof(float); }
 
+template <typename T, bool TAIL>
+static void norm_fwd(const NormArgs& A, hipStream_t st) {
+    const int tpr = tpr_of(A.D);
+    const dim3 g((unsigned)fwd_blocks(A.rows, A.D)), b(tpr > 256 ? tpr : 256);
+    switch (tpr) {
+        case 16: hipLaunchKernelGGL((k_norm_fwd<T, 16, TAIL>), g, b, 0, st, A); break;
+        case 64: hipLaunchKernelGGL((k_norm_fwd<T, 64, TAIL>), g, b, 0, st, A); break;
+        case 128: hipLaunchKernelGGL((k_norm_fwd<T, 128, TAIL>), g, b, 0, st, A); break;
+        case 256: hipLaunchKernelGGL((k_norm_fwd<T, 256, TAIL>), g, b, 0, st, A); break;
+        case 512: hipLaunchKernelGGL((k_norm_fwd<T, 512, TAIL>), g, b, 0, st, A); break;
+        default: hipLaunchKernelGGL((k_norm_fwd<T, 1024, TAIL>), g, b, 0, st, A);
+    }
+}
 template <typename T>
 static void norm_fwd(const NormArgs& A, hipStream_t st) {
-    if (A.D > NORM_MAX_D) {
-        hipLaunchKernelGGL(k_norm_fwd_wide<T>, dim3(wide_blocks(A.rows)), dim3(1024), 0, st, A);
-        return;
-    }
-    const int tpr = tpr_of(A.D), block = tpr > 256 ? tpr : 256;
-    const int64_t need = (A.rows + block / tpr - 1) / (block / tpr);
-    const dim3 g((unsigned)(need < 65536 ? need : 65536)), b(block);
-    if (tpr == 16) hipLaunchKernelGGL((k_norm_fwd<T, 16>), g, b, 0, st, A);
-    else if (tpr == 64) hipLaunchKernelGGL((k_norm_fwd<T, 64>), g, b, 0, st, A);
-    else if (tpr == 256) hipLaunchKernelGGL((k_norm_fwd<T, 256>), g, b, 0, st, A);
-    else hipLaunchKernelGGL((k_norm_fwd<T, 1024>), g, b, 0, st, A);
+    if (A.D > NORM_MAX_D) hipLaunchKernelGGL(k_norm_fwd_wide<T>, dim3(wide_blocks(A.rows)), dim3(1024), 0, st, A);
+    else if (A.D % Wide<T>::N) norm_fwd<T, true>(A, st);
+    else norm_fwd<T, false>(A, st);
 }
 hipError_t launch_layer_norm(const IvaeNorm& N, const void* x, const void* w, const void* b, void* y, float* stats, hipStream_t st) {
     if (N.rows == 0) return hipSuccess;
@@ -346,18 +406,27 @@ hipError_t launch_layer_norm(const IvaeNorm& N, const void* x, const void* w, co
     return hipGetLastError();
 }
 
+template <typename T, bool TAIL>
+static void norm_bwd(const NormArgs& A, int blocks, hipStream_t st) {
+    const int tpr = tpr_of(A.D);
+    const dim3 g((unsigned)blocks), b(tpr > 256 ? tpr : 256);
+    switch (tpr) {
+        case 16: hipLaunchKernelGGL((k_norm_bwd<T, 16, TAIL>), g, b, 0, st, A); break;
+        case 64: hipLaunchKernelGGL((k_norm_bwd<T, 64, TAIL>), g, b, 0, st, A); break;
+        case 128: hipLaunchKernelGGL((k_norm_bwd<T, 128, TAIL>), g, b, 0, st, A); break;
+        case 256: hipLaunchKernelGGL((k_norm_bwd<T, 256, TAIL>), g, b, 0, st, A); break;
+        case 512: hipLaunchKernelGGL((k_norm_bwd<T, 512, TAIL>), g, b, 0, st, A); break;
+        default: hipLaunchKernelGGL((k_norm_bwd<T, 1024, TAIL>), g, b, 0, st, A);
+    }
+}
 template <typename T>
 static void norm_bwd(const NormArgs& A, int blocks, void* dg, void* dc, hipStream_t st) {
-    const dim3 g((unsigned)blocks);
     if (blocks > 0 && A.D > NORM_MAX_D) {
         if (A.y) hipLaunchKernelGGL(k_norm_bwd_wide<T>, dim3(wide_blocks(A.rows)), dim3(1024), 0, st, A);
         if (A.part) hipLaunchKernelGGL(k_norm_cols_wide<T>, dim3((A.D + 63) / 64, (unsigned)blocks), dim3(256), 0, st, A);
     } else if (blocks > 0) {
-        const int tpr = tpr_of(A.D);
-        if (tpr == 16) hipLaunchKernelGGL((k_norm_bwd<T, 16>), g, dim3(256), 0, st, A);
-        else if (tpr == 64) hipLaunchKernelGGL((k_norm_bwd<T, 64>), g, dim3(256), 0, st, A);
-        else if (tpr == 256) hipLaunchKernelGGL((k_norm_bwd<T, 256>), g, dim3(256), 0, st, A);
-        else hipLaunchKernelGGL((k_norm_bwd<T, 1024>), g, dim3(1024), 0, st, A);
+        if (A.D % Wide<T>::N) norm_bwd<T, true>(A, blocks, st);
+        else norm_bwd<T, false>(A, blocks, st);
     }
     if (dg || dc) hipLaunchKernelGGL(k_norm_join<T>, dim3((A.D + 31) / 32, 2), dim3(1024), 0, st, A.part, blocks, A.D, A.w_f32, dg, dc);
 }
