@@ -110,7 +110,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_rows(LinArgs A, int len, 
     }
 }
 
-static int rows_nf(const LinArgs& A) { return A.M > 16 && A.N >= 16384 ? 2 : 1; }
+static int rows_nf(const LinArgs& A) { return A.M > 16 && A.N >= 8192 ? 2 : 1; }
 RowsPlan rows_plan(const LinArgs& A) {
     RowsPlan p;
     p.nf = rows_nf(A);
