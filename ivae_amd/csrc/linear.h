@@ -92,7 +92,3 @@ size_t linear_small_ws(const LinArgs& A, bool backward);
 struct LinParts { const float* x; const float* w; const float* b; int kx, kw, kb; };
 hipError_t linear_join_forward(const LinArgs& A, int splits, int dtype, hipStream_t st);
 hipError_t linear_join_backward(const LinArgs& A, const LinParts& J, int dtype, hipStream_t st);
-// fp32 tiles whose flag is set in any of the `splits` runs of flags, computed again from the tensors themselves
-struct LinMarks { const int* flags; int tile_p, tile_q, splits; };
-hipError_t linear_mend_forward(const LinArgs& A, const LinMarks& y, hipStream_t st);
-hipError_t linear_mend_backward(const LinArgs& A, const LinMarks& x, const LinMarks& w, hipStream_t st);

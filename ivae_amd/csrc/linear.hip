@@ -18,20 +18,45 @@ static const int64_t BIG_MAX_LD = 1 << 21;              // 32-bit byte offsets i
 static bool big_product(int64_t P, int64_t Q, int64_t R) {
     return P >= 64 && Q >= 64 && R >= 64 && 2.0 * (double)P * (double)Q * (double)R >= 5e8;
 }
+static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 static int64_t tiles_of(const BigProduct& B, int tp, int tq) { return ((B.p_end + tp - 1) / tp) * ((B.q_end + tq - 1) / tq); }
-static void big_geometry(BigProduct& B, int dtype) {
-    const int wide = dtype == IVAE_F32 ? 128 : 256;
-    const bool large = tiles_of(B, 256, wide) >= (dtype == IVAE_F32 ? 96 : 192);
-    B.tile_p = large ? 256 : 128;
-    B.tile_q = large ? wide : 128;
-    const int64_t tiles = tiles_of(B, B.tile_p, B.tile_q);
-    int64_t s = tiles < 256 ? (large ? 256 : 512) / tiles : 1;
-    const int64_t most = B.R / 512;
-    if (s > most) s = most;
-    if (s > 32) s = 32;
-    if (s < 1) s = 1;
-    B.len = ((B.R + s - 1) / s + 63) / 64 * 64;
-    B.splits = (int)((B.R + B.len - 1) / B.len);
+// Tiles and splits of the products of one launch: the choice for which a simple model of its time is least.  A block takes `start` us and
+// `per` ns for each of its summed index (measured: a 256 x 256 tile of 16-bit values 27 ns, bound by the matrix cores; a 128 x 128
+// tile 17 ns, bound by the latency of its loads; split fp32 82 and 46 ns); blocks beyond one a CU queue up; split sums are written,
+// read and joined at 4 TB/s and one more launch.
+struct BigModel { int tile_p, tile_q; double start, per; int slots; };
+static double big_time(BigProduct** B, int n, const BigModel& m, const int64_t* s) {
+    double work = 0, longest = 0, join = 0;
+    int64_t blocks = 0;
+    for (int i = 0; i < n; ++i) {
+        const int64_t tiles = tiles_of(*B[i], m.tile_p, m.tile_q) * s[i];
+        const double t = m.start + 1e-3 * m.per * (double)((B[i]->R + s[i] - 1) / s[i]);
+        work += (double)tiles * t;
+        blocks += tiles;
+        if (t > longest) longest = t;
+        if (s[i] > 1) join += 3.0 + (double)(2 * s[i] + 1) * (double)B[i]->p_end * (double)B[i]->q_end * 4 / 4e6;
+    }
+    return (blocks <= m.slots ? longest : work / m.slots + 0.5 * longest) + join;
+}
+static void big_geometry(BigProduct** B, int n, int dtype) {
+    static const BigModel m16[2] = {{256, 256, 10.0, 27.0, 256}, {128, 128, 4.0, 17.0, 256}};
+    static const BigModel m32[2] = {{256, 128, 10.0, 82.0, 256}, {128, 128, 5.0, 46.0, 256}};
+    double best = 1e30;
+    for (const BigModel& m : dtype == IVAE_F32 ? m32 : m16)
+        for (int64_t s0 = 1; s0 <= 16; s0 *= 2)
+            for (int64_t s1 = 1; s1 <= (n == 2 ? 16 : 1); s1 *= 2) {
+                const int64_t s[2] = {s0, s1};
+                if ((s0 > 1 && B[0]->R / s0 < 192) || (n == 2 && s1 > 1 && B[1]->R / s1 < 192)) continue;
+                const double t = big_time(B, n, m, s);
+                if (t >= best) continue;
+                best = t;
+                for (int i = 0; i < n; ++i) {
+                    B[i]->tile_p = m.tile_p;
+                    B[i]->tile_q = m.tile_q;
+                    B[i]->len = up((B[i]->R + s[i] - 1) / s[i], 64);
+                    B[i]->splits = (int)((B[i]->R + B[i]->len - 1) / B[i]->len);
+                }
+            }
 }
 
 struct Bytes {                                          // a workspace, handed out in pieces of 256 bytes
@@ -43,7 +68,6 @@ struct Bytes {                                          // a workspace, handed o
         return p;
     }
 };
-static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // A matrix as an operand: in place where its rows are 16-byte groups already, packed otherwise (fp32 always)
 struct Packed { BigOperand O; PackArgs P; bool needed; };
@@ -84,22 +108,20 @@ static BigForward plan_big_forward(const LinArgs& A, int dtype, void* ws) {
     B.P = along(f.x, A.M);
     B.Q = along(f.w, A.N);
     B.p_end = A.M; B.q_end = A.N; B.R = A.K;
-    B.epi = EPI_FWD;
-    big_geometry(B, dtype);
+    BigProduct* one[1] = {&B};
+    big_geometry(one, 1, dtype);
     if (B.splits > 1) B.part = m.take<float>(B.splits * A.M * A.N);
-    if (dtype == IVAE_F32) B.nan_seen = m.take<int>(big_tiles(B) * B.splits);
     f.bytes = m.used;
     return f;
 }
 static hipError_t big_forward(LinArgs A, int dtype, void* ws, hipStream_t st) {
     const BigForward f = plan_big_forward(A, dtype, ws);
     hipError_t e = hipSuccess;
-    if (f.x.needed) e = launch_pack(f.x.P, dtype, st);
-    if (e == hipSuccess && f.w.needed) e = launch_pack(f.w.P, dtype, st);
-    if (e == hipSuccess) e = big_launch(f.B, A, dtype, st);
+    const PackArgs* packs[2] = {f.x.needed ? &f.x.P : nullptr, f.w.needed ? &f.w.P : nullptr};
+    e = launch_packs(packs, 2, dtype, st);
+    if (e == hipSuccess) e = big_forward_launch(f.B, A, dtype, st);
     A.part = f.B.part;
     if (e == hipSuccess) e = linear_join_forward(A, f.B.splits, dtype, st);
-    if (e == hipSuccess && dtype == IVAE_F32) e = linear_mend_forward(A, {f.B.nan_seen, f.B.tile_p, f.B.tile_q, f.B.splits}, st);
     return e;
 }
 
@@ -129,11 +151,9 @@ static BigBackward plan_big_backward(const LinArgs& A, int dtype, void* ws) {
     W.p_end = A.N; W.q_end = A.K; W.R = A.M;
     W.out = A.dw;
     BigProduct* both[2] = {&X, &W};
+    big_geometry(both, 2, dtype);
     for (BigProduct* B : both) {
-        B->epi = EPI_STORE;
-        big_geometry(*B, dtype);
         if (B->splits > 1) B->part = m.take<float>(B->splits * B->p_end * B->q_end);
-        if (dtype == IVAE_F32) B->nan_seen = m.take<int>(big_tiles(*B) * B->splits);
     }
     f.bytes = m.used;
     return f;
@@ -142,24 +162,20 @@ static hipError_t big_backward(const LinArgs& A, int dtype, void* ws, hipStream_
     BigBackward f = plan_big_backward(A, dtype, ws);
     hipError_t e = hipSuccess;
     f.ds.P.colsum = A.db ? f.colsum : nullptr;
-    if (f.ds.needed || A.db) e = launch_pack(f.ds.P, dtype, st);
-    if (e == hipSuccess && A.dx && f.w.needed) e = launch_pack(f.w.P, dtype, st);
-    if (e == hipSuccess && A.dw && f.x.needed) e = launch_pack(f.x.P, dtype, st);
-    if (e == hipSuccess && A.dx) e = big_launch(f.X, A, dtype, st);
-    if (e == hipSuccess && A.dw) e = big_launch(f.W, A, dtype, st);
+    const PackArgs* packs[3] = {f.ds.needed || A.db ? &f.ds.P : nullptr, A.dx && f.w.needed ? &f.w.P : nullptr, A.dw && f.x.needed ? &f.x.P : nullptr};
+    e = launch_packs(packs, 3, dtype, st);
+    if (e == hipSuccess) e = big_backward_launch(f.X, f.W, A, dtype, st);
     if (e == hipSuccess) e = linear_join_backward(A, {f.X.part, f.W.part, f.colsum, f.X.splits, f.W.splits, f.kb}, dtype, st);
-    if (e == hipSuccess && dtype == IVAE_F32)
-        e = linear_mend_backward(A, {f.X.nan_seen, f.X.tile_p, f.X.tile_q, f.X.splits}, {f.W.nan_seen, f.W.tile_p, f.W.tile_q, f.W.splits}, st);
     return e;
 }
 
 // ---- which kernel -----------------------------------------------------------------------------------------------------
 static bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
-static bool big_by_size(const LinArgs& A, bool backward) {
+static bool big_by_size(const LinArgs& A) {
     const int64_t lds[] = {A.ldx, A.lddy, A.K, A.N};
     for (int64_t ld : lds)
         if (ld > BIG_MAX_LD) return false;
-    return big_product(A.M, A.N, A.K) && (!backward || A.M > 0);
+    return A.M < 1 << 29 && big_product(A.M, A.N, A.K);        // (blocks are counted in 32 bits)
 }
 // a matrix that would be loaded in place has to start on 16 bytes
 static bool big_in_place(const void* p, int64_t cols, int64_t ld, int dtype) { return dtype == IVAE_F32 || ld % 8 || cols % 8 || aligned(p); }
@@ -169,7 +185,7 @@ size_t linear_ws_bytes(const IvaeLinear& L, bool backward) {
     A.dx = A.dw = A.db = &A;           // the size serves a call that asks for all of them
     if (!backward && A.M <= ROWS_MAX) return rows_ws(A);
     size_t n = linear_small_ws(A, backward);
-    if (big_by_size(A, backward)) {
+    if (big_by_size(A)) {
         const size_t big = backward ? plan_big_backward(A, L.dtype, nullptr).bytes : plan_big_forward(A, L.dtype, nullptr).bytes;
         if (big > n) n = big;
     }
@@ -180,7 +196,7 @@ hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, cons
     LinArgs A = lin_args(L);
     A.x = x; A.w = w; A.b = b; A.res = residual; A.y = y; A.pre = saved; A.part = (float*)ws;
     if (A.M <= ROWS_MAX) return linear_rows_forward(A, L.dtype, st);
-    if (big_by_size(A, false) && big_in_place(x, A.K, A.ldx, L.dtype) && big_in_place(w, A.K, A.K, L.dtype) && aligned(ws))
+    if (big_by_size(A) && big_in_place(x, A.K, A.ldx, L.dtype) && big_in_place(w, A.K, A.K, L.dtype) && aligned(ws))
         return big_forward(A, L.dtype, ws, st);
     return linear_small_forward(A, L.dtype, st);
 }
@@ -188,7 +204,7 @@ hipError_t launch_linear_backward(const IvaeLinear& L, const void* dy, const voi
                                   void* db, void* ws, hipStream_t st) {
     LinArgs A = lin_args(L);
     A.x = x; A.w = w; A.dy = dy; A.cpre = saved; A.dx = dx; A.dw = dw; A.db = db; A.part = (float*)ws;
-    if (big_by_size(A, true) && (A.act != IVAE_ACT_NONE || big_in_place(dy, A.N, A.lddy, L.dtype)) && (!dw || big_in_place(x, A.K, A.ldx, L.dtype)) &&
+    if (big_by_size(A) && (A.act != IVAE_ACT_NONE || big_in_place(dy, A.N, A.lddy, L.dtype)) && (!dw || big_in_place(x, A.K, A.ldx, L.dtype)) &&
         (!dx || big_in_place(w, A.K, A.K, L.dtype)) && aligned(ws))
         return big_backward(A, L.dtype, ws, st);
     return linear_small_backward(A, L.dtype, st);

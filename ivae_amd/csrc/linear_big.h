@@ -12,20 +12,19 @@ struct BigOperand {
     bool along;
 };
 
-enum { EPI_FWD, EPI_STORE };
+enum { EPI_FWD, EPI_STORE };    // what follows the sums: forward_store's, or a store of the result type
 
 struct BigProduct {
     BigOperand P, Q;
     int64_t p_end, q_end, R;    // size of C and of the sum
-    int epi;
-    void* out;                  // EPI_STORE: (p_end, q_end) of the output type
+    void* out;                  // backward pass: (p_end, q_end) of the tensors' type
     float* part;                // split sums: (splits, p_end, q_end)
-    int* nan_seen;              // split fp32: one flag a tile and split: 1 where a sum came out as NaN
     int tile_p, tile_q;         // 16-bit types: 256 x 256 or 128 x 128; fp32: 256 x 128 or 128 x 128
     int splits;
     int64_t len;                // R of a split, a multiple of 64
 };
 
 int64_t big_tiles(const BigProduct& B);
-// T: type of the tensors (float: operands are split bf16)
-hipError_t big_launch(const BigProduct& B, const LinArgs& A, int dtype, hipStream_t st);
+// dtype: of the tensors (fp32: operands are split bf16).  The two products of a backward pass have tiles of one size.
+hipError_t big_forward_launch(const BigProduct& B, const LinArgs& A, int dtype, hipStream_t st);
+hipError_t big_backward_launch(const BigProduct& X, const BigProduct& W, const LinArgs& A, int dtype, hipStream_t st);

@@ -7,14 +7,15 @@
 // LDS rows cannot be padded (a load fills them in lane order), so the 16-byte groups of a row are permuted instead, by an XOR with
 // bits of the row number that puts every 16 lanes (along) or every 8 groups of 32 bytes (down) on distinct banks.
 //
-// fp32 (k_big_split): x = x0 + x1 + x2 with bf16 parts cut off after 8 bits each (exact), and x y = x0 y0 + x0 y1 + x1 y0 + x1 y1 + x0 y2 +
+// fp32 (k_split_*): x = x0 + x1 + x2 with bf16 parts cut off after 8 bits each (exact), and x y = x0 y0 + x0 y1 + x1 y0 + x1 y1 + x0 y2 +
 // x2 y0 up to 2^-23 |x y|: six products at 16 times the rate of the fp32 matrix instructions.  The bf16 matrix instructions round their
 // running sum downwards, by little but always the same way, and a column sum over such results would add that up; so every 32 of
 // the summed index start from zero, smallest products first, and are added to the sum by fp32 additions that round to nearest.
-// An infinity times a part that is 0 makes a NaN that fp32 would not: a tile with a NaN in it is marked, and computed again in
-// fp32 by the small kernel.
+// An infinity times a part that is 0 makes a NaN that fp32 would not: a tile with a NaN in it is computed again in fp32, from the
+// tensors themselves.
 #include "kernels.h"
 #include "linear_big.h"
+#include "linear_tile.h"
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char* lds_ptr;
@@ -138,15 +139,23 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int n, const 
         store_some<T>(p + h * N, n - h * N, u);
     }
 }
-// LDS of a block: two buffers of a step, and in the end 128 rows of sums (4 words of padding keep a column off one bank)
-static constexpr int big_lds(int step_bytes, int btq) { return 2 * step_bytes > 128 * (btq + 4) * 4 ? 2 * step_bytes : 128 * (btq + 4) * 4; }
+// LDS of a block: `buffers` of a step, and in the end 128 rows of sums (4 words of padding keep a column off one bank)
+static constexpr int big_lds(int buffers, int step_bytes, int btq) {
+    return buffers * step_bytes > 128 * (btq + 4) * 4 ? buffers * step_bytes : 128 * (btq + 4) * 4;
+}
+
+// all but the last N loads into LDS have arrived (they are counted in the order of their issue), and all LDS reads
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void block_barrier() {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 // Tiles in bands of 8 rows of tiles, neighbours in a band one after the other, and a contiguous run of them for each of the 8 dies
 // (blocks go to the dies in turn): a die's cache then serves the few operand strips that its run shares.
-struct Place { int64_t p0, q0, ra, rb; int split, tile; };
-template <int BTP, int BTQ> __device__ __forceinline__ Place place(const BigProduct& G) {
+struct Place { int64_t p0, q0, ra, rb; int split; };
+template <int BTP, int BTQ> __device__ __forceinline__ Place place(const BigProduct& G, int b) {
     const int tp = (int)((G.p_end + BTP - 1) / BTP), tq = (int)((G.q_end + BTQ - 1) / BTQ), tiles = tp * tq, blocks = tiles * G.splits;
-    int b = blockIdx.x;
     const int per = blocks / 8, extra = blocks % 8, die = b % 8;
     b = die * per + (die < extra ? die : extra) + b / 8;
     Place r;
@@ -154,7 +163,6 @@ template <int BTP, int BTQ> __device__ __forceinline__ Place place(const BigProd
     b -= r.split * tiles;
     const int band = b / (8 * tq), in_band = b - band * 8 * tq, rows = tp - band * 8 < 8 ? tp - band * 8 : 8;
     const int ip = band * 8 + in_band % rows, iq = in_band / rows;
-    r.tile = ip * tq + iq;
     r.p0 = (int64_t)ip * BTP;
     r.q0 = (int64_t)iq * BTQ;
     r.ra = r.split * G.len;
@@ -222,29 +230,28 @@ __device__ __forceinline__ void finish(const BigProduct& G, const LinArgs& A, co
     }
 }
 
-// 16-bit types.  BT x BT tiles, WP x WQ waves, 64 of the summed index a step.
-template <typename T, int BT, int WP, int WQ, bool PA, bool QA, int EPI>
-__global__ __launch_bounds__(WP * WQ * 64, 2) void k_big(BigProduct G, LinArgs A) {
+// 16-bit types.  BT x BT tiles, WP x WQ waves, 64 of the summed index a step, BUFS buffers.
+template <typename T, int BT, int WP, int WQ, int BUFS, bool PA, bool QA, int EPI>
+__device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, int block, char* smem) {
     constexpr int THREADS = WP * WQ * 64, FP = BT / WP / 16, FQ = BT / WQ / 16, BR = 64;
     typedef Stage<BT, BR, PA, THREADS> SP;
     typedef Stage<BT, BR, QA, THREADS> SQ;
     typedef typename E8<T>::t v8;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)smem;
-    constexpr int BUF = SP::BYTES + SQ::BYTES;
-    const Place at0 = place<BT, BT>(G);
+    constexpr int BUF = SP::BYTES + SQ::BYTES, LOADS = SP::LOADS + SQ::LOADS;
+    const Place at0 = place<BT, BT>(G, block);
 
     SP sp;
     SQ sq;
     sp.init(G.P, at0.p0, at0.ra);
     sq.init(G.Q, at0.q0, at0.ra);
     const int wave = threadIdx.x / 64;
-    const int op = SP::frag(wave / WQ * (BT / WP)), oq = SQ::frag(wave % WQ * (BT / WQ));
+    const int op = SP::frag(wave / WQ * (BT / WP)), oq = SP::BYTES + SQ::frag(wave % WQ * (BT / WQ));
 
-    const int64_t steps = (at0.rb - at0.ra + BR - 1) / BR;
-    auto load = [&](int64_t s) {
-        const uint32_t at = lds0 + (int)(s & 1) * BUF;
-        const int64_t r = at0.ra + s * BR, end = at0.rb;
+    const int steps = (int)((at0.rb - at0.ra + BR - 1) / BR);
+    auto load = [&](int s) {
+        const uint32_t at = lds0 + s % BUFS * BUF;
+        const int64_t r = at0.ra + (int64_t)s * BR, end = at0.rb;
         // a split ends at a multiple of BR or at R, so only R itself cuts a step short
         const int64_t lp = (end < G.R ? end : PA ? G.P.limit : G.R) - r, lq = (end < G.R ? end : QA ? G.Q.limit : G.R) - r;
         if (lp >= BR) sp.load_full(at, s * sp.step);
@@ -253,10 +260,10 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void k_big(BigProduct G, LinArgs A
         else sq.load_part(at + SP::BYTES, s * sq.step, lq);
     };
     v8 p0[FP], q0[FQ], p1[FP], q1[FQ];          // fragments of the first and the second 32 of a step
-    auto read = [&](v8 (&p)[FP], v8 (&q)[FQ], int64_t s, int k) {
-        const uint32_t at = lds0 + (int)(s & 1) * BUF;
+    auto read = [&](v8 (&p)[FP], v8 (&q)[FQ], int s, int k) {
+        const uint32_t at = lds0 + s % BUFS * BUF;
 #pragma unroll
-        for (int j = 0; j < FQ; ++j) q[j] = read_frag<T, BT, QA, THREADS>(at + SP::BYTES, SQ::frag(oq, j, k));
+        for (int j = 0; j < FQ; ++j) q[j] = read_frag<T, BT, QA, THREADS>(at, SQ::frag(oq, j, k));
 #pragma unroll
         for (int i = 0; i < FP; ++i) p[i] = read_frag<T, BT, PA, THREADS>(at, SP::frag(op, i, k));
     };
@@ -280,27 +287,26 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void k_big(BigProduct G, LinArgs A
             __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, REST, 0);
+        __builtin_amdgcn_sched_barrier(0);
     };
 
     if (steps > 0) {
-        load(0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (steps > 1) load(1);
+        for (int s = 0; s < BUFS && s < steps; ++s) load(s);
+        if (steps >= BUFS) wait_loads<(BUFS - 1) * LOADS>();
+        else wait_loads<0>();
+        block_barrier();
         read(p0, q0, 0, 0);
-        for (int64_t s = 0; s + 1 < steps; ++s) {
+        for (int s = 0; s + 1 < steps; ++s) {
             read(p1, q1, s, 1);
             multiply(p0, q0);
             interleave();
-            __builtin_amdgcn_sched_barrier(0);
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();       // the next step's operands are in LDS, and all of this one's have been read
-            asm volatile("" ::: "memory");
-            if (s + 2 < steps) load(s + 2);
+            if (s + BUFS <= steps) wait_loads<(BUFS - 2) * LOADS>();
+            else wait_loads<0>();
+            block_barrier();                    // the next step's operands are in LDS, and all of this one's have been read
+            if (s + BUFS < steps) load(s + BUFS);
             read(p0, q0, s + 1, 0);
             multiply(p1, q1);
             interleave();
-            __builtin_amdgcn_sched_barrier(0);
         }
         read(p1, q1, steps - 1, 1);
         multiply(p0, q0);
@@ -311,15 +317,14 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void k_big(BigProduct G, LinArgs A
 
 // fp32 in three bf16 parts.  BTP x BTQ tiles, 64 x 64 a wave, 32 of the summed index a step, all three parts of both operands in LDS:
 // six products for each pair of fragments that is read.
-template <int BTP, int BTQ, bool PA, bool QA, int EPI>
-__global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_big_split(BigProduct G, LinArgs A) {
+template <int BTP, int BTQ, int BUFS, bool PA, bool QA, int EPI>
+__device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A, int block, char* smem) {
     constexpr int WP = BTP / 64, WQ = BTQ / 64, THREADS = WP * WQ * 64, BR = 32;
     typedef Stage<BTP, BR, PA, THREADS> SP;
     typedef Stage<BTQ, BR, QA, THREADS> SQ;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)smem;
-    constexpr int BUF = 3 * (SP::BYTES + SQ::BYTES);
-    const Place at0 = place<BTP, BTQ>(G);
+    constexpr int BUF = 3 * (SP::BYTES + SQ::BYTES), LOADS = 3 * (SP::LOADS + SQ::LOADS);
+    const Place at0 = place<BTP, BTQ>(G, block);
 
     SP sp;
     SQ sq;
@@ -327,10 +332,10 @@ __global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_big_split(BigProduct G, L
     sq.init(G.Q, at0.q0, at0.ra);
     const int wave = threadIdx.x / 64, op = SP::frag(wave / WQ * 64), oq = 3 * SP::BYTES + SQ::frag(wave % WQ * 64);
 
-    const int64_t steps = (at0.rb - at0.ra + BR - 1) / BR;
-    auto load = [&](int64_t s) {
-        const uint32_t at = lds0 + (int)(s & 1) * BUF;
-        const int64_t r = at0.ra + s * BR, end = at0.rb;
+    const int steps = (int)((at0.rb - at0.ra + BR - 1) / BR);
+    auto load = [&](int s) {
+        const uint32_t at = lds0 + s % BUFS * BUF;
+        const int64_t r = at0.ra + (int64_t)s * BR, end = at0.rb;
         const int64_t lp = (end < G.R ? end : PA ? G.P.limit : G.R) - r, lq = (end < G.R ? end : QA ? G.Q.limit : G.R) - r;
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
@@ -348,13 +353,13 @@ __global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_big_split(BigProduct G, L
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     bf16x8 p[3][4], q[2][3][2];                 // parts of the P fragments; parts of the Q fragments, two columns of tiles at a time
-    auto read_p = [&](int64_t s, int k) {
-        const uint32_t at = lds0 + (int)(s & 1) * BUF + k * SP::BYTES;
+    auto read_p = [&](int s, int k) {
+        const uint32_t at = lds0 + s % BUFS * BUF + k * SP::BYTES;
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[k][i] = read_frag<bf16_t, BTP, PA, THREADS>(at, SP::frag(op, i, 0));
     };
-    auto read_q = [&](int64_t s, int half) {
-        const uint32_t at = lds0 + (int)(s & 1) * BUF;
+    auto read_q = [&](int s, int half) {
+        const uint32_t at = lds0 + s % BUFS * BUF;
 #pragma unroll
         for (int k = 0; k < 3; ++k)
 #pragma unroll
@@ -375,25 +380,26 @@ __global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_big_split(BigProduct G, L
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[i][half * 2 + j][e] = __fmaf_rn(c[i][j][e], sign, acc[i][half * 2 + j][e]);
     };
+
     if (steps > 0) {
-        load(0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (steps > 1) load(1);
+        for (int s = 0; s < BUFS && s < steps; ++s) load(s);
+        if (steps >= BUFS) wait_loads<(BUFS - 1) * LOADS>();
+        else wait_loads<0>();
+        block_barrier();
         read_p(0, 0), read_p(0, 1), read_p(0, 2), read_q(0, 0);
-        auto first_half = [&](int64_t s, float sign) {
+        auto first_half = [&](int s, float sign) {
             read_q(s, 1);
             product(0, 0, 2, true), product(0, 2, 0, false), product(0, 1, 1, false), product(0, 0, 1, false), product(0, 1, 0, false), product(0, 0, 0, false);
             add(0, sign);
             __builtin_amdgcn_sched_barrier(0);
         };
         float sign = 1.f;                       // (a split starts at a multiple of 64)
-        for (int64_t s = 0; s + 1 < steps; ++s) {
+        for (int s = 0; s + 1 < steps; ++s) {
             first_half(s, sign);
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();       // the next step's operands are in LDS, and all of this one's have been read
-            asm volatile("" ::: "memory");
-            if (s + 2 < steps) load(s + 2);
+            if (s + BUFS <= steps) wait_loads<(BUFS - 2) * LOADS>();
+            else wait_loads<0>();
+            block_barrier();                    // the next step's operands are in LDS, and all of this one's have been read
+            if (s + BUFS < steps) load(s + BUFS);
             read_q(s + 1, 0);
             // the next step's P takes each part's registers as soon as its last product is issued
             product(1, 0, 2, true), product(1, 2, 0, false);
@@ -421,46 +427,98 @@ __global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_big_split(BigProduct G, L
 #pragma unroll
             for (int e = 0; e < 4; ++e) nan |= acc[i][j][e] != acc[i][j][e];
     nan = __syncthreads_or(nan);
-    if (threadIdx.x == 0) {
-        const int64_t tiles = ((G.p_end + BTP - 1) / BTP) * ((G.q_end + BTQ - 1) / BTQ);
-        G.nan_seen[at0.split * tiles + at0.tile] = nan;
+    if (nan) {                                  // 64 x 64 at a time by every 256 threads
+        constexpr int GROUPS = THREADS / 256, SUBS = (BTP / 64) * (BTQ / 64), MODE = EPI == EPI_FWD ? MODE_FWD : PA ? MODE_DX : MODE_DW;
+        static_assert(SUBS % GROUPS == 0, "the groups meet the same barriers");
+        const LinSplit S = {0, 0, G.splits, G.len};
+        LinArgs B = A;
+        B.db = nullptr;                         // (its sums are fp32 already)
+        const int group = threadIdx.x / 256;
+        float* lds = (float*)smem + group * 2 * TP * Lds<float>::LD;
+        __syncthreads();
+        for (int u = group; u < SUBS; u += GROUPS)
+            tile_product<float, MODE>(threadIdx.x % 256, B, S, at0.split, at0.p0 + u / (BTQ / 64) * 64, at0.q0 + u % (BTQ / 64) * 64, G.part, nullptr, lds,
+                                      lds + TP * Lds<float>::LD, nullptr, nullptr);
+        return;
     }
     finish<float, BTP, BTQ, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
 }
 
-int64_t big_tiles(const BigProduct& B) { return ((B.p_end + B.tile_p - 1) / B.tile_p) * ((B.q_end + B.tile_q - 1) / B.tile_q); }
+// One launch for both products of the backward pass: the first nx blocks are dx's.
+template <typename T, int BT, int WP, int WQ, int BUFS>
+__global__ __launch_bounds__(WP * WQ * 64, 2) void k_big_fwd(BigProduct G, LinArgs A) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    big_tile<T, BT, WP, WQ, BUFS, true, true, EPI_FWD>(G, A, blockIdx.x, smem);
+}
+template <typename T, int BT, int WP, int WQ, int BUFS>
+__global__ __launch_bounds__(WP * WQ * 64, 2) void k_big_bwd(BigProduct X, int nx, BigProduct W, LinArgs A) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    if ((int)blockIdx.x < nx) big_tile<T, BT, WP, WQ, BUFS, true, false, EPI_STORE>(X, A, blockIdx.x, smem);
+    else big_tile<T, BT, WP, WQ, BUFS, false, false, EPI_STORE>(W, A, blockIdx.x - nx, smem);
+}
+template <int BTP, int BTQ, int BUFS>
+__global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_split_fwd(BigProduct G, LinArgs A) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    split_tile<BTP, BTQ, BUFS, true, true, EPI_FWD>(G, A, blockIdx.x, smem);
+}
+template <int BTP, int BTQ, int BUFS>
+__global__ __launch_bounds__(BTP * BTQ / 64, 2) void k_split_bwd(BigProduct X, int nx, BigProduct W, LinArgs A) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    if ((int)blockIdx.x < nx) split_tile<BTP, BTQ, BUFS, true, false, EPI_STORE>(X, A, blockIdx.x, smem);
+    else split_tile<BTP, BTQ, BUFS, false, false, EPI_STORE>(W, A, blockIdx.x - nx, smem);
+}
 
-template <typename F>
-static hipError_t go(F fn, int bytes, int threads, SmemCache& cache, const BigProduct& B, const LinArgs& A, hipStream_t st) {
+int64_t big_tiles(const BigProduct& B) { return ((B.p_end + B.tile_p - 1) / B.tile_p) * ((B.q_end + B.tile_q - 1) / B.tile_q); }
+static int blocks_of(const BigProduct& B) { return (int)(big_tiles(B) * B.splits); }
+
+template <typename F, typename... Args>
+static hipError_t go(F fn, int bytes, int threads, SmemCache& cache, int blocks, hipStream_t st, Args... args) {
     const hipError_t e = set_smem((const void*)fn, bytes, cache);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(fn, dim3((unsigned)(big_tiles(B) * B.splits)), dim3(threads), bytes, st, B, A);
+    hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(threads), bytes, st, args...);
     return hipGetLastError();
 }
-template <typename T, int BT, int WP, int WQ, bool PA, bool QA, int EPI>
-static hipError_t go16(const BigProduct& B, const LinArgs& A, hipStream_t st) {
-    static SmemCache cache;
-    return go(k_big<T, BT, WP, WQ, PA, QA, EPI>, big_lds(2 * BT * 64 * 2, BT), WP * WQ * 64, cache, B, A, st);
+template <typename T, int BT, int WP, int WQ, int BUFS> struct Big16 {
+    static constexpr int LDS = big_lds(BUFS, 2 * BT * 64 * 2, BT), THREADS = WP * WQ * 64;
+    static hipError_t fwd(const BigProduct& B, const LinArgs& A, hipStream_t st) {
+        static SmemCache cache;
+        return go(k_big_fwd<T, BT, WP, WQ, BUFS>, LDS, THREADS, cache, blocks_of(B), st, B, A);
+    }
+    static hipError_t bwd(const BigProduct& X, int nx, const BigProduct& W, int nw, const LinArgs& A, hipStream_t st) {
+        static SmemCache cache;
+        return go(k_big_bwd<T, BT, WP, WQ, BUFS>, LDS, THREADS, cache, nx + nw, st, X, nx, W, A);
+    }
+};
+template <int BTP, int BTQ, int BUFS> struct Big32 {
+    static constexpr int LDS = big_lds(BUFS, 3 * (BTP + BTQ) * 32 * 2, BTQ), THREADS = BTP * BTQ / 64;
+    static hipError_t fwd(const BigProduct& B, const LinArgs& A, hipStream_t st) {
+        static SmemCache cache;
+        return go(k_split_fwd<BTP, BTQ, BUFS>, LDS, THREADS, cache, blocks_of(B), st, B, A);
+    }
+    static hipError_t bwd(const BigProduct& X, int nx, const BigProduct& W, int nw, const LinArgs& A, hipStream_t st) {
+        static SmemCache cache;
+        return go(k_split_bwd<BTP, BTQ, BUFS>, LDS, THREADS, cache, nx + nw, st, X, nx, W, A);
+    }
+};
+// 128 x 128 tiles of 16-bit types: up to one block a CU has four buffers (its loads are three steps ahead: such products wait for
+// memory, not for the matrix cores), more have two, and two blocks share a CU.
+template <typename T, typename... Args> static hipError_t fwd16(int blocks, int tile, Args... a) {
+    if (tile == 256) return Big16<T, 256, 2, 4, 2>::fwd(a...);
+    return blocks <= 256 ? Big16<T, 128, 2, 2, 4>::fwd(a...) : Big16<T, 128, 2, 2, 2>::fwd(a...);
 }
-template <int BTP, int BTQ, bool PA, bool QA, int EPI>
-static hipError_t go32(const BigProduct& B, const LinArgs& A, hipStream_t st) {
-    static SmemCache cache;
-    return go(k_big_split<BTP, BTQ, PA, QA, EPI>, big_lds(3 * (BTP + BTQ) * 32 * 2, BTQ), BTP * BTQ / 64, cache, B, A, st);
+template <typename T, typename... Args> static hipError_t bwd16(int blocks, int tile, Args... a) {
+    if (tile == 256) return Big16<T, 256, 2, 4, 2>::bwd(a...);
+    return blocks <= 256 ? Big16<T, 128, 2, 2, 4>::bwd(a...) : Big16<T, 128, 2, 2, 2>::bwd(a...);
 }
-template <typename T, int BT, int WP, int WQ>
-static hipError_t forms16(const BigProduct& B, const LinArgs& A, hipStream_t st) {
-    if (B.epi == EPI_FWD) return go16<T, BT, WP, WQ, true, true, EPI_FWD>(B, A, st);      // forward
-    if (B.P.along) return go16<T, BT, WP, WQ, true, false, EPI_STORE>(B, A, st);          // dx
-    return go16<T, BT, WP, WQ, false, false, EPI_STORE>(B, A, st);                        // dw
+hipError_t big_forward_launch(const BigProduct& B, const LinArgs& A, int dtype, hipStream_t st) {
+    if (dtype == IVAE_F32) return B.tile_p == 256 ? Big32<256, 128, 2>::fwd(B, A, st) : Big32<128, 128, 3>::fwd(B, A, st);
+    if (dtype == IVAE_BF16) return fwd16<bf16_t>(blocks_of(B), B.tile_p, B, A, st);
+    return fwd16<f16_t>(blocks_of(B), B.tile_p, B, A, st);
 }
-template <int BTP, int BTQ>
-static hipError_t forms32(const BigProduct& B, const LinArgs& A, hipStream_t st) {
-    if (B.epi == EPI_FWD) return go32<BTP, BTQ, true, true, EPI_FWD>(B, A, st);
-    if (B.P.along) return go32<BTP, BTQ, true, false, EPI_STORE>(B, A, st);
-    return go32<BTP, BTQ, false, false, EPI_STORE>(B, A, st);
-}
-hipError_t big_launch(const BigProduct& B, const LinArgs& A, int dtype, hipStream_t st) {
-    if (dtype == IVAE_F32) return B.tile_p == 256 ? forms32<256, 128>(B, A, st) : forms32<128, 128>(B, A, st);
-    if (dtype == IVAE_BF16) return B.tile_p == 256 ? forms16<bf16_t, 256, 2, 4>(B, A, st) : forms16<bf16_t, 128, 2, 2>(B, A, st);
-    return B.tile_p == 256 ? forms16<f16_t, 256, 2, 4>(B, A, st) : forms16<f16_t, 128, 2, 2>(B, A, st);
+hipError_t big_backward_launch(const BigProduct& X, const BigProduct& W, const LinArgs& A, int dtype, hipStream_t st) {
+    const int nx = A.dx ? blocks_of(X) : 0, nw = A.dw ? blocks_of(W) : 0;
+    if (nx + nw == 0) return hipSuccess;
+    if (dtype == IVAE_F32) return X.tile_p == 256 ? Big32<256, 128, 2>::bwd(X, nx, W, nw, A, st) : Big32<128, 128, 3>::bwd(X, nx, W, nw, A, st);
+    if (dtype == IVAE_BF16) return bwd16<bf16_t>(nx + nw, X.tile_p, X, nx, W, nw, A, st);
+    return bwd16<f16_t>(nx + nw, X.tile_p, X, nx, W, nw, A, st);
 }

@@ -19,14 +19,19 @@ __device__ __forceinline__ void cut(float x, bf16_t (&o)[3]) {
     o[2] = __builtin_bit_cast(bf16_t, (uint16_t)(__builtin_bit_cast(uint32_t, r2) >> 16));
 }
 
+struct PackJobs { PackArgs job[3]; };
 template <typename T>
-__global__ __launch_bounds__(256) void k_pack(PackArgs A) {
+__global__ __launch_bounds__(256) void k_pack(PackJobs J) {
     typedef typename Pre<T>::t pre_t;
+    int block = blockIdx.x, k = 0;
+    while (block >= J.job[k].blocks) block -= J.job[k++].blocks;
+    const PackArgs& A = J.job[k];
+    const int bx = block % A.blocks_x, by = block / A.blocks_x, rows_of_blocks = A.blocks / A.blocks_x;
     const int group = A.group;                          // threads that share a row of 8 * group values
-    const int col = (blockIdx.x * group + threadIdx.x % group) * 8, sub = threadIdx.x / group, subs = 256 / group;
+    const int col = (bx * group + threadIdx.x % group) * 8, sub = threadIdx.x / group, subs = 256 / group;
     float sum[8] = {};
     const int left = A.cols - col;                      // <= 0: beyond the last value (the padding is zeros)
-    for (int64_t r = (int64_t)blockIdx.y * subs + sub; r < A.rows && col < A.ldo; r += (int64_t)gridDim.y * subs) {
+    for (int64_t r = (int64_t)by * subs + sub; r < A.rows && col < A.ldo; r += (int64_t)rows_of_blocks * subs) {
         float v[8], s[8];
         const T* p = (const T*)A.src + r * A.ld + col;
         constexpr int N = Wide<T>::N;
@@ -82,8 +87,8 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs A) {
     for (int i = threadIdx.x; i < group * 8; i += 256) {
         float s = 0.f;
         for (int k = 0; k < subs; ++k) s += fold[k * group + i / 8][i % 8];
-        const int c = blockIdx.x * group * 8 + i;
-        if (c < A.cols) A.colsum[(int64_t)blockIdx.y * A.cols + c] = s;
+        const int c = bx * group * 8 + i;
+        if (c < A.cols) A.colsum[(int64_t)by * A.cols + c] = s;
     }
 }
 
@@ -92,20 +97,29 @@ static int group_of(int64_t width) {                    // a power of two: 8 * g
     while (g < 64 && g * 8 < width) g *= 2;
     return g;
 }
-// blocks along the rows: about 2048 blocks in all, 8 rows a thread at least
+// blocks along the rows: about 2048 blocks in all, and then more rows a thread
 int pack_row_blocks(int64_t rows, int64_t width) {
     const int g = group_of(width);
     const int64_t strips = (width + g * 8 - 1) / (g * 8), subs = 256 / g;
-    int64_t y = (rows + subs * 8 - 1) / (subs * 8), most = 2048 / strips;
+    int64_t y = (rows + subs - 1) / subs, most = 2048 / strips;
     if (y > most) y = most;
     return (int)(y < 1 ? 1 : y);
 }
-hipError_t launch_pack(const PackArgs& P, int dtype, hipStream_t st) {
-    PackArgs A = P;
-    A.group = group_of(A.ldo);
-    const dim3 g((unsigned)((A.ldo + A.group * 8 - 1) / (A.group * 8)), (unsigned)pack_row_blocks(A.rows, A.ldo)), b(256);
-    if (dtype == IVAE_F32) hipLaunchKernelGGL(k_pack<float>, g, b, 0, st, A);
-    else if (dtype == IVAE_BF16) hipLaunchKernelGGL(k_pack<bf16_t>, g, b, 0, st, A);
-    else hipLaunchKernelGGL(k_pack<f16_t>, g, b, 0, st, A);
+hipError_t launch_packs(const PackArgs* const* P, int n, int dtype, hipStream_t st) {
+    PackJobs J = {};
+    int jobs = 0, blocks = 0;
+    for (int i = 0; i < n; ++i) {
+        if (!P[i]) continue;
+        PackArgs& A = J.job[jobs++] = *P[i];
+        A.group = group_of(A.ldo);
+        A.blocks_x = (int)((A.ldo + A.group * 8 - 1) / (A.group * 8));
+        A.blocks = A.blocks_x * pack_row_blocks(A.rows, A.ldo);
+        blocks += A.blocks;
+    }
+    if (blocks == 0) return hipSuccess;
+    const dim3 g((unsigned)blocks), b(256);
+    if (dtype == IVAE_F32) hipLaunchKernelGGL(k_pack<float>, g, b, 0, st, J);
+    else if (dtype == IVAE_BF16) hipLaunchKernelGGL(k_pack<bf16_t>, g, b, 0, st, J);
+    else hipLaunchKernelGGL(k_pack<f16_t>, g, b, 0, st, J);
     return hipGetLastError();
 }

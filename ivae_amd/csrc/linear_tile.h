@@ -1,0 +1,185 @@
+// The 64 x 64 tile of a product, staged through registers: any size, any row stride, any alignment.
+//
+// One tile product serves the three products.  P rows, Q columns, R summed over:
+//   forward  P = m, Q = n, R = k     y[m,n]  = sum_k x[m,k] w[n,k]
+//   dx       P = m, Q = k, R = n     dx[m,k] = sum_n ds[m,n] w[n,k]
+//   dw       P = n, Q = k, R = m     dw[n,k] = sum_m ds[m,n] x[m,k]        (db[n] = sum_m ds[m,n] on the way)
+// The Q operand is the matrix instruction's first one, so that a lane ends up with 4 neighbouring columns of one row.
+// In the 16-bit types the gradient of the pre-activation, act'(s) dy, enters as the sum of two numbers of the type (the second is
+// the first's rounding error), one more matrix instruction each: these sizes wait for memory and launches, and the products then
+// have no rounding but their result's.
+#pragma once
+#include "linear.h"
+
+static constexpr int TP = 64, TQ = 64, TR = 32;
+
+template <typename T> struct Lds { static constexpr int LD = TR + 8; };       // row stride in elements; rows stay 16-byte aligned
+template <> struct Lds<float> { static constexpr int LD = TR + 4; };
+
+enum { MODE_FWD, MODE_DX, MODE_DW };
+
+struct LinSplit { int64_t tp, tq; int splits; int64_t len; };   // tiles along P and Q, parts of R, each `len` long
+
+// 8 neighbouring elements from (outer, inner) of a row-major matrix, zero outside [0, outers) x [0, inner_end)
+template <typename T>
+__device__ __forceinline__ void fetch8(const T* base, int64_t ld, int64_t outer, int64_t outers, int64_t inner, int64_t inner_end, float (&v)[8]) {
+    const int64_t left = outer < outers ? inner_end - inner : 0;
+    const T* p = base + outer * ld + inner;
+    constexpr int N = Wide<T>::N;
+#pragma unroll
+    for (int h = 0; h < 8 / N; ++h) {
+        float u[N];
+        if (left >= (h + 1) * N) load_wide<T>(p + h * N, u);
+        else
+#pragma unroll
+            for (int j = 0; j < N; ++j) u[j] = left > h * N + j ? to_f(p[h * N + j]) : 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[h * N + j] = u[j];
+    }
+}
+
+// RC: the summed index is the contiguous one.  (i0, r0): the tile's corner.
+template <typename T, bool RC>
+__device__ __forceinline__ void fetch_tile(int t, const T* base, int64_t ld, int64_t i0, int64_t i_end, int64_t r0, int64_t r_end, float (&v)[8]) {
+    if (RC) fetch8<T>(base, ld, i0 + t / 4, i_end, r0 + t % 4 * 8, r_end, v);
+    else fetch8<T>(base, ld, r0 + t / 8, r_end, i0 + t % 8 * 8, i_end, v);
+}
+// ERR: what rounding to T leaves of them
+template <typename T, bool RC, bool ERR = false>
+__device__ __forceinline__ void put_tile(int t, T* lds, const float (&u)[8]) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float r = to_f(from_f<T>(u[j]));
+        v[j] = !ERR ? u[j] : fabsf(r) < __builtin_inff() ? u[j] - r : 0.f;       // (infinities and NaN are whole in the first number)
+    }
+    constexpr int LD = Lds<T>::LD;
+    if (RC) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lds[(t / 4) * LD + t % 4 * 8 + j] = from_f<T>(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lds[(t % 8 * 8 + j) * LD + t / 8] = from_f<T>(v[j]);
+    }
+}
+
+__device__ __forceinline__ f32x4 mma32(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma32(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+template <typename T> struct V8;
+template <> struct V8<bf16_t> { typedef bf16x8 t; };
+template <> struct V8<f16_t> { typedef f16x8 t; };
+
+// one TR-long step of a wave's 32 x 32 part
+template <typename T>
+__device__ __forceinline__ void tile_mma(int t, const T* lp, const T* lq, f32x4 (&acc)[2][2]) {
+    typedef typename V8<T>::t v8;
+    const int l = t % 64, w = t / 64, row = l % 16, r = l / 16 * 8;
+    constexpr int LD = Lds<T>::LD;
+    v8 p[2], q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        p[i] = *(const v8*)(lp + (w / 2 * 32 + i * 16 + row) * LD + r);
+        q[i] = *(const v8*)(lq + (w % 2 * 32 + i * 16 + row) * LD + r);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mma32(q[j], p[i], acc[i][j]);
+}
+template <>
+__device__ __forceinline__ void tile_mma<float>(int t, const float* lp, const float* lq, f32x4 (&acc)[2][2]) {
+    const int l = t % 64, w = t / 64, row = l % 16, r = l / 16 * 4;
+    constexpr int LD = Lds<float>::LD;
+#pragma unroll
+    for (int b = 0; b < TR; b += 16) {
+        f32x4 p[2], q[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            p[i] = *(const f32x4*)(lp + (w / 2 * 32 + i * 16 + row) * LD + b + r);
+            q[i] = *(const f32x4*)(lq + (w % 2 * 32 + i * 16 + row) * LD + b + r);
+        }
+        // step e takes element e of each lane group's four: the same permutation of the summed index on both sides
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[j][e], p[i][e], acc[i][j], 0, 0, 0);
+    }
+}
+
+// The tile at (p0, q0), whole or (S.splits > 1) its part over a split of R.  256 threads, numbered t; several such groups of a block may run
+// together if they all walk the same R.  A tile outside the matrix stores nothing.
+template <typename T, int MODE>
+__device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinSplit& S, int64_t split, int64_t p0, int64_t q0, float* part, float* part_db,
+                                             T* lp, T* lq, T* le, float* lsum) {
+    const int64_t P = MODE == MODE_DW ? A.N : A.M, Q = MODE == MODE_FWD ? A.N : A.K, R = MODE == MODE_FWD ? A.K : MODE == MODE_DX ? A.N : A.M;
+    const int64_t ra = split * S.len, rb = ra + S.len < R ? ra + S.len : R;
+    const T* x = (const T*)A.x;
+    const T* w = (const T*)A.w;
+    const T* dy = (const T*)A.dy;
+    typedef typename Pre<T>::t pre_t;
+    const pre_t* pre = (const pre_t*)A.cpre;
+
+    float vp[8], vq[8], sum[8] = {};
+    auto fetch = [&](int64_t r0) {
+        if constexpr (MODE == MODE_FWD) {
+            fetch_tile<T, true>(t, x, A.ldx, p0, P, r0, rb, vp);
+            fetch_tile<T, true>(t, w, A.K, q0, Q, r0, rb, vq);
+        } else {
+            constexpr bool RC = MODE == MODE_DX;
+            fetch_tile<T, RC>(t, dy, A.lddy, p0, P, r0, rb, vp);
+            if (A.act != IVAE_ACT_NONE) {
+                float s[8];
+                fetch_tile<pre_t, RC>(t, pre, A.N, p0, P, r0, rb, s);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) vp[j] *= lin_act_slope<T>(A.act, A.slope, s[j]);
+            }
+            if (MODE == MODE_DW)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += vp[j];
+            if (MODE == MODE_DX) fetch_tile<T, false>(t, w, A.K, q0, Q, r0, rb, vq);
+            else fetch_tile<T, false>(t, x, A.ldx, q0, Q, r0, rb, vq);
+        }
+    };
+    f32x4 acc[2][2] = {};
+    if (ra < rb) fetch(ra);
+    for (int64_t r = ra; r < rb; r += TR) {
+        __syncthreads();
+        put_tile<T, MODE != MODE_DW>(t, lp, vp);
+        put_tile<T, MODE == MODE_FWD>(t, lq, vq);
+        const bool two = sizeof(T) == 2 && MODE != MODE_FWD && A.act != IVAE_ACT_NONE;
+        if (two) put_tile<T, MODE != MODE_DW, true>(t, le, vp);
+        __syncthreads();
+        if (r + TR < rb) fetch(r + TR);
+        tile_mma<T>(t, lp, lq, acc);
+        if (two) tile_mma<T>(t, le, lq, acc);
+    }
+    const int l = t % 64, wv = t / 64;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t p = p0 + wv / 2 * 32 + i * 16 + l % 16, q = q0 + wv % 2 * 32 + j * 16 + l / 16 * 4 + e;
+                if (p >= P || q >= Q) continue;
+                if (S.splits > 1) part[(split * P + p) * Q + q] = acc[i][j][e];
+                else if (MODE == MODE_FWD) forward_store<T>(A, p, (int)q, acc[i][j][e]);
+                else if (MODE == MODE_DX) ((T*)A.dx)[p * Q + q] = from_f<T>(acc[i][j][e]);
+                else if (A.dw) ((T*)A.dw)[p * Q + q] = from_f<T>(acc[i][j][e]);
+            }
+    if (MODE == MODE_DW && A.db && q0 == 0) {       // thread t holds the sums of 8 columns over every 32nd row: 32 threads hold each column
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lsum[(t / 8) * TP + t % 8 * 8 + j] = sum[j];
+        __syncthreads();
+        if (t < TP && p0 + t < P) {
+            float s = 0.f;
+            for (int i = 0; i < 32; ++i) s += lsum[i * TP + t];
+            if (S.splits > 1) part_db[split * P + p0 + t] = s;
+            else ((T*)A.db)[p0 + t] = from_f<T>(s);
+        }
+    }
+    __syncthreads();                                // the tiles are free for the next round
+}
