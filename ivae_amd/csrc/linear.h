@@ -74,6 +74,23 @@ __device__ __forceinline__ float lin_act_slope(int act, float slope, float s) {
     }
 }
 
+// over N values, the switch outside of the loop over them
+template <typename T, int N> __device__ __forceinline__ void lin_act_all(int act, float slope, float (&v)[N]) {
+    switch (act) {
+#define EACH(ID) case ID: _Pragma("unroll") for (int e = 0; e < N; ++e) v[e] = lin_act<T>(ID, slope, v[e]); break;
+        EACH(IVAE_ACT_LRELU) EACH(IVAE_ACT_XTANH) EACH(IVAE_ACT_SIGMOID) EACH(IVAE_ACT_GELU) EACH(IVAE_ACT_SILU)
+#undef EACH
+    }
+}
+// v *= act'(s)
+template <typename T, int N> __device__ __forceinline__ void lin_act_slope_all(int act, float slope, const float (&s)[N], float (&v)[N]) {
+    switch (act) {
+#define EACH(ID) case ID: _Pragma("unroll") for (int e = 0; e < N; ++e) v[e] *= lin_act_slope<T>(ID, slope, s[e]); break;
+        EACH(IVAE_ACT_LRELU) EACH(IVAE_ACT_XTANH) EACH(IVAE_ACT_SIGMOID) EACH(IVAE_ACT_GELU) EACH(IVAE_ACT_SILU)
+#undef EACH
+    }
+}
+
 // what follows the sum of one result of the forward pass
 template <typename T>
 __device__ __forceinline__ void forward_store(const LinArgs& A, int64_t m, int n, float s) {

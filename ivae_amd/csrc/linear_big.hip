@@ -118,17 +118,21 @@ __device__ __forceinline__ typename E8<E>::t read_frag(uint32_t lds, int off) {
     }
 }
 
-// 8 neighbouring values, `n` of them inside the matrix
-template <typename T> __device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
-    constexpr int N = Wide<T>::N;
+// 8 neighbouring values as they lie in memory, `n` of them inside the matrix
+template <typename T> struct Raw8 {
+    Vec<T> v[8 / Wide<T>::N];
+    __device__ __forceinline__ void load(const T* p, int n) {
+        constexpr int N = Wide<T>::N;
 #pragma unroll
-    for (int h = 0; h < 8 / N; ++h) {
-        float u[N];
-        load_some<T>(p + h * N, n - h * N, u);
+        for (int h = 0; h < 8 / N; ++h) {
+            if (n >= (h + 1) * N) v[h] = *(const Vec<T>*)(p + h * N);
+            else
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[h * N + j] = u[j];
+                for (int j = 0; j < N; ++j) v[h].e[j] = n > h * N + j ? p[h * N + j] : (T)0.f;
+        }
     }
-}
+    __device__ __forceinline__ float at(int e) const { return to_f(v[e / Wide<T>::N].e[e % Wide<T>::N]); }
+};
 template <typename T> __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
     constexpr int N = Wide<T>::N;
 #pragma unroll
@@ -170,16 +174,39 @@ template <int BTP, int BTQ> __device__ __forceinline__ Place place(const BigProd
     return r;
 }
 
-// The sums go through LDS, 128 rows of the tile at a time, so that what follows runs along whole rows: 16-byte loads of the residual
-// and stores of the results, side by side, and one copy of the code for them.
+// The sums go through LDS, up to 128 rows of the tile at a time, so that what follows runs along whole rows: 16-byte loads of the residual
+// (two rows ahead of their use) and stores of the results, side by side, and one copy of the code for them.
 template <typename T, int BTP, int BTQ, int WP, int WQ, int EPI, int FP, int FQ>
 __device__ __forceinline__ void finish(const BigProduct& G, const LinArgs& A, const Place& at0, const f32x4 (&acc)[FP][FQ], float* sums) {
-    constexpr int THREADS = WP * WQ * 64, HALVES = BTP / 128, LD = BTQ + 4, RW = 16 * FP / HALVES;      // RW rows of each row of waves
-    static_assert(WP * RW == 128 && FP % HALVES == 0, "128 rows a pass");
+    constexpr int THREADS = WP * WQ * 64, ROWS = BTP < 128 ? BTP : 128, HALVES = BTP / ROWS, LD = BTQ + 4;
+    constexpr int RW = 16 * FP / HALVES, STEP = THREADS / (BTQ / 8), ITERS = ROWS / STEP;          // RW rows of each row of waves
+    static_assert(WP * RW == ROWS && FP % HALVES == 0 && ITERS * STEP == ROWS, "whole passes");
     const int wave = threadIdx.x / 64, l = threadIdx.x % 64, wq = wave % WQ * (BTQ / WQ);
-    const int64_t Q = G.q_end;
+    const int col = threadIdx.x % (BTQ / 8) * 8, row0 = threadIdx.x / (BTQ / 8);
+    const int64_t Q = G.q_end, q = at0.q0 + col, left = Q - q;
+    const int n = left >= 8 ? 8 : left > 0 ? (int)left : 0;
+    const bool fwd = EPI == EPI_FWD && G.splits == 1, res = fwd && A.res;
+    float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (fwd && A.b) {
+        Raw8<T> b;
+        b.load((const T*)A.b + q, n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bias[e] = b.at(e);
+    }
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) {
+        auto p_of = [&](int it) {
+            const int row = row0 + it * STEP;
+            return at0.p0 + (HALVES == 1 ? row : row / RW * (BTP / WP) + h * RW + row % RW);
+        };
+        auto load_res = [&](int it) {
+            Raw8<T> r;
+            const int64_t p = p_of(it);
+            r.load((const T*)A.res + p * A.ldr + q, it < ITERS && p < G.p_end ? n : 0);
+            return r;
+        };
+        Raw8<T> r0, r1;
+        if (res) r0 = load_res(0), r1 = load_res(1);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < FP / HALVES; ++i)
@@ -188,44 +215,39 @@ __device__ __forceinline__ void finish(const BigProduct& G, const LinArgs& A, co
                 *(f32x4*)(sums + (wave / WQ * RW + i * 16 + l % 16) * LD + wq + j * 16 + l / 16 * 4) = acc[h * (FP / HALVES) + i][j];
         __syncthreads();
 #pragma unroll 1
-        for (int c = threadIdx.x; c < 128 * (BTQ / 8); c += THREADS) {
-            const int row = c / (BTQ / 8), col = c % (BTQ / 8) * 8;
-            const int64_t p = at0.p0 + row / RW * (BTP / WP) + h * RW + row % RW, q = at0.q0 + col;
-            if (p >= G.p_end || q >= Q) continue;
-            const int n = Q - q < 8 ? (int)(Q - q) : 8;
+        for (int it = 0; it < ITERS; ++it) {
+            Raw8<T> r2;
+            if (res) r2 = load_res(it + 2);
+            const int64_t p = p_of(it), at = p * Q + q;
+            const float* from = sums + (row0 + it * STEP) * LD + col;
             float v[8];
-            load8(sums + row * LD + col, 8, v);
-            const int64_t at = p * Q + q;
-            if (G.splits > 1) {
-                store8(G.part + (int64_t)at0.split * G.p_end * Q + at, n, v);
-            } else if (EPI == EPI_FWD) {
-                typedef typename Pre<T>::t pre_t;
-                float u[8];
-                if (A.b) {
-                    load8((const T*)A.b + q, n, u);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] += u[e];
-                }
-                if (A.pre) {
+            for (int e = 0; e < 8; ++e) v[e] = from[e] + bias[e];
+            const int m = p < G.p_end ? n : 0;
+            if (fwd) {
+                if (A.pre && m) {
+                    typedef typename Pre<T>::t pre_t;
                     struct __attribute__((packed, aligned(sizeof(pre_t)))) { pre_t e[8]; } s;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) s.e[e] = pre_pack(v[e], pre_t());
                     pre_t* to = (pre_t*)A.pre + at;
-                    if (n == 8) *(decltype(s)*)to = s;
+                    if (m == 8) *(decltype(s)*)to = s;
                     else
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            if (e < n) to[e] = s.e[e];
+                            if (e < m) to[e] = s.e[e];
                 }
+                lin_act_all<T>(A.act, A.slope, v);
+                if (res)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = lin_act<T>(A.act, A.slope, v[e]);
-                if (A.res) {
-                    load8((const T*)A.res + p * A.ldr + q, n, u);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] += u[e];
-                }
-                store8((T*)A.y + at, n, v);
-            } else store8((T*)G.out + at, n, v);
+                    for (int e = 0; e < 8; ++e) v[e] += r0.at(e);
+                if (m) store8((T*)A.y + at, m, v);
+            } else if (m) {
+                if (G.splits > 1) store8(G.part + (int64_t)at0.split * G.p_end * Q + at, m, v);
+                else store8((T*)G.out + at, m, v);
+            }
+            r0 = r1;
+            r1 = r2;
         }
     }
 }

@@ -54,8 +54,7 @@ __global__ __launch_bounds__(256) void k_pack(PackJobs J) {
 #pragma unroll
                 for (int j = 0; j < NP; ++j) s[h * NP + j] = u[j];
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= lin_act_slope<T>(A.act, A.slope, s[j]);
+            lin_act_slope_all<T>(A.act, A.slope, s, v);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += v[j];

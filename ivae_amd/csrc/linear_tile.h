@@ -132,8 +132,7 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
             if (A.act != IVAE_ACT_NONE) {
                 float s[8];
                 fetch_tile<pre_t, RC>(t, pre, A.N, p0, P, r0, rb, s);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) vp[j] *= lin_act_slope<T>(A.act, A.slope, s[j]);
+                lin_act_slope_all<T>(A.act, A.slope, s, vp);
             }
             if (MODE == MODE_DW)
 #pragma unroll
