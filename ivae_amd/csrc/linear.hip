@@ -15,9 +15,6 @@ static LinArgs lin_args(const IvaeLinear& L) {
 // ---- large products -------------------------------------------------------------------------------------------------
 static const int64_t BIG_MAX_LD = 1 << 21;              // 32-bit byte offsets inside a tile of 256 rows
 
-static bool big_product(int64_t P, int64_t Q, int64_t R) {
-    return P >= 64 && Q >= 64 && R >= 64 && 2.0 * (double)P * (double)Q * (double)R >= 5e8;
-}
 static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 static int64_t tiles_of(const BigProduct& B, int tp, int tq) { return ((B.p_end + tp - 1) / tp) * ((B.q_end + tq - 1) / tq); }
 // Tiles and splits of the products of one launch: the choice for which a simple model of its time is least.  A block takes `start` us and
@@ -135,7 +132,7 @@ static BigBackward plan_big_backward(const LinArgs& A, int dtype, void* ws) {
     if (!f.ds.needed) {                                 // dy itself; only its column sums are taken
         f.ds.P.src = A.dy; f.ds.P.rows = A.M; f.ds.P.cols = A.N; f.ds.P.ld = A.lddy; f.ds.P.ldo = A.N;
     }
-    f.kb = pack_row_blocks(A.M, f.ds.P.ldo);
+    f.kb = pack_row_blocks(A.M, f.ds.P.ldo, true);
     f.colsum = m.take<float>((int64_t)f.kb * A.N);
     f.x = pack_of(A.x, A.M, A.K, A.ldx, dtype, m);
     f.w = pack_of(A.w, A.N, A.K, A.K, dtype, m);
@@ -171,11 +168,21 @@ static hipError_t big_backward(const LinArgs& A, int dtype, void* ws, hipStream_
 
 // ---- which kernel -----------------------------------------------------------------------------------------------------
 static bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
-static bool big_by_size(const LinArgs& A) {
+// The large kernels from the size on from which they take less time, all their launches together (us, small | large):
+//   16 bits, forward    1024 x 512 x 512 14 | 15, 2048 x 512 x 1024 20 | 16, 2048 x 1024 x 1024 31 | 21, 128 x 4096 x 4096 36 | 23
+//   16 bits, backward   128 x 512 x 512 21 | 16, 1024 x 512 x 512 33 | 22, 1024 x 1024 x 1024 85 | 29 (but the small kernel does not round
+//                       act' dy: it keeps what it loses little by)
+//   fp32, forward       1024 x 1024 x 1024 34 | 42, 2048 x 1024 x 1024 52 | 55, 300 x 4096 x 2048 82 | 76, 128 x 4096 x 4096 53 | 77
+//                       (cutting the weight in three costs as much as a product with 128 rows)
+//   fp32, backward      512 x 512 x 512 31 | 31, 1024 x 512 x 512 39 | 35, 1024 x 1024 x 1024 108 | 51
+static bool big_by_size(const LinArgs& A, int dtype, bool backward) {
     const int64_t lds[] = {A.ldx, A.lddy, A.K, A.N};
     for (int64_t ld : lds)
         if (ld > BIG_MAX_LD) return false;
-    return A.M < 1 << 29 && big_product(A.M, A.N, A.K);        // (blocks are counted in 32 bits)
+    if (A.M < 64 || A.N < 64 || A.K < 64 || A.M >= 1 << 29) return false;      // (blocks are counted in 32 bits)
+    const double flops = 2.0 * (double)A.M * (double)A.N * (double)A.K;
+    if (dtype == IVAE_F32) return backward ? flops >= 5e8 : flops >= 5e9 && A.M >= 256;
+    return flops >= (backward ? 1e8 : 1.5e9);
 }
 // a matrix that would be loaded in place has to start on 16 bytes
 static bool big_in_place(const void* p, int64_t cols, int64_t ld, int dtype) { return dtype == IVAE_F32 || ld % 8 || cols % 8 || aligned(p); }
@@ -185,7 +192,7 @@ size_t linear_ws_bytes(const IvaeLinear& L, bool backward) {
     A.dx = A.dw = A.db = &A;           // the size serves a call that asks for all of them
     if (!backward && A.M <= ROWS_MAX) return rows_ws(A);
     size_t n = linear_small_ws(A, backward);
-    if (big_by_size(A)) {
+    if (big_by_size(A, L.dtype, backward)) {
         const size_t big = backward ? plan_big_backward(A, L.dtype, nullptr).bytes : plan_big_forward(A, L.dtype, nullptr).bytes;
         if (big > n) n = big;
     }
@@ -196,7 +203,7 @@ hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, cons
     LinArgs A = lin_args(L);
     A.x = x; A.w = w; A.b = b; A.res = residual; A.y = y; A.pre = saved; A.part = (float*)ws;
     if (A.M <= ROWS_MAX) return linear_rows_forward(A, L.dtype, st);
-    if (big_by_size(A) && big_in_place(x, A.K, A.ldx, L.dtype) && big_in_place(w, A.K, A.K, L.dtype) && aligned(ws))
+    if (big_by_size(A, L.dtype, false) && big_in_place(x, A.K, A.ldx, L.dtype) && big_in_place(w, A.K, A.K, L.dtype) && aligned(ws))
         return big_forward(A, L.dtype, ws, st);
     return linear_small_forward(A, L.dtype, st);
 }
@@ -204,7 +211,7 @@ hipError_t launch_linear_backward(const IvaeLinear& L, const void* dy, const voi
                                   void* db, void* ws, hipStream_t st) {
     LinArgs A = lin_args(L);
     A.x = x; A.w = w; A.dy = dy; A.cpre = saved; A.dx = dx; A.dw = dw; A.db = db; A.part = (float*)ws;
-    if (big_by_size(A) && (A.act != IVAE_ACT_NONE || big_in_place(dy, A.N, A.lddy, L.dtype)) && (!dw || big_in_place(x, A.K, A.ldx, L.dtype)) &&
+    if (big_by_size(A, L.dtype, true) && (A.act != IVAE_ACT_NONE || big_in_place(dy, A.N, A.lddy, L.dtype)) && (!dw || big_in_place(x, A.K, A.ldx, L.dtype)) &&
         (!dx || big_in_place(w, A.K, A.K, L.dtype)) && aligned(ws))
         return big_backward(A, L.dtype, ws, st);
     return linear_small_backward(A, L.dtype, st);

@@ -16,5 +16,5 @@ struct PackArgs {
     int flip;                   // fp32: every second run of 32 rows (FLIP_ROWS) or columns (FLIP_COLS) with its sign turned
     int group, blocks_x, blocks;    // set by the launcher
 };
-int pack_row_blocks(int64_t rows, int64_t width);       // of a launch with ldo = width: rows of colsum
+int pack_row_blocks(int64_t rows, int64_t width, bool colsum);  // of a job with ldo = width: rows of its colsum
 hipError_t launch_packs(const PackArgs* const* P, int n, int dtype, hipStream_t st);    // up to three in one launch; null: none

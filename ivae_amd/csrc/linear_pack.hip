@@ -96,11 +96,12 @@ static int group_of(int64_t width) {                    // a power of two: 8 * g
     while (g < 64 && g * 8 < width) g *= 2;
     return g;
 }
-// blocks along the rows: about 2048 blocks in all, and then more rows a thread
-int pack_row_blocks(int64_t rows, int64_t width) {
+// blocks along the rows: about 2048 blocks in all, and then more rows a thread; with column sums at most 256, whose sums are joined
+int pack_row_blocks(int64_t rows, int64_t width, bool colsum) {
     const int g = group_of(width);
     const int64_t strips = (width + g * 8 - 1) / (g * 8), subs = 256 / g;
     int64_t y = (rows + subs - 1) / subs, most = 2048 / strips;
+    if (colsum && most > 256) most = 256;
     if (y > most) y = most;
     return (int)(y < 1 ? 1 : y);
 }
@@ -112,7 +113,7 @@ hipError_t launch_packs(const PackArgs* const* P, int n, int dtype, hipStream_t 
         PackArgs& A = J.job[jobs++] = *P[i];
         A.group = group_of(A.ldo);
         A.blocks_x = (int)((A.ldo + A.group * 8 - 1) / (A.group * 8));
-        A.blocks = A.blocks_x * pack_row_blocks(A.rows, A.ldo);
+        A.blocks = A.blocks_x * pack_row_blocks(A.rows, A.ldo, A.colsum != nullptr);
         blocks += A.blocks;
     }
     if (blocks == 0) return hipSuccess;
