@@ -38,7 +38,10 @@ build/asan_%.o: $(CSRC)/%.hip $(HDRS)
 build/abi_asan: $(ASANOBJS) tests/host/abi_asan.c
 	gcc -O1 -g -fsanitize=address,undefined -fno-sanitize-recover=undefined -c tests/host/abi_asan.c -o build/abi_asan_main.o
 	$(HIPCC) --offload-arch=$(ARCH) -fsanitize=address,undefined -fno-gpu-sanitize build/abi_asan_main.o $(ASANOBJS) -o $@
-asan: build/abi_asan
+build/abi_asan_ops: $(ASANOBJS) tests/host/abi_asan_ops.c
+	gcc -O1 -g -fsanitize=address,undefined -fno-sanitize-recover=undefined -c tests/host/abi_asan_ops.c -o build/abi_asan_ops_main.o
+	$(HIPCC) --offload-arch=$(ARCH) -fsanitize=address,undefined -fno-gpu-sanitize build/abi_asan_ops_main.o $(ASANOBJS) -o $@
+asan: build/abi_asan build/abi_asan_ops
 
 clean:
 	rm -f $(OBJS) $(LIB)

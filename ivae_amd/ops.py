@@ -428,6 +428,12 @@ def _matrix(t):
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
+def _aligned(t):
+    """t, copied where it starts off a 16-byte boundary and is large: the kernels of large products load matrices in place, 16 bytes at
+    a time, and the library takes the kernel for any alignment otherwise."""
+    return t.clone() if t.data_ptr() & 15 and t.numel() >= 1 << 16 else t
+
+
 def _call(dev, fn, what, *args):
     """fn(*args, stream) with `dev` current."""
     i = dev.index
@@ -479,8 +485,8 @@ def linear(x, weight, bias=None, activation="none", slope=.1, residual=None, sav
     out = x.shape[:-1] + (n,)
     if bias is not None:
         bias = _dense(_like(bias, x, "bias", (n,)))
-    x, ldx = _matrix(x)
-    weight = _dense(weight)
+    x, ldx = _matrix(_aligned(x))
+    weight = _aligned(_dense(weight))
     ldr = 0
     if residual is not None:
         residual, ldr = _matrix(_like(residual, x, "residual", out))
@@ -507,9 +513,9 @@ def linear_backward(dy, x, weight, saved=None, activation="none", slope=.1, need
     else:
         saved = None
     shape = x.shape
-    x, ldx = _matrix(x)
-    dy, lddy = _matrix(dy)
-    weight = _dense(weight)
+    x, ldx = _matrix(_aligned(x))
+    dy, lddy = _matrix(_aligned(dy))
+    weight = _aligned(_dense(weight))
     dev = x.device
     lin, nb = _linear_plan(rows, k, n, dt, act, float(slope), ldx, 0, lddy, 1)
     dx = x.new_empty(shape) if need[0] else None

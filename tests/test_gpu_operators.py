@@ -182,6 +182,67 @@ def test_linear_large_keeps_nan_and_infinities(dt, m, k, n):
     assert float(db[6]) == -float("inf")
 
 
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_linear_large_misaligned(dt):
+    """Dense matrices that start off a 16-byte boundary, and rows at one whose first element is off it."""
+    g = torch.Generator().manual_seed(14)
+    m, k, n = 1024, 1024, 768
+    mats = []
+    for r, c in ((m, k), (n, k), (m, n)):
+        t = torch.randint(-3, 4, (r, c), generator=g).to(dt)
+        flat = torch.empty(r * c + 1, dtype=dt, device=dev())
+        flat[1:].view(r, c).copy_(t.to(dev()))
+        mats.append(flat[1:].view(r, c))
+        wide = torch.zeros(r, c + 16, dtype=dt, device=dev())
+        wide[:, 3:3 + c].copy_(t.to(dev()))
+        mats.append(wide[:, 3:3 + c])
+    for x, w, dy in (mats[0::2], mats[1::2]):
+        X, W, D = x.double(), w.double(), dy.double()
+        assert x.data_ptr() % 16 and torch.equal(ops.linear(x, w), (X @ W.t()).to(dt))
+        for got, want in zip(ops.linear_backward(dy, x, w), (D @ W, D.t() @ X, D.sum(0))):
+            assert torch.equal(got, want.to(dt))
+
+
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_linear_large_on_two_streams_and_in_graphs(dt):
+    """Large calls at once on two streams, and two graphs captured from them and replayed together, give what one call alone gives."""
+    g = torch.Generator().manual_seed(15)
+    m, k, n = 1500, 1016, 1200
+    sets = [tuple(normal(g, *s, scale=.2, dtype=dt).to(dev()) for s in ((m, k), (n, k), (m, n))) for _ in range(2)]
+
+    def step(s):
+        y, saved = ops.linear(s[0], s[1], None, "silu", residual=s[2], save=True)
+        return y, *ops.linear_backward(s[2], s[0], s[1], saved, "silu")
+    want = [[t.clone() for t in step(s)] for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        got = []
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(step(s))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+        del got
+    graphs, outs = [], []
+    for s, st in zip(sets, streams):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=st):
+            outs.append(step(s))
+        graphs.append(gr)
+    for _ in range(3):
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(outs, want) for a, b in zip(x, y))
+        step(sets[0])
+
+
 def test_linear_fp32_range():
     """The three parts of a value keep its range: products near both ends of fp32's."""
     g = torch.Generator().manual_seed(13)

@@ -1,5 +1,8 @@
 """What the tensor operators refuse, without a GPU: the C entries' codes, the Python checks, and the oracle itself."""
 import ctypes as C
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -163,3 +166,16 @@ def test_mlp_options():
         MLP(3, 2, 8, 3, activation="gelu")               # the torch path keeps the reference's activations
     with pytest.raises(ValueError):
         MLP(3, 2, 8, 3, dropout=1.5)
+
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.skipif(not (shutil.which("hipcc") or os.path.exists("/opt/rocm/bin/hipcc")), reason="needs hipcc to build")
+def test_host_paths_are_clean_under_asan_and_ubsan():
+    """Every choice that the host makes for a call (kernel, tiles, splits, pieces of the workspace), over random shapes, instrumented."""
+    b = subprocess.run(["make", "-j8", "build/abi_asan_ops"], cwd=ROOT, capture_output=True, text=True, timeout=900)
+    assert b.returncode == 0, b.stdout[-2000:] + b.stderr[-2000:]
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=0:abort_on_error=0", UBSAN_OPTIONS="print_stacktrace=1")
+    r = subprocess.run([os.path.join(ROOT, "build", "abi_asan_ops")], cwd=ROOT, capture_output=True, text=True, timeout=600, env=env)
+    assert r.returncode == 0 and "abi_asan_ops: OK" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
