@@ -91,7 +91,54 @@ template <typename T, int N> __device__ __forceinline__ void lin_act_slope_all(i
     }
 }
 
-// what follows the sum of one result of the forward pass
+// 8 neighbouring values as they lie in memory, `n` of them inside the matrix
+template <typename T> struct Raw8 {
+    Vec<T> v[8 / Wide<T>::N];
+    __device__ __forceinline__ void load(const T* p, int n) {
+        constexpr int N = Wide<T>::N;
+#pragma unroll
+        for (int h = 0; h < 8 / N; ++h) {
+            if (n >= (h + 1) * N) v[h] = *(const Vec<T>*)(p + h * N);
+            else
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[h].e[j] = n > h * N + j ? p[h * N + j] : (T)0.f;
+        }
+    }
+    __device__ __forceinline__ float at(int e) const { return to_f(v[e / Wide<T>::N].e[e % Wide<T>::N]); }
+};
+template <typename T> __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
+    constexpr int N = Wide<T>::N;
+#pragma unroll
+    for (int h = 0; h < 8 / N; ++h) {
+        float u[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) u[j] = v[h * N + j];
+        store_some<T>(p + h * N, n - h * N, u);
+    }
+}
+
+// What follows the sums of 8 neighbouring results (bias included, n of them inside the matrix, the first at element `at` of y).
+template <typename T>
+__device__ __forceinline__ void forward_store8(const LinArgs& A, int64_t at, int n, float (&v)[8], const Raw8<T>* res) {
+    typedef typename Pre<T>::t pre_t;
+    if (A.pre && n) {
+        struct __attribute__((packed, aligned(sizeof(pre_t)))) { pre_t e[8]; } s;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s.e[e] = pre_pack(v[e], pre_t());
+        pre_t* to = (pre_t*)A.pre + at;
+        if (n == 8) *(decltype(s)*)to = s;
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < n) to[e] = s.e[e];
+    }
+    lin_act_all<T>(A.act, A.slope, v);
+    if (res)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += res->at(e);
+    if (n) store8((T*)A.y + at, n, v);
+}
+// what follows the sum of one result
 template <typename T>
 __device__ __forceinline__ void forward_store(const LinArgs& A, int64_t m, int n, float s) {
     if (A.b) s += to_f(((const T*)A.b)[n]);

@@ -19,7 +19,7 @@ static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 static int64_t tiles_of(const BigProduct& B, int tp, int tq) { return ((B.p_end + tp - 1) / tp) * ((B.q_end + tq - 1) / tq); }
 // Tiles and splits of the products of one launch: the choice for which a simple model of its time is least.  A block takes `start` us and
 // `per` ns for each of its summed index (measured: a 256 x 256 tile of 16-bit values 27 ns, bound by the matrix cores; a 128 x 128
-// tile 17 ns, bound by the latency of its loads; split fp32 82 and 46 ns); blocks beyond one a CU queue up; split sums are written,
+// tile 17 ns, bound by the latency of its loads; split fp32 82 and 60 ns); blocks beyond one a CU queue up; split sums are written,
 // read and joined at 4 TB/s and one more launch.
 struct BigModel { int tile_p, tile_q; double start, per; int slots; };
 static double big_time(BigProduct** B, int n, const BigModel& m, const int64_t* s) {
@@ -37,7 +37,7 @@ static double big_time(BigProduct** B, int n, const BigModel& m, const int64_t* 
 }
 static void big_geometry(BigProduct** B, int n, int dtype) {
     static const BigModel m16[2] = {{256, 256, 10.0, 27.0, 256}, {128, 128, 4.0, 17.0, 256}};
-    static const BigModel m32[2] = {{256, 128, 10.0, 82.0, 256}, {128, 128, 5.0, 46.0, 256}};
+    static const BigModel m32[2] = {{256, 128, 10.0, 82.0, 256}, {128, 128, 5.0, 60.0, 256}};
     double best = 1e30;
     for (const BigModel& m : dtype == IVAE_F32 ? m32 : m16)
         for (int64_t s0 = 1; s0 <= 16; s0 *= 2)
@@ -76,10 +76,10 @@ static Packed pack_of(const void* src, int64_t rows, int cols, int64_t ld, int d
         r.P.ldo = cols;
         return r;
     }
-    const int64_t ldo = up(cols, 64), plane = rows * ldo;
+    const int64_t ldo = up(cols, 64), plane = rows * ldo;           // (fp32: columns of 32, `rows` long each)
     void* out = ws.take<uint16_t>(plane * (dtype == IVAE_F32 ? 3 : 1));
     r.P.src = src; r.P.out = out; r.P.rows = rows; r.P.cols = cols; r.P.ld = ld; r.P.ldo = ldo; r.P.plane = plane;
-    r.O = {out, ldo, 0, 0, plane, false};
+    r.O = {out, dtype == IVAE_F32 ? rows : ldo, 0, 0, plane, false};
     return r;
 }
 // rows are what the product has as rows or columns, the summed index runs along them / down the rows
@@ -132,7 +132,7 @@ static BigBackward plan_big_backward(const LinArgs& A, int dtype, void* ws) {
     if (!f.ds.needed) {                                 // dy itself; only its column sums are taken
         f.ds.P.src = A.dy; f.ds.P.rows = A.M; f.ds.P.cols = A.N; f.ds.P.ld = A.lddy; f.ds.P.ldo = A.N;
     }
-    f.kb = pack_row_blocks(A.M, f.ds.P.ldo, true);
+    f.kb = pack_row_blocks(A.M, f.ds.P.ldo, true, dtype);
     f.colsum = m.take<float>((int64_t)f.kb * A.N);
     f.x = pack_of(A.x, A.M, A.K, A.ldx, dtype, m);
     f.w = pack_of(A.w, A.N, A.K, A.K, dtype, m);
@@ -179,7 +179,8 @@ static bool big_by_size(const LinArgs& A, int dtype, bool backward) {
     const int64_t lds[] = {A.ldx, A.lddy, A.K, A.N};
     for (int64_t ld : lds)
         if (ld > BIG_MAX_LD) return false;
-    if (A.M < 64 || A.N < 64 || A.K < 64 || A.M >= 1 << 29) return false;      // (blocks are counted in 32 bits)
+    // (blocks are counted, and bytes inside a tile of fp32 columns offset, in 32 bits)
+    if (A.M < 64 || A.N < 64 || A.K < 64 || A.M >= (dtype == IVAE_F32 ? 1 << 22 : 1 << 29)) return false;
     const double flops = 2.0 * (double)A.M * (double)A.N * (double)A.K;
     if (dtype == IVAE_F32) return backward ? flops >= 5e8 : flops >= 5e9 && A.M >= 256;
     return flops >= (backward ? 1e8 : 1.5e9);

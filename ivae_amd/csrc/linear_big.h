@@ -4,7 +4,9 @@
 
 // One operand of a product C[p][q] = sum_r P(p, r) Q(q, r), in memory as a row-major 16-bit matrix.
 //   along = true:  (extent, R): the summed index runs along a row;   along = false: (R, extent): it runs down the rows
-// Rows start at multiples of 16 bytes and hold whole 16-byte groups; `limit` is the end of the stored values along R (a multiple
+// Rows start at multiples of 16 bytes and hold whole 16-byte groups.  Split fp32 is stored in columns of 32 values, ld rows each
+// (value (r, c) at (c / 32 * ld + r) * 32 + c % 32): what a step loads of a tile lies in one piece, or (down) in pieces of 2 KB, where
+// rows of 64 bytes out of a row-major matrix would use half of each cache line.  `limit` is the end of the stored values along R (a multiple
 // of 8 where `along`; values between R and limit are 0).  Split fp32: of every second 32 along R, Q has its sign turned.  `plane`: elements between the three parts of split fp32 values.
 struct BigOperand {
     const void* base;

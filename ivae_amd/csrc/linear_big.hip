@@ -29,9 +29,10 @@ template <> struct E8<f16_t> { typedef f16x8 t; };
 __device__ const uint4 g_zeros = {0, 0, 0, 0};          // where lanes beyond the sum read
 
 // One operand's tile of B rows (along) or B columns (down) and BR (64 or 32) of the summed index.  THREADS x 16 bytes a load.
-template <int B, int BR, bool ALONG, int THREADS>
+template <int B, int BR, bool ALONG, bool COLUMNS, int THREADS>
 struct Stage {
     static constexpr int BYTES = B * BR * 2, LOADS = BYTES / (THREADS * 16), PER_ROW = (ALONG ? BR : B) / 8;
+    static_assert(!COLUMNS || BR == 32, "a step is one column");
     static_assert(BYTES % (THREADS * 16) == 0 && THREADS / PER_ROW % 16 == 0, "whole loads; the rows of one thread share a swizzle");
     uint32_t voff[LOADS];       // bytes from the tile's corner
     int row, col;               // of load 0, in elements; load j is j * (THREADS / PER_ROW) rows further
@@ -48,21 +49,24 @@ struct Stage {
         row = t / PER_ROW;
         col = (t % PER_ROW ^ swizzle(row)) * 8;
         if (ALONG) {
-            corner = (const char*)O.base + (e0 * O.ld + r0) * 2;
-            step = BR * 2;
+            corner = (const char*)O.base + (COLUMNS ? (r0 / 32 * O.ld + e0) * 64 : (e0 * O.ld + r0) * 2);
+            step = COLUMNS ? O.ld * 64 : BR * 2;
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
                 int64_t e = row + j * (THREADS / PER_ROW);
                 if (e0 + e >= O.extent) e = O.extent - 1 - e0;             // rows past the end repeat the last one; their results are not stored
-                voff[j] = (uint32_t)((e * O.ld + col) * 2);
+                voff[j] = (uint32_t)(COLUMNS ? e * 64 + col * 2 : (e * O.ld + col) * 2);
             }
         } else {
-            corner = (const char*)O.base + (r0 * O.ld + e0) * 2;
-            step = (int64_t)BR * O.ld * 2;
+            corner = (const char*)O.base + (COLUMNS ? (e0 / 32 * O.ld + r0) * 64 : (r0 * O.ld + e0) * 2);
+            step = COLUMNS ? BR * 64 : (int64_t)BR * O.ld * 2;
             int64_t c = col;
             if (e0 + c >= O.extent) c = O.extent - 8 - e0;
 #pragma unroll
-            for (int j = 0; j < LOADS; ++j) voff[j] = (uint32_t)(((row + j * (THREADS / PER_ROW)) * O.ld + c) * 2);
+            for (int j = 0; j < LOADS; ++j) {
+                const int r = row + j * (THREADS / PER_ROW);
+                voff[j] = (uint32_t)(COLUMNS ? (c / 32 * O.ld + r) * 64 + c % 32 * 2 : (r * O.ld + c) * 2);
+            }
         }
     }
     // all of BR lies inside the operand
@@ -118,31 +122,6 @@ __device__ __forceinline__ typename E8<E>::t read_frag(uint32_t lds, int off) {
     }
 }
 
-// 8 neighbouring values as they lie in memory, `n` of them inside the matrix
-template <typename T> struct Raw8 {
-    Vec<T> v[8 / Wide<T>::N];
-    __device__ __forceinline__ void load(const T* p, int n) {
-        constexpr int N = Wide<T>::N;
-#pragma unroll
-        for (int h = 0; h < 8 / N; ++h) {
-            if (n >= (h + 1) * N) v[h] = *(const Vec<T>*)(p + h * N);
-            else
-#pragma unroll
-                for (int j = 0; j < N; ++j) v[h].e[j] = n > h * N + j ? p[h * N + j] : (T)0.f;
-        }
-    }
-    __device__ __forceinline__ float at(int e) const { return to_f(v[e / Wide<T>::N].e[e % Wide<T>::N]); }
-};
-template <typename T> __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
-    constexpr int N = Wide<T>::N;
-#pragma unroll
-    for (int h = 0; h < 8 / N; ++h) {
-        float u[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) u[j] = v[h * N + j];
-        store_some<T>(p + h * N, n - h * N, u);
-    }
-}
 // LDS of a block: `buffers` of a step, and in the end 128 rows of sums (4 words of padding keep a column off one bank)
 static constexpr int big_lds(int buffers, int step_bytes, int btq) {
     return buffers * step_bytes > 128 * (btq + 4) * 4 ? buffers * step_bytes : 128 * (btq + 4) * 4;
@@ -224,25 +203,8 @@ __device__ __forceinline__ void finish(const BigProduct& G, const LinArgs& A, co
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = from[e] + bias[e];
             const int m = p < G.p_end ? n : 0;
-            if (fwd) {
-                if (A.pre && m) {
-                    typedef typename Pre<T>::t pre_t;
-                    struct __attribute__((packed, aligned(sizeof(pre_t)))) { pre_t e[8]; } s;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s.e[e] = pre_pack(v[e], pre_t());
-                    pre_t* to = (pre_t*)A.pre + at;
-                    if (m == 8) *(decltype(s)*)to = s;
-                    else
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (e < m) to[e] = s.e[e];
-                }
-                lin_act_all<T>(A.act, A.slope, v);
-                if (res)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] += r0.at(e);
-                if (m) store8((T*)A.y + at, m, v);
-            } else if (m) {
+            if (fwd) forward_store8<T>(A, at, m, v, res ? &r0 : nullptr);
+            else if (m) {
                 if (G.splits > 1) store8(G.part + (int64_t)at0.split * G.p_end * Q + at, m, v);
                 else store8((T*)G.out + at, m, v);
             }
@@ -256,8 +218,8 @@ __device__ __forceinline__ void finish(const BigProduct& G, const LinArgs& A, co
 template <typename T, int BT, int WP, int WQ, int BUFS, bool PA, bool QA, int EPI>
 __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, int block, char* smem) {
     constexpr int THREADS = WP * WQ * 64, FP = BT / WP / 16, FQ = BT / WQ / 16, BR = 64;
-    typedef Stage<BT, BR, PA, THREADS> SP;
-    typedef Stage<BT, BR, QA, THREADS> SQ;
+    typedef Stage<BT, BR, PA, false, THREADS> SP;
+    typedef Stage<BT, BR, QA, false, THREADS> SQ;
     typedef typename E8<T>::t v8;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)smem;
     constexpr int BUF = SP::BYTES + SQ::BYTES, LOADS = SP::LOADS + SQ::LOADS;
@@ -342,8 +304,8 @@ __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, 
 template <int BTP, int BTQ, int BUFS, bool PA, bool QA, int EPI>
 __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A, int block, char* smem) {
     constexpr int WP = BTP / 64, WQ = BTQ / 64, THREADS = WP * WQ * 64, BR = 32;
-    typedef Stage<BTP, BR, PA, THREADS> SP;
-    typedef Stage<BTQ, BR, QA, THREADS> SQ;
+    typedef Stage<BTP, BR, PA, true, THREADS> SP;
+    typedef Stage<BTQ, BR, QA, true, THREADS> SQ;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)smem;
     constexpr int BUF = 3 * (SP::BYTES + SQ::BYTES), LOADS = 3 * (SP::LOADS + SQ::LOADS);
     const Place at0 = place<BTP, BTQ>(G, block);

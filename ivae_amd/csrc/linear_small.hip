@@ -34,16 +34,35 @@ __global__ __launch_bounds__(256) void k_linear_bwd(LinArgs A, LinSplit X, LinSp
     }
 }
 
-__device__ __forceinline__ float join(const float* part, int splits, int64_t n, int64_t i) {
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += part[k * n + i];
-    return s;
+// 8 neighbouring sums of `splits` parts of n values
+__device__ __forceinline__ void join8(const float* part, int splits, int64_t n, int64_t i, int left, float (&v)[8]) {
+    Raw8<float> u;
+    u.load(part + i, left);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = u.at(e);
+    for (int k = 1; k < splits; ++k) {
+        u.load(part + k * n + i, left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += u.at(e);
+    }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void k_linear_join_fwd(LinArgs A, int splits) {
-    const int64_t n = A.M * A.N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-        forward_store<T>(A, i / A.N, (int)(i % A.N), join(A.part, splits, n, i));
+    const int64_t n = A.M * A.N, groups = (A.N + 7) / 8, all = A.M * groups;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / groups, q = (i - m * groups) * 8, at = m * A.N + q;
+        const int left = A.N - q < 8 ? (int)(A.N - q) : 8;
+        Raw8<T> r, b;
+        if (A.res) r.load((const T*)A.res + m * A.ldr + q, left);
+        float v[8];
+        join8(A.part, splits, n, at, left, v);
+        if (A.b) {
+            b.load((const T*)A.b + q, left);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += b.at(e);
+        }
+        forward_store8<T>(A, at, left, v, A.res ? &r : nullptr);
+    }
 }
 // db is a sum over up to hundreds of parts of a few thousand columns: its blocks (the first ones) take 64 columns each, four walks
 // over the parts side by side, eight loads in flight
@@ -72,9 +91,14 @@ __global__ __launch_bounds__(256) void k_linear_join_bwd(LinArgs A, LinParts J) 
         if (w == 0 && i < A.N) ((T*)A.db)[i] = from_f<T>((fold[0][l] + fold[1][l]) + (fold[2][l] + fold[3][l]));
         return;
     }
-    for (int64_t i = (int64_t)(blockIdx.x - nb) * 256 + threadIdx.x; i < nx + nw; i += (int64_t)(gridDim.x - nb) * 256) {
-        if (i < nx) ((T*)A.dx)[i] = from_f<T>(join(J.x, J.kx, nx, i));
-        else ((T*)A.dw)[i - nx] = from_f<T>(join(J.w, J.kw, nw, i - nx));
+    const int64_t gx = (nx + 7) / 8, gw = (nw + 7) / 8;
+    for (int64_t g = (int64_t)(blockIdx.x - nb) * 256 + threadIdx.x; g < gx + gw; g += (int64_t)(gridDim.x - nb) * 256) {
+        const bool x = g < gx;
+        const int64_t n = x ? nx : nw, i = (x ? g : g - gx) * 8;
+        const int left = n - i < 8 ? (int)(n - i) : 8;
+        float v[8];
+        join8(x ? J.x : J.w, x ? J.kx : J.kw, n, i, left, v);
+        store8((T*)(x ? A.dx : A.dw) + i, left, v);
     }
 }
 
@@ -118,7 +142,7 @@ static unsigned cap(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blo
 
 hipError_t linear_join_forward(const LinArgs& A, int splits, int dtype, hipStream_t st) {
     if (splits < 2) return hipSuccess;
-    const dim3 g(cap((A.M * A.N + 255) / 256)), b(256);
+    const dim3 g(cap((A.M * ((A.N + 7) / 8) + 255) / 256)), b(256);
     if (dtype == IVAE_F32) hipLaunchKernelGGL(k_linear_join_fwd<float>, g, b, 0, st, A, splits);
     else if (dtype == IVAE_BF16) hipLaunchKernelGGL(k_linear_join_fwd<bf16_t>, g, b, 0, st, A, splits);
     else hipLaunchKernelGGL(k_linear_join_fwd<f16_t>, g, b, 0, st, A, splits);
@@ -129,7 +153,7 @@ hipError_t linear_join_backward(const LinArgs& A, const LinParts& J0, int dtype,
     if (!A.dx) J.kx = 0;
     if (!A.dw) J.kw = 0;
     if (!A.db) J.kb = 0;
-    const int64_t n = (J.kx > 1 ? A.M * A.K : 0) + (J.kw > 1 ? (int64_t)A.N * A.K : 0);
+    const int64_t n = (J.kx > 1 ? (A.M * A.K + 7) / 8 : 0) + (J.kw > 1 ? ((int64_t)A.N * A.K + 7) / 8 : 0);
     const unsigned blocks = cap((n + 255) / 256) + (J.kb > 0 ? (unsigned)((A.N + 63) / 64) : 0);
     if (blocks == 0) return hipSuccess;
     const dim3 g(blocks), b(256);

@@ -61,10 +61,14 @@ template <typename T, int TPR, bool TAIL> struct Row {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int e = (c * TPR + t) * N;
-            if (live && (TAIL ? e + N <= D : e < D)) v[c] = *(const Vec<T>*)(row + e);
-            else
 #pragma unroll
-                for (int j = 0; j < N; ++j) v[c].e[j] = TAIL && live && e + j < D ? row[e + j] : (T)0.f;
+            for (int j = 0; j < N; ++j) v[c].e[j] = (T)0.f;
+            if (c * TPR * N >= D) continue;                     // (the same for all threads: groups that no row reaches)
+            if (live && (TAIL ? e + N <= D : e < D)) v[c] = *(const Vec<T>*)(row + e);
+            else if (TAIL && live && e < D)
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (e + j < D) v[c].e[j] = row[e + j];
         }
     }
 };
