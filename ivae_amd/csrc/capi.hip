@@ -381,7 +381,7 @@ int ivae_layer_norm_workspace_bytes(const IvaeNorm* norm, size_t* out) {
     if (!out) return IVAE_E_NULLPTR;
     const int rc = check_norm(norm);
     if (rc) return rc;
-    *out = norm_ws_bytes(norm->rows, norm->width);
+    *out = norm_ws_bytes(norm->rows, norm->width, norm->dtype);
     return IVAE_OK;
 }
 
@@ -400,7 +400,7 @@ int ivae_layer_norm_backward(const IvaeNorm* norm, const void* dy, const void* x
     const int rc = check_norm(norm);
     if (rc) return rc;
     if (norm->rows > 0 && (!dy || !x || !stats)) return IVAE_E_NULLPTR;
-    const size_t need = dweight || dbias ? norm_ws_bytes(norm->rows, norm->width) : 0;
+    const size_t need = dweight || dbias ? norm_ws_bytes(norm->rows, norm->width, norm->dtype) : 0;
     if (need && !workspace) return IVAE_E_NULLPTR;
     if (workspace_bytes < need) return IVAE_E_WORKSPACE;
     if (!dx && !dweight && !dbias) return IVAE_OK;

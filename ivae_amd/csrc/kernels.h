@@ -51,7 +51,7 @@ hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, cons
                          void* ws, hipStream_t st);
 hipError_t launch_linear_backward(const IvaeLinear& L, const void* dy, const void* x, const void* w, const void* saved, void* dx, void* dw,
                                   void* db, void* ws, hipStream_t st);
-size_t norm_ws_bytes(int64_t rows, int width);
+size_t norm_ws_bytes(int64_t rows, int width, int dtype);
 hipError_t launch_layer_norm(const IvaeNorm& N, const void* x, const void* w, const void* b, void* y, float* stats, hipStream_t st);
 hipError_t launch_layer_norm_backward(const IvaeNorm& N, const void* dy, const void* x, const float* stats, const void* w, const void* residual,
                                       void* dx, void* dw, void* db, float* ws, hipStream_t st);

@@ -1,13 +1,12 @@
 // Layer norm over the last dimension, forward and backward.
 //   forward   y = (x - mean) r g + c,  r = 1 / sqrt(var + eps); (mean, r) of a row are kept for the backward pass
 //   backward  xh = (x - mean) r, a = dy g:   dx = r (a - mean(a) - xh mean(a xh)) [+ residual],  dg = sum_rows dy xh,  dc = sum_rows dy
-// Both are bound by memory: a row is read once, held in registers by the TPR threads that share it (16 elements each), and the
+// Both are bound by memory: a row is read once, held in registers by the TPR threads that share it (E = 16 or 8 elements each), and the
 // variance is summed from the centred values in those registers, so it does not cancel.  All sums are in 32 bits and in a fixed order.
 #include "kernels.h"
 #include "ops_common.h"
 
-static constexpr int EPT = 16;                 // elements a thread holds of a row
-static constexpr int NORM_MAX_D = 1024 * EPT;  // wider rows are walked instead of held
+static constexpr int NORM_MAX_D = 1024 * 16;   // wider rows are walked instead of held
 
 struct NormArgs {
     const void* x; const void* dy; const void* w; const void* b; const void* residual;
@@ -52,10 +51,10 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* lds) {
     }
 }
 
-// The thread's 16 elements of a row as they lie in memory: C groups of 16 bytes, the c-th at element (c TPR + t) N.  A group that the row
+// The thread's E elements of a row as they lie in memory: C groups of 16 bytes, the c-th at element (c TPR + t) N.  A group that the row
 // ends in is loaded by elements (TAIL: the width is no multiple of N); what lies beyond the row is 0.
-template <typename T, int TPR, bool TAIL> struct Row {
-    static constexpr int N = Wide<T>::N, C = EPT / N;
+template <typename T, int TPR, int E, bool TAIL> struct Row {
+    static constexpr int N = Wide<T>::N, C = E / N;
     Vec<T> v[C];
     __device__ __forceinline__ void load(const T* row, int t, int D, bool live) {
 #pragma unroll
@@ -108,14 +107,14 @@ __device__ __forceinline__ void load_weight(const void* w, int w_f32, int t, int
 }
 
 // A block walks rows; the next row's loads are under way while a row is summed.
-template <typename T, int TPR, bool TAIL>
+template <typename T, int TPR, int E, bool TAIL>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs A) {
-    constexpr int N = Wide<T>::N, C = EPT / N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+    constexpr int N = Wide<T>::N, C = E / N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
     __shared__ float lds[BLOCK / 64];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const int64_t step = (int64_t)gridDim.x * RPB;
     int64_t r0 = (int64_t)blockIdx.x * RPB;
-    Row<T, TPR, TAIL> now, next;
+    Row<T, TPR, E, TAIL> now, next;
     now.load((const T*)A.x + (r0 + sub < A.rows ? r0 + sub : 0) * A.ldx, t, A.D, r0 + sub < A.rows);
     float g[C][N], b[C][N];
     load_weight<T, TPR, TAIL>(A.w, A.w_f32, t, A.D, 1.f, g);
@@ -190,19 +189,19 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_wide(NormArgs A) {
 
 // dx, and each block's sums of dy xh and dy over the rows it walks (block, block + grid, ...).  (1024 threads have 128 registers each:
 // no room for the next row.)
-template <typename T, int TPR, bool TAIL>
+template <typename T, int TPR, int E, bool TAIL>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs A) {
-    constexpr int N = Wide<T>::N, C = EPT / N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+    constexpr int N = Wide<T>::N, C = E / N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
     constexpr bool AHEAD = TPR < 1024;
     __shared__ float lds[BLOCK / 64 * 2];
-    __shared__ float fold[RPB > 1 ? TPR * EPT * 2 : 1];
+    __shared__ float fold[RPB > 1 ? TPR * E * 2 : 1];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const float inv = 1.f / (float)A.D;
     const int64_t step = (int64_t)gridDim.x * RPB;
     int64_t r0 = (int64_t)blockIdx.x * RPB;
-    Row<T, TPR, TAIL> x, dy, xn, dyn;
+    Row<T, TPR, E, TAIL> x, dy, xn, dyn;
     float mean = 0.f, r = 0.f, mean_n = 0.f, r_n = 0.f;
-    auto load = [&](Row<T, TPR, TAIL>& a, Row<T, TPR, TAIL>& b, float& m, float& rs, int64_t row) {
+    auto load = [&](Row<T, TPR, E, TAIL>& a, Row<T, TPR, E, TAIL>& b, float& m, float& rs, int64_t row) {
         const bool live = row < A.rows;
         const int64_t at = live ? row : 0;
         a.load((const T*)A.x + at * A.ldx, t, A.D, live);
@@ -222,7 +221,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs A) 
         const bool live = row < A.rows;
         if (!AHEAD) load(x, dy, mean, r, row);
         else if (r0 + step < A.rows) load(xn, dyn, mean_n, r_n, row + step);
-        Row<T, TPR, TAIL> add;
+        Row<T, TPR, E, TAIL> add;
         if (A.residual) add.load((const T*)A.residual + (live ? row : 0) * A.ldr, t, A.D, live);
         float xh[C][N], d[C][N];
         float s[2] = {0.f, 0.f};
@@ -263,13 +262,13 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs A) 
                     for (int j = 0; j < N; ++j) {
                         const int i = (c * TPR + t) * N + j;
                         fold[i] = s ? fold[i] + dg[c][j] : dg[c][j];
-                        fold[TPR * EPT + i] = s ? fold[TPR * EPT + i] + dc[c][j] : dc[c][j];
+                        fold[TPR * E + i] = s ? fold[TPR * E + i] + dc[c][j] : dc[c][j];
                     }
             __syncthreads();
         }
         for (int i = threadIdx.x; i < A.D; i += BLOCK) {
             part[i] = fold[i];
-            part[A.D + i] = fold[TPR * EPT + i];
+            part[A.D + i] = fold[TPR * E + i];
         }
     } else {
 #pragma unroll
@@ -359,39 +358,44 @@ __global__ __launch_bounds__(1024) void k_norm_join(const float* part, int block
 }
 
 static unsigned wide_blocks(int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
-// threads that share a row: the fewest whose registers hold it
-static int tpr_of(int D) {
+// Threads that share a row and elements that each holds: the fewest threads with 16 where there is enough to read (16384 x 2048 bf16: 24 us
+// forward, 29 backward, against 27 and 38 with 8), and with 8 in small matrices and rows of ragged width, which wait for latencies (5003 x 1037
+// fp32: 14 and 18 us against 16 and 22 with 16; 64 x 200: 3 and 4 against 3 and 7).
+struct Share { int tpr, e; };
+static Share share_of(int64_t rows, int D, bool tail) {
+    if (D <= 4096 && (tail || rows * D <= 1 << 21)) return {D <= 512 ? 64 : D <= 2048 ? 256 : 512, 8};
     for (int t : {16, 64, 128, 256, 512})
-        if (D <= t * EPT) return t;
-    return 1024;
+        if (D <= t * 16) return {t, 16};
+    return {1024, 16};
 }
-static int64_t groups_of(int64_t rows, int D, int64_t most) {       // blocks of RPB rows each, at most `most`
-    const int tpr = tpr_of(D), rpb = tpr < 256 ? 256 / tpr : 1;
+static bool tail_of(int D, int dtype) { return D % (dtype == IVAE_F32 ? 4 : 8) != 0; }
+static int64_t groups_of(int64_t rows, int tpr, int64_t most) {     // blocks of RPB rows each, at most `most`
+    const int rpb = tpr < 256 ? 256 / tpr : 1;
     const int64_t need = (rows + rpb - 1) / rpb;
     return need < most ? need : most;
 }
 // about as many blocks as the chip holds: each keeps the weight in registers, and in the backward pass its sums
-static int fwd_blocks(int64_t rows, int D) { return (int)groups_of(rows, D, tpr_of(D) <= 256 ? 1280 : tpr_of(D) == 512 ? 640 : 320); }
+static int fwd_blocks(int64_t rows, Share h) { return (int)groups_of(rows, h.tpr, h.tpr <= 256 ? 1280 : h.tpr == 512 ? 640 : 320); }
 // blocks of the backward pass = rows of `part`
-static int norm_blocks(int64_t rows, int D) {
+static int norm_blocks(int64_t rows, int D, int dtype) {
     if (rows == 0) return 0;
     if (D > NORM_MAX_D) return (int)(rows < 256 ? (rows + 3) / 4 : 64);
-    return (int)groups_of(rows, D, tpr_of(D) <= 256 ? 768 : tpr_of(D) == 512 ? 512 : 256);
+    const Share h = share_of(rows, D, tail_of(D, dtype));
+    return (int)groups_of(rows, h.tpr, h.tpr <= 256 ? 768 : h.tpr == 512 ? 512 : 256);
 }
-size_t norm_ws_bytes(int64_t rows, int D) { return (size_t)norm_blocks(rows, D) * 2 * D * sizeof(float); }
+size_t norm_ws_bytes(int64_t rows, int D, int dtype) { return (size_t)norm_blocks(rows, D, dtype) * 2 * D * sizeof(float); }
 
+#define NORM_CASE(K, TPR, E) case TPR * 32 + E: hipLaunchKernelGGL((K<T, TPR, E, TAIL>), g, b, 0, st, A); break;
+#define NORM_CASES(K)                                                                                                                    \
+    switch (h.tpr * 32 + h.e) {                                                                                                          \
+        NORM_CASE(K, 64, 8) NORM_CASE(K, 256, 8) NORM_CASE(K, 512, 8) NORM_CASE(K, 16, 16) NORM_CASE(K, 64, 16) NORM_CASE(K, 128, 16)    \
+        NORM_CASE(K, 256, 16) NORM_CASE(K, 512, 16) NORM_CASE(K, 1024, 16)                                                               \
+    }
 template <typename T, bool TAIL>
 static void norm_fwd(const NormArgs& A, hipStream_t st) {
-    const int tpr = tpr_of(A.D);
-    const dim3 g((unsigned)fwd_blocks(A.rows, A.D)), b(tpr > 256 ? tpr : 256);
-    switch (tpr) {
-        case 16: hipLaunchKernelGGL((k_norm_fwd<T, 16, TAIL>), g, b, 0, st, A); break;
-        case 64: hipLaunchKernelGGL((k_norm_fwd<T, 64, TAIL>), g, b, 0, st, A); break;
-        case 128: hipLaunchKernelGGL((k_norm_fwd<T, 128, TAIL>), g, b, 0, st, A); break;
-        case 256: hipLaunchKernelGGL((k_norm_fwd<T, 256, TAIL>), g, b, 0, st, A); break;
-        case 512: hipLaunchKernelGGL((k_norm_fwd<T, 512, TAIL>), g, b, 0, st, A); break;
-        default: hipLaunchKernelGGL((k_norm_fwd<T, 1024, TAIL>), g, b, 0, st, A);
-    }
+    const Share h = share_of(A.rows, A.D, TAIL);
+    const dim3 g((unsigned)fwd_blocks(A.rows, h)), b(h.tpr > 256 ? h.tpr : 256);
+    NORM_CASES(k_norm_fwd)
 }
 template <typename T>
 static void norm_fwd(const NormArgs& A, hipStream_t st) {
@@ -412,16 +416,9 @@ hipError_t launch_layer_norm(const IvaeNorm& N, const void* x, const void* w, co
 
 template <typename T, bool TAIL>
 static void norm_bwd(const NormArgs& A, int blocks, hipStream_t st) {
-    const int tpr = tpr_of(A.D);
-    const dim3 g((unsigned)blocks), b(tpr > 256 ? tpr : 256);
-    switch (tpr) {
-        case 16: hipLaunchKernelGGL((k_norm_bwd<T, 16, TAIL>), g, b, 0, st, A); break;
-        case 64: hipLaunchKernelGGL((k_norm_bwd<T, 64, TAIL>), g, b, 0, st, A); break;
-        case 128: hipLaunchKernelGGL((k_norm_bwd<T, 128, TAIL>), g, b, 0, st, A); break;
-        case 256: hipLaunchKernelGGL((k_norm_bwd<T, 256, TAIL>), g, b, 0, st, A); break;
-        case 512: hipLaunchKernelGGL((k_norm_bwd<T, 512, TAIL>), g, b, 0, st, A); break;
-        default: hipLaunchKernelGGL((k_norm_bwd<T, 1024, TAIL>), g, b, 0, st, A);
-    }
+    const Share h = share_of(A.rows, A.D, TAIL);
+    const dim3 g((unsigned)blocks), b(h.tpr > 256 ? h.tpr : 256);
+    NORM_CASES(k_norm_bwd)
 }
 template <typename T>
 static void norm_bwd(const NormArgs& A, int blocks, void* dg, void* dc, hipStream_t st) {
@@ -439,7 +436,7 @@ hipError_t launch_layer_norm_backward(const IvaeNorm& N, const void* dy, const v
     NormArgs A = {};
     A.x = x; A.dy = dy; A.w = w; A.residual = residual; A.y = dx; A.cstats = stats; A.part = dg || dc ? ws : nullptr;
     A.rows = N.rows; A.ldx = N.ldx; A.lddy = N.lddy; A.ldr = N.ld_residual; A.D = N.width; A.w_f32 = N.weight_f32 || N.dtype == IVAE_F32;
-    const int blocks = norm_blocks(N.rows, N.width);
+    const int blocks = norm_blocks(N.rows, N.width, N.dtype);
     if (N.dtype == IVAE_F32) norm_bwd<float>(A, blocks, dg, dc, st);
     else if (N.dtype == IVAE_BF16) norm_bwd<bf16_t>(A, blocks, dg, dc, st);
     else norm_bwd<f16_t>(A, blocks, dg, dc, st);

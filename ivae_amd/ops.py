@@ -401,9 +401,10 @@ def _dtype_id(t, name):
 
 def _like(t, ref, name, shape=None, dtype=None):
     """t, checked to have ref's type (or `dtype`) and device and the given shape."""
-    if t.dtype is not (dtype or ref.dtype):
-        raise TypeError(f"{name} must be {dtype or ref.dtype}, got {t.dtype}")
-    if t.device != ref.device:
+    dtype = dtype or ref.dtype
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != ref.get_device():
         raise RuntimeError(f"{name} must live on {ref.device}, got {t.device}")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
@@ -450,8 +451,9 @@ def _opt(t):
     return None if t is None else t.data_ptr()
 
 
-def _scratch(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _empty(ref, shape, dtype):
+    """On ref's device.  (new_empty without a type is the quickest way to a tensor.)"""
+    return ref.new_empty(shape) if dtype is ref.dtype else torch.empty(shape, dtype=dtype, device=ref.device)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -482,7 +484,7 @@ def linear(x, weight, bias=None, activation="none", slope=.1, residual=None, sav
     type; activation: none, lrelu (slope), xtanh (tanh(s) + slope s), sigmoid, gelu (the erf form), silu.
     -> y, or with save=True (y, saved): saved is what linear_backward needs of the pre-activation, None for 'none'."""
     dt, act, rows, k, n = _linear_shapes(x, weight, activation)
-    out = x.shape[:-1] + (n,)
+    out = (rows, n) if x.dim() == 2 else (*x.shape[:-1], n)
     if bias is not None:
         bias = _dense(_like(bias, x, "bias", (n,)))
     x, ldx = _matrix(_aligned(x))
@@ -493,8 +495,8 @@ def linear(x, weight, bias=None, activation="none", slope=.1, residual=None, sav
     dev = x.device
     lin, nb = _linear_plan(rows, k, n, dt, act, float(slope), ldx, ldr, 0, 0)
     y = x.new_empty(out)
-    saved = torch.empty(out, dtype=_SAVED[dt], device=dev) if save and act else None
-    ws = _scratch(nb, dev)
+    saved = _empty(x, out, _SAVED[dt]) if save and act else None
+    ws = _empty(x, nb, torch.uint8) if nb else None
     _call(dev, _lib.lib().ivae_linear, "ivae_linear", lin, x.data_ptr(), weight.data_ptr(), _opt(bias), _opt(residual), y.data_ptr(), _opt(saved),
           _opt(ws), nb)
     return (y, saved) if save else y
@@ -504,7 +506,7 @@ def linear_backward(dy, x, weight, saved=None, activation="none", slope=.1, need
     """ivae_linear_backward: -> (dx, dweight, dbias), None where `need` says no.  `saved`: linear's, of the same x, weight and
     activation.  The gradient of the residual is dy itself."""
     dt, act, rows, k, n = _linear_shapes(x, weight, activation)
-    out = x.shape[:-1] + (n,)
+    out = (rows, n) if x.dim() == 2 else (*x.shape[:-1], n)
     _like(dy, x, "dy", out)
     if act:
         if saved is None:
@@ -521,7 +523,7 @@ def linear_backward(dy, x, weight, saved=None, activation="none", slope=.1, need
     dx = x.new_empty(shape) if need[0] else None
     dw = x.new_empty((n, k)) if need[1] else None
     db = x.new_empty((n,)) if need[2] else None
-    ws = _scratch(nb, dev)
+    ws = _empty(x, nb, torch.uint8) if nb else None
     _call(dev, _lib.lib().ivae_linear_backward, "ivae_linear_backward", lin, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _opt(saved),
           _opt(dx), _opt(dw), _opt(db), _opt(ws), nb)
     return dx, dw, db
@@ -559,7 +561,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, save=False):
     dev = x.device
     norm, _ = _norm_plan(rows, d, dt, int(wt == torch.float32), float(eps), ldx, 0, 0)
     y = x.new_empty(shape)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=dev) if save else None
+    stats = _empty(x, (2, rows), torch.float32) if save else None
     _call(dev, _lib.lib().ivae_layer_norm, "ivae_layer_norm", norm, x.data_ptr(), _opt(weight), _opt(bias), y.data_ptr(), _opt(stats))
     return (y, stats) if save else y
 
@@ -579,9 +581,9 @@ def layer_norm_backward(dy, x, stats, weight=None, residual=None, need=(True, Tr
     dev = x.device
     norm, nb = _norm_plan(rows, d, dt, int(wt == torch.float32), 0., ldx, lddy, ldr)
     dx = x.new_empty(shape) if need[0] else None
-    dw = torch.empty((d,), dtype=wt, device=dev) if need[1] else None
-    db = torch.empty((d,), dtype=wt, device=dev) if need[2] else None
-    ws = _scratch(nb, dev) if need[1] or need[2] else None
+    dw = _empty(x, (d,), wt) if need[1] else None
+    db = _empty(x, (d,), wt) if need[2] else None
+    ws = _empty(x, nb, torch.uint8) if nb and (need[1] or need[2]) else None
     _call(dev, _lib.lib().ivae_layer_norm_backward, "ivae_layer_norm_backward", norm, dy.data_ptr(), x.data_ptr(), stats.data_ptr(), _opt(weight),
           _opt(residual), _opt(dx), _opt(dw), _opt(db), _opt(ws), nb if ws is not None else 0)
     return dx, dw, db
