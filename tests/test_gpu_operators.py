@@ -97,7 +97,8 @@ def test_linear_long_sums(dt, m, k, n):
 
 
 # large products: whole tiles, ragged in every direction, summed dimensions that end inside a step, few tiles with long sums
-BIG = [(1024, 512, 512), (520, 768, 648), (777, 1001, 531), (64, 4104, 1000), (4100, 64, 1024), (1030, 1024, 264), (70, 72, 60000), (70, 60000, 72), (2050, 520, 1100)]
+BIG = [(1024, 512, 512), (520, 768, 648), (777, 1001, 531), (64, 4104, 1000), (4100, 64, 1024), (1030, 1024, 264), (70, 72, 60000), (70, 60000, 72), (2050, 520, 1100),
+       (2048, 1100, 1200), (300, 4104, 2100), (4100, 264, 2600)]
 
 
 @pytest.mark.parametrize("m,k,n", BIG)
@@ -106,7 +107,8 @@ def test_linear_large(dt, m, k, n):
     run_linear(dt, m, k, n, "gelu", seed=m + 1)
 
 
-@pytest.mark.parametrize("m,k,n", SIZES + BIG + [(64, 60000, 256), (4096, 200, 264), (8200, 1032, 136)])
+@pytest.mark.parametrize("m,k,n", SIZES + BIG + [(64, 60000, 256), (4096, 200, 264), (8200, 1032, 136), (8192, 512, 4096), (3000, 2000, 2001),
+                                                       (256, 4096, 8200)])
 @pytest.mark.parametrize("dt", R.DTYPES)
 def test_linear_integers_are_exact(dt, m, k, n):
     """Small whole numbers: every product and sum is one too, below 2^24, so each result is the exact one, rounded once to its type."""
@@ -155,7 +157,7 @@ def test_linear_large_rows_past_the_last_are_left_alone():
 
 
 @pytest.mark.parametrize("dt", R.DTYPES)
-@pytest.mark.parametrize("m,k,n", [(600, 1024, 520), (64, 8192, 520)])
+@pytest.mark.parametrize("m,k,n", [(600, 1024, 520), (64, 8192, 520), (1200, 2048, 1100), (260, 16384, 640)])
 def test_linear_large_keeps_nan_and_infinities(dt, m, k, n):
     g = torch.Generator().manual_seed(12)
     x, w, b, dy = normal(g, m, k, dtype=dt), normal(g, n, k, scale=.03, dtype=dt), normal(g, n, dtype=dt), normal(g, m, n, dtype=dt)
