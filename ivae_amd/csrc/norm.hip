@@ -386,11 +386,12 @@ static int norm_blocks(int64_t rows, int D, int dtype) {
 size_t norm_ws_bytes(int64_t rows, int D, int dtype) { return (size_t)norm_blocks(rows, D, dtype) * 2 * D * sizeof(float); }
 
 #define NORM_CASE(K, TPR, E) case TPR * 32 + E: hipLaunchKernelGGL((K<T, TPR, E, TAIL>), g, b, 0, st, A); break;
-#define NORM_CASES(K)                                                                                                                    \
-    switch (h.tpr * 32 + h.e) {                                                                                                          \
-        NORM_CASE(K, 64, 8) NORM_CASE(K, 256, 8) NORM_CASE(K, 512, 8) NORM_CASE(K, 16, 16) NORM_CASE(K, 64, 16) NORM_CASE(K, 128, 16)    \
-        NORM_CASE(K, 256, 16) NORM_CASE(K, 512, 16) NORM_CASE(K, 1024, 16)                                                               \
-    }
+#define NORM_CASES(K)                                                                                                                       \
+    switch (h.tpr * 32 + h.e) {                                                                                                             \
+        NORM_CASE(K, 64, 8) NORM_CASE(K, 256, 8) NORM_CASE(K, 512, 8) NORM_CASE(K, 512, 16) NORM_CASE(K, 1024, 16)                          \
+    }                                                                                                                                       \
+    if constexpr (!TAIL)                                                                                                                    \
+        switch (h.tpr * 32 + h.e) { NORM_CASE(K, 16, 16) NORM_CASE(K, 64, 16) NORM_CASE(K, 128, 16) NORM_CASE(K, 256, 16) }
 template <typename T, bool TAIL>
 static void norm_fwd(const NormArgs& A, hipStream_t st) {
     const Share h = share_of(A.rows, A.D, TAIL);

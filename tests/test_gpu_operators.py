@@ -108,7 +108,7 @@ def test_linear_large(dt, m, k, n):
 
 
 @pytest.mark.parametrize("m,k,n", SIZES + BIG + [(64, 60000, 256), (4096, 200, 264), (8200, 1032, 136), (8192, 512, 4096), (3000, 2000, 2001),
-                                                       (256, 4096, 8200)])
+                                                       (256, 4096, 8200), (20000, 256, 200), (24, 264, 8200), (50, 72, 8195)])
 @pytest.mark.parametrize("dt", R.DTYPES)
 def test_linear_integers_are_exact(dt, m, k, n):
     """Small whole numbers: every product and sum is one too, below 2^24, so each result is the exact one, rounded once to its type."""
@@ -362,7 +362,8 @@ def run_norm(dt, m, d, wdtype=None, affine=True, layout="dense", seed=0, shift=.
 
 
 @pytest.mark.parametrize("m,d", [(1, 1), (1, 2), (5, 1), (64, 50), (3, 255), (70, 256), (37, 257), (130, 1000), (9, 1024), (33, 1025), (3, 4096), (5, 4099),
-                                 (3, 5000), (2, 16384), (700, 200), (3000, 24), (1, 20001), (6, 20001)])
+                                 (3, 5000), (2, 16384), (700, 200), (3000, 24), (1, 20001), (6, 20001),
+                                 (3, 5001), (600, 4090), (40, 16381), (10500, 200), (2200, 1000), (1100, 2000), (520, 4096)])
 @pytest.mark.parametrize("dt", R.DTYPES)
 def test_layer_norm_sizes(dt, m, d):
     run_norm(dt, m, d, seed=m + d)
