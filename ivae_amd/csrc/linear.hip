@@ -169,12 +169,14 @@ static hipError_t big_backward(const LinArgs& A, int dtype, void* ws, hipStream_
 // ---- which kernel -----------------------------------------------------------------------------------------------------
 static bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
 // The large kernels from the size on from which they take less time, all their launches together (us, small | large):
-//   16 bits, forward    1024 x 512 x 512 14 | 15, 2048 x 512 x 1024 20 | 16, 2048 x 1024 x 1024 31 | 21, 128 x 4096 x 4096 36 | 23
-//   16 bits, backward   128 x 512 x 512 21 | 16, 1024 x 512 x 512 33 | 22, 1024 x 1024 x 1024 85 | 29 (but the small kernel does not round
+//   16 bits, forward    2048 x 512 x 1024 14 | 16, 1024 x 1024 x 1024 19 | 25, 2048 x 1024 x 1024 26 | 21, 128 x 4096 x 4096 33 | 22;
+//                       1531 x 1001 x 777 34 | 31
+//   16 bits, backward   128 x 512 x 512 18 | 17, 1024 x 512 x 512 28 | 22, 1024 x 1024 x 1024 66 | 29 (but the small kernel does not round
 //                       act' dy: it keeps what it loses little by)
-//   fp32, forward       1024 x 1024 x 1024 34 | 42, 2048 x 1024 x 1024 52 | 55, 300 x 4096 x 2048 82 | 76, 128 x 4096 x 4096 53 | 77
-//                       (cutting the weight in three costs as much as a product with 128 rows)
-//   fp32, backward      512 x 512 x 512 31 | 31, 1024 x 512 x 512 39 | 35, 1024 x 1024 x 1024 108 | 51
+//   fp32, forward       1024 x 1024 x 1024 30 | 42, 2048 x 1024 x 1024 48 | 55, 300 x 4096 x 2048 80 | 76, 128 x 4096 x 4096 51 | 74
+//                       (cutting the weight in three costs as much as a product with 128 rows); 1531 x 1001 x 777 65 | 50
+//   fp32, backward      512 x 512 x 512 27 | 29, 1024 x 512 x 512 35 | 33, 1024 x 1024 x 1024 96 | 52
+// Forward, rows that do not start on 16 bytes cost the small kernel twice the loads, the large one only its packing.
 static bool big_by_size(const LinArgs& A, int dtype, bool backward) {
     const int64_t lds[] = {A.ldx, A.lddy, A.K, A.N};
     for (int64_t ld : lds)
@@ -182,8 +184,9 @@ static bool big_by_size(const LinArgs& A, int dtype, bool backward) {
     // (blocks are counted, and bytes inside a tile of fp32 columns offset, in 32 bits)
     if (A.M < 64 || A.N < 64 || A.K < 64 || A.M >= (dtype == IVAE_F32 ? 1 << 22 : 1 << 29)) return false;
     const double flops = 2.0 * (double)A.M * (double)A.N * (double)A.K;
-    if (dtype == IVAE_F32) return backward ? flops >= 5e8 : flops >= 5e9 && A.M >= 256;
-    return flops >= (backward ? 1e8 : 1.5e9);
+    const bool ragged = A.K % (dtype == IVAE_F32 ? 4 : 8) != 0;
+    if (dtype == IVAE_F32) return backward ? flops >= 5e8 : flops >= (ragged ? 2e9 : 5e9) && A.M >= 256;
+    return flops >= (backward ? 1e8 : ragged ? 2e9 : 3e9);
 }
 // a matrix that would be loaded in place has to start on 16 bytes
 static bool big_in_place(const void* p, int64_t cols, int64_t ld, int dtype) { return dtype == IVAE_F32 || ld % 8 || cols % 8 || aligned(p); }

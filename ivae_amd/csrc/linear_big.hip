@@ -418,11 +418,10 @@ __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A
         LinArgs B = A;
         B.db = nullptr;                         // (its sums are fp32 already)
         const int group = threadIdx.x / 256;
-        float* lds = (float*)smem + group * 2 * TP * Lds<float>::LD;
         __syncthreads();
         for (int u = group; u < SUBS; u += GROUPS)
-            tile_product<float, MODE>(threadIdx.x % 256, B, S, at0.split, at0.p0 + u / (BTQ / 64) * 64, at0.q0 + u % (BTQ / 64) * 64, G.part, nullptr, lds,
-                                      lds + TP * Lds<float>::LD, nullptr, nullptr);
+            tile_product<float, MODE>(threadIdx.x % 256, B, S, at0.split, at0.p0 + u / (BTQ / 64) * 64, at0.q0 + u % (BTQ / 64) * 64, G.part, nullptr,
+                                      smem + group * tile_lds<float>(true));
         return;
     }
     finish<float, BTP, BTQ, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
@@ -475,6 +474,7 @@ template <typename T, int BT, int WP, int WQ, int BUFS> struct Big16 {
 };
 template <int BTP, int BTQ, int BUFS> struct Big32 {
     static constexpr int LDS = big_lds(BUFS, 3 * (BTP + BTQ) * 32 * 2, BTQ), THREADS = BTP * BTQ / 64;
+    static_assert(LDS >= THREADS / 256 * tile_lds<float>(true), "a tile with a NaN is computed again here");
     static hipError_t fwd(const BigProduct& B, const LinArgs& A, hipStream_t st) {
         static SmemCache cache;
         return go(k_split_fwd<BTP, BTQ, BUFS>, LDS, THREADS, cache, blocks_of(B), st, B, A);

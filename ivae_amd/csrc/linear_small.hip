@@ -12,25 +12,21 @@ __device__ __forceinline__ At at_of(const LinSplit& S, int64_t b) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_linear_fwd(LinArgs A, LinSplit S) {
-    __shared__ __attribute__((aligned(16))) T lp[TP * Lds<T>::LD];
-    __shared__ __attribute__((aligned(16))) T lq[TQ * Lds<T>::LD];
+    __shared__ __attribute__((aligned(16))) char smem[tile_lds<T>(false)];
     const int64_t tiles = S.tp * S.tq * S.splits;
     for (int64_t b = blockIdx.x; b < tiles; b += gridDim.x) {
         const At at = at_of(S, b);
-        tile_product<T, MODE_FWD>(threadIdx.x, A, S, at.split, at.p0, at.q0, A.part, nullptr, lp, lq, nullptr, nullptr);
+        tile_product<T, MODE_FWD>(threadIdx.x, A, S, at.split, at.p0, at.q0, A.part, nullptr, smem);
     }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void k_linear_bwd(LinArgs A, LinSplit X, LinSplit W, float* part_w, float* part_b) {
-    __shared__ __attribute__((aligned(16))) T lp[TP * Lds<T>::LD];
-    __shared__ __attribute__((aligned(16))) T lq[TQ * Lds<T>::LD];
-    __shared__ __attribute__((aligned(16))) T le[sizeof(T) == 2 ? TP * Lds<T>::LD : 1];
-    __shared__ float lsum[32 * TP];
+    __shared__ __attribute__((aligned(16))) char smem[tile_lds<T>(true)];
     const int64_t nx = X.tp * X.tq * X.splits, tiles = nx + W.tp * W.tq * W.splits;
     for (int64_t b = blockIdx.x; b < tiles; b += gridDim.x) {
         const At at = b < nx ? at_of(X, b) : at_of(W, b - nx);
-        if (b < nx) tile_product<T, MODE_DX>(threadIdx.x, A, X, at.split, at.p0, at.q0, A.part, nullptr, lp, lq, le, nullptr);
-        else tile_product<T, MODE_DW>(threadIdx.x, A, W, at.split, at.p0, at.q0, part_w, part_b, lp, lq, le, lsum);
+        if (b < nx) tile_product<T, MODE_DX>(threadIdx.x, A, X, at.split, at.p0, at.q0, A.part, nullptr, smem);
+        else tile_product<T, MODE_DW>(threadIdx.x, A, W, at.split, at.p0, at.q0, part_w, part_b, smem);
     }
 }
 

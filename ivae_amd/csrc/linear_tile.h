@@ -11,7 +11,11 @@
 #pragma once
 #include "linear.h"
 
-static constexpr int TP = 64, TQ = 64, TR = 32;
+// A step holds 64 of the summed index: with 32 there are twice the barriers, and each waits for a load's whole latency (fp16 1024 x 1024 x
+// 1024, us: forward 22.6 with 32, 21.5 with 64; gradients 85 and 67).  The tiles lie in LDS as in memory, and dw's operands and dx's
+// weight are turned by the LDS reads that transpose.  The sums leave through LDS as well, so that residual, output and saved values move 16
+// bytes a thread along rows (forward 21.5 -> 19.2 us).
+static constexpr int TP = 64, TQ = 64, TR = 64;
 
 template <typename T> struct Lds { static constexpr int LD = TR + 8; };       // row stride in elements; rows stay 16-byte aligned
 template <> struct Lds<float> { static constexpr int LD = TR + 4; };
@@ -38,28 +42,30 @@ __device__ __forceinline__ void fetch8(const T* base, int64_t ld, int64_t outer,
     }
 }
 
-// RC: the summed index is the contiguous one.  (i0, r0): the tile's corner.
+// A thread's 16 values of a tile, in two groups of 8 neighbours.  RC: the summed index is the contiguous one.  (i0, r0): the tile's corner.
 template <typename T, bool RC>
-__device__ __forceinline__ void fetch_tile(int t, const T* base, int64_t ld, int64_t i0, int64_t i_end, int64_t r0, int64_t r_end, float (&v)[8]) {
-    if (RC) fetch8<T>(base, ld, i0 + t / 4, i_end, r0 + t % 4 * 8, r_end, v);
-    else fetch8<T>(base, ld, r0 + t / 8, r_end, i0 + t % 8 * 8, i_end, v);
+__device__ __forceinline__ void fetch_tile(int t, const T* base, int64_t ld, int64_t i0, int64_t i_end, int64_t r0, int64_t r_end, float (&v)[2][8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (RC) fetch8<T>(base, ld, i0 + t / 4, i_end, r0 + h * 32 + t % 4 * 8, r_end, v[h]);
+        else fetch8<T>(base, ld, r0 + h * 32 + t / 8, r_end, i0 + t % 8 * 8, i_end, v[h]);
+    }
 }
+// ... into LDS as they lie in memory, 16 bytes at a time: [row of the tile][summed index] (RC) or [summed index][column of the tile].
 // ERR: what rounding to T leaves of them
 template <typename T, bool RC, bool ERR = false>
-__device__ __forceinline__ void put_tile(int t, T* lds, const float (&u)[8]) {
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float r = to_f(from_f<T>(u[j]));
-        v[j] = !ERR ? u[j] : fabsf(r) < __builtin_inff() ? u[j] - r : 0.f;       // (infinities and NaN are whole in the first number)
-    }
+__device__ __forceinline__ void put_tile(int t, T* lds, const float (&u)[2][8]) {
     constexpr int LD = Lds<T>::LD;
-    if (RC) {
+    struct __attribute__((aligned(16))) V { T e[8]; };
 #pragma unroll
-        for (int j = 0; j < 8; ++j) lds[(t / 4) * LD + t % 4 * 8 + j] = from_f<T>(v[j]);
-    } else {
+    for (int h = 0; h < 2; ++h) {
+        V v;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) lds[(t % 8 * 8 + j) * LD + t / 8] = from_f<T>(v[j]);
+        for (int j = 0; j < 8; ++j) {
+            const float r = to_f(from_f<T>(u[h][j]));
+            v.e[j] = from_f<T>(!ERR ? u[h][j] : fabsf(r) < __builtin_inff() ? u[h][j] - r : 0.f);      // (infinities and NaN are whole in the first number)
+        }
+        *(V*)(lds + (RC ? (t / 4) * LD + h * 32 + t % 4 * 8 : (h * 32 + t / 8) * LD + t % 8 * 8)) = v;
     }
 }
 
@@ -69,42 +75,67 @@ template <typename T> struct V8;
 template <> struct V8<bf16_t> { typedef bf16x8 t; };
 template <> struct V8<f16_t> { typedef f16x8 t; };
 
-// one TR-long step of a wave's 32 x 32 part
-template <typename T>
-__device__ __forceinline__ void tile_mma(int t, const T* lp, const T* lq, f32x4 (&acc)[2][2]) {
-    typedef typename V8<T>::t v8;
-    const int l = t % 64, w = t / 64, row = l % 16, r = l / 16 * 8;
+// A lane's part of a fragment of 16 rows or columns from `base`: 16-bit types 8 of the summed index from b + l / 16 * 8 on (out of [summed
+// index][column] by two reads that transpose 4 x 16 values), fp32 4 from b + l / 16 * 4 on.
+typedef short tile_s16x4 __attribute__((ext_vector_type(4)));
+template <typename T, bool RC> __device__ __forceinline__ typename V8<T>::t fragment(int l, const T* lds, int base, int b) {
     constexpr int LD = Lds<T>::LD;
-    v8 p[2], q[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        p[i] = *(const v8*)(lp + (w / 2 * 32 + i * 16 + row) * LD + r);
-        q[i] = *(const v8*)(lq + (w % 2 * 32 + i * 16 + row) * LD + r);
+    const int i = l % 16, g = l / 16;
+    if constexpr (RC) return *(const typename V8<T>::t*)(lds + (base + i) * LD + b + g * 8);
+    else {
+        typedef __attribute__((address_space(3))) tile_s16x4* p4;
+        const T* at = lds + (b + g * 8 + i / 4) * LD + base + i % 4 * 4;
+        const tile_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(at + 4 * LD));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(typename V8<T>::t, v);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mma32(q[j], p[i], acc[i][j]);
 }
-template <>
-__device__ __forceinline__ void tile_mma<float>(int t, const float* lp, const float* lq, f32x4 (&acc)[2][2]) {
-    const int l = t % 64, w = t / 64, row = l % 16, r = l / 16 * 4;
+template <bool RC> __device__ __forceinline__ f32x4 fragment32(int l, const float* lds, int base, int b) {
     constexpr int LD = Lds<float>::LD;
+    const int i = l % 16, g = l / 16;
+    if constexpr (RC) return *(const f32x4*)(lds + (base + i) * LD + b + g * 4);
+    else {
+        const float* at = lds + (b + g * 4) * LD + base + i;
+        return f32x4{at[0], at[LD], at[2 * LD], at[3 * LD]};
+    }
+}
+
+// one TR-long step of a wave's 32 x 32 part
+template <typename T, bool PRC, bool QRC>
+__device__ __forceinline__ void tile_mma(int t, const T* lp, const T* lq, f32x4 (&acc)[2][2]) {
+    const int l = t % 64, w = t / 64;
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int b = 0; b < TR; b += 16) {
-        f32x4 p[2], q[2];
+        for (int b = 0; b < TR; b += 32) {
+            typename V8<T>::t p[2], q[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            p[i] = *(const f32x4*)(lp + (w / 2 * 32 + i * 16 + row) * LD + b + r);
-            q[i] = *(const f32x4*)(lq + (w % 2 * 32 + i * 16 + row) * LD + b + r);
-        }
-        // step e takes element e of each lane group's four: the same permutation of the summed index on both sides
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
+            for (int i = 0; i < 2; ++i) {
+                p[i] = fragment<T, PRC>(l, lp, w / 2 * 32 + i * 16, b);
+                q[i] = fragment<T, QRC>(l, lq, w % 2 * 32 + i * 16, b);
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[j][e], p[i][e], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < 2; ++j) acc[i][j] = mma32(q[j], p[i], acc[i][j]);
+        }
+    } else {
+#pragma unroll
+        for (int b = 0; b < TR; b += 16) {
+            f32x4 p[2], q[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                p[i] = fragment32<PRC>(l, lp, w / 2 * 32 + i * 16, b);
+                q[i] = fragment32<QRC>(l, lq, w % 2 * 32 + i * 16, b);
+            }
+            // step e takes element e of each lane group's four: the same permutation of the summed index on both sides
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[j][e], p[i][e], acc[i][j], 0, 0, 0);
+        }
     }
 }
 
@@ -112,7 +143,10 @@ __device__ __forceinline__ void tile_mma<float>(int t, const float* lp, const fl
 // together if they all walk the same R.  A tile outside the matrix stores nothing.
 template <typename T, int MODE>
 __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinSplit& S, int64_t split, int64_t p0, int64_t q0, float* part, float* part_db,
-                                             T* lp, T* lq, T* le, float* lsum) {
+                                             char* smem) {
+    T* lp = (T*)smem;
+    T* lq = lp + TP * Lds<T>::LD;
+    T* le = lq + TQ * Lds<T>::LD;                   // (16-bit types, backward)
     const int64_t P = MODE == MODE_DW ? A.N : A.M, Q = MODE == MODE_FWD ? A.N : A.K, R = MODE == MODE_FWD ? A.K : MODE == MODE_DX ? A.N : A.M;
     const int64_t ra = split * S.len, rb = ra + S.len < R ? ra + S.len : R;
     const T* x = (const T*)A.x;
@@ -121,7 +155,7 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
     typedef typename Pre<T>::t pre_t;
     const pre_t* pre = (const pre_t*)A.cpre;
 
-    float vp[8], vq[8], sum[8] = {};
+    float vp[2][8], vq[2][8], sum[8] = {};
     auto fetch = [&](int64_t r0) {
         if constexpr (MODE == MODE_FWD) {
             fetch_tile<T, true>(t, x, A.ldx, p0, P, r0, rb, vp);
@@ -130,13 +164,14 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
             constexpr bool RC = MODE == MODE_DX;
             fetch_tile<T, RC>(t, dy, A.lddy, p0, P, r0, rb, vp);
             if (A.act != IVAE_ACT_NONE) {
-                float s[8];
+                float s[2][8];
                 fetch_tile<pre_t, RC>(t, pre, A.N, p0, P, r0, rb, s);
-                lin_act_slope_all<T>(A.act, A.slope, s, vp);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) lin_act_slope_all<T>(A.act, A.slope, s[h], vp[h]);
             }
             if (MODE == MODE_DW)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sum[j] += vp[j];
+                for (int j = 0; j < 8; ++j) sum[j] += vp[0][j] + vp[1][j];
             if (MODE == MODE_DX) fetch_tile<T, false>(t, w, A.K, q0, Q, r0, rb, vq);
             else fetch_tile<T, false>(t, x, A.ldx, q0, Q, r0, rb, vq);
         }
@@ -151,24 +186,50 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
         if (two) put_tile<T, MODE != MODE_DW, true>(t, le, vp);
         __syncthreads();
         if (r + TR < rb) fetch(r + TR);
-        tile_mma<T>(t, lp, lq, acc);
-        if (two) tile_mma<T>(t, le, lq, acc);
+        tile_mma<T, MODE != MODE_DW, MODE == MODE_FWD>(t, lp, lq, acc);
+        if constexpr (sizeof(T) == 2 && MODE != MODE_FWD)
+            if (two) tile_mma<T, MODE != MODE_DW, false>(t, le, lq, acc);
     }
+    // the sums go through LDS, so that what follows runs along rows, 8 columns a thread
+    constexpr int LD = TQ + 4;
+    float* sums = (float*)smem;
     const int l = t % 64, wv = t / 64;
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j) *(f32x4*)(sums + (wv / 2 * 32 + i * 16 + l % 16) * LD + wv % 2 * 32 + j * 16 + l / 16 * 4) = acc[i][j];
+    const int64_t q = q0 + t % 8 * 8, left = Q - q;
+    const int n = left >= 8 ? 8 : left > 0 ? (int)left : 0;
+    const bool fwd = MODE == MODE_FWD && S.splits == 1;
+    Raw8<T> bias, res[2];
+    if (fwd) {
+        if (A.b) bias.load((const T*)A.b + q, n);
+        if (A.res)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t p = p0 + wv / 2 * 32 + i * 16 + l % 16, q = q0 + wv % 2 * 32 + j * 16 + l / 16 * 4 + e;
-                if (p >= P || q >= Q) continue;
-                if (S.splits > 1) part[(split * P + p) * Q + q] = acc[i][j][e];
-                else if (MODE == MODE_FWD) forward_store<T>(A, p, (int)q, acc[i][j][e]);
-                else if (MODE == MODE_DX) ((T*)A.dx)[p * Q + q] = from_f<T>(acc[i][j][e]);
-                else if (A.dw) ((T*)A.dw)[p * Q + q] = from_f<T>(acc[i][j][e]);
+            for (int h = 0; h < 2; ++h) {
+                const int64_t p = p0 + h * 32 + t / 8;
+                res[h].load((const T*)A.res + p * A.ldr + q, p < P ? n : 0);
             }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int64_t p = p0 + h * 32 + t / 8, at = p * Q + q;
+        const int m = p < P ? n : 0;
+        const float* from = sums + (h * 32 + t / 8) * LD + t % 8 * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = from[e] + (fwd && A.b ? bias.at(e) : 0.f);
+        if (fwd) forward_store8<T>(A, at, m, v, A.res ? &res[h] : nullptr);
+        else if (m) {
+            if (S.splits > 1) store8(part + split * P * Q + at, m, v);
+            else if (MODE == MODE_DX) store8((T*)A.dx + at, m, v);
+            else if (A.dw) store8((T*)A.dw + at, m, v);
+        }
+    }
     if (MODE == MODE_DW && A.db && q0 == 0) {       // thread t holds the sums of 8 columns over every 32nd row: 32 threads hold each column
+        float* lsum = (float*)smem;
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 8; ++j) lsum[(t / 8) * TP + t % 8 * 8 + j] = sum[j];
@@ -182,3 +243,6 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
     }
     __syncthreads();                                // the tiles are free for the next round
 }
+// LDS of one group of 256 threads: the tiles, then the sums
+template <typename T> static constexpr int tile_lds(bool backward) { return (sizeof(T) == 2 && backward ? 3 : 2) * TP * Lds<T>::LD * (int)sizeof(T); }
+static_assert(tile_lds<f16_t>(false) >= TP * (TQ + 4) * 4, "the sums fit");

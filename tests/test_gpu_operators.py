@@ -98,7 +98,7 @@ def test_linear_long_sums(dt, m, k, n):
 
 # large products: whole tiles, ragged in every direction, summed dimensions that end inside a step, few tiles with long sums
 BIG = [(1024, 512, 512), (520, 768, 648), (777, 1001, 531), (64, 4104, 1000), (4100, 64, 1024), (1030, 1024, 264), (70, 72, 60000), (70, 60000, 72), (2050, 520, 1100),
-       (2048, 1100, 1200), (300, 4104, 2100), (4100, 264, 2600)]
+       (2048, 1100, 1200), (300, 4104, 2100), (4100, 264, 2600), (6000, 264, 1000)]
 
 
 @pytest.mark.parametrize("m,k,n", BIG)
