@@ -153,6 +153,23 @@ template <int BTP, int BTQ> __device__ __forceinline__ Place place(const BigProd
     return r;
 }
 
+// The residual of a tile on its way into the L2 cache while the last step is multiplied: 4 bytes of each 64 are loaded, into LDS `at` which
+// nothing reads.
+template <typename T, int BTP, int BTQ, int THREADS>
+__device__ __forceinline__ void touch_residual(const BigProduct& G, const LinArgs& A, const Place& at0, uint32_t at) {
+    constexpr int E = 64 / sizeof(T), PER_ROW = BTQ / E, LOADS = BTP * PER_ROW / THREADS;
+    const uint32_t base = __builtin_amdgcn_readfirstlane(at + threadIdx.x / 64 * 256);
+    int64_t q = at0.q0 + threadIdx.x % PER_ROW * E;
+    if (q >= G.q_end) q = G.q_end - 1;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+        int64_t p = at0.p0 + threadIdx.x / PER_ROW + j * (THREADS / PER_ROW);
+        if (p >= G.p_end) p = G.p_end - 1;
+        const uintptr_t a = (uintptr_t)((const T*)A.res + p * A.ldr + q) & ~(uintptr_t)3;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(a) : "memory");
+    }
+}
+
 // The sums go through LDS, up to 128 rows of the tile at a time, so that what follows runs along whole rows: 16-byte loads of the residual
 // (two rows ahead of their use) and stores of the results, side by side, and one copy of the code for them.
 template <typename T, int BTP, int BTQ, int WP, int WQ, int EPI, int FP, int FQ>
@@ -193,6 +210,7 @@ __device__ __forceinline__ void finish(const BigProduct& G, const LinArgs& A, co
             for (int j = 0; j < FQ; ++j)
                 *(f32x4*)(sums + (wave / WQ * RW + i * 16 + l % 16) * LD + wq + j * 16 + l / 16 * 4) = acc[h * (FP / HALVES) + i][j];
         __syncthreads();
+        if (EPI == EPI_FWD && h == 0) wait_loads<0>();          // (what touch_residual loads into LDS among them)
 #pragma unroll 1
         for (int it = 0; it < ITERS; ++it) {
             Raw8<T> r2;
@@ -274,6 +292,7 @@ __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, 
         __builtin_amdgcn_sched_barrier(0);
     };
 
+    const bool touch = G.splits == 1 && A.res;
     if (steps > 0) {
         for (int s = 0; s < BUFS && s < steps; ++s) load(s);
         if (steps >= BUFS) wait_loads<(BUFS - 1) * LOADS>();
@@ -288,6 +307,7 @@ __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, 
             else wait_loads<0>();
             block_barrier();                    // the next step's operands are in LDS, and all of this one's have been read
             if (s + BUFS < steps) load(s + BUFS);
+            if (EPI == EPI_FWD && s + 2 == steps && touch) touch_residual<T, BT, BT, THREADS>(G, A, at0, lds0 + big_lds(BUFS, BUF, BT));
             read(p0, q0, s + 1, 0);
             multiply(p1, q1);
             interleave();
@@ -365,6 +385,7 @@ __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A
                 for (int e = 0; e < 4; ++e) acc[i][half * 2 + j][e] = __fmaf_rn(c[i][j][e], sign, acc[i][half * 2 + j][e]);
     };
 
+    const bool touch = G.splits == 1 && A.res;
     if (steps > 0) {
         for (int s = 0; s < BUFS && s < steps; ++s) load(s);
         if (steps >= BUFS) wait_loads<(BUFS - 1) * LOADS>();
@@ -384,6 +405,7 @@ __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A
             else wait_loads<0>();
             block_barrier();                    // the next step's operands are in LDS, and all of this one's have been read
             if (s + BUFS < steps) load(s + BUFS);
+            if (EPI == EPI_FWD && s + 2 == steps && touch) touch_residual<float, BTP, BTQ, THREADS>(G, A, at0, lds0 + big_lds(BUFS, BUF, BTQ));
             read_q(s + 1, 0);
             // the next step's P takes each part's registers as soon as its last product is issued
             product(1, 0, 2, true), product(1, 2, 0, false);
@@ -418,6 +440,7 @@ __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A
         LinArgs B = A;
         B.db = nullptr;                         // (its sums are fp32 already)
         const int group = threadIdx.x / 256;
+        wait_loads<0>();
         __syncthreads();
         for (int u = group; u < SUBS; u += GROUPS)
             tile_product<float, MODE>(threadIdx.x % 256, B, S, at0.split, at0.p0 + u / (BTQ / 64) * 64, at0.q0 + u % (BTQ / 64) * 64, G.part, nullptr,
@@ -462,7 +485,7 @@ static hipError_t go(F fn, int bytes, int threads, SmemCache& cache, int blocks,
     return hipGetLastError();
 }
 template <typename T, int BT, int WP, int WQ, int BUFS> struct Big16 {
-    static constexpr int LDS = big_lds(BUFS, 2 * BT * 64 * 2, BT), THREADS = WP * WQ * 64;
+    static constexpr int THREADS = WP * WQ * 64, LDS = big_lds(BUFS, 2 * BT * 64 * 2, BT) + THREADS * 4;
     static hipError_t fwd(const BigProduct& B, const LinArgs& A, hipStream_t st) {
         static SmemCache cache;
         return go(k_big_fwd<T, BT, WP, WQ, BUFS>, LDS, THREADS, cache, blocks_of(B), st, B, A);
@@ -473,7 +496,7 @@ template <typename T, int BT, int WP, int WQ, int BUFS> struct Big16 {
     }
 };
 template <int BTP, int BTQ, int BUFS> struct Big32 {
-    static constexpr int LDS = big_lds(BUFS, 3 * (BTP + BTQ) * 32 * 2, BTQ), THREADS = BTP * BTQ / 64;
+    static constexpr int THREADS = BTP * BTQ / 64, LDS = big_lds(BUFS, 3 * (BTP + BTQ) * 32 * 2, BTQ) + THREADS * 4;
     static_assert(LDS >= THREADS / 256 * tile_lds<float>(true), "a tile with a NaN is computed again here");
     static hipError_t fwd(const BigProduct& B, const LinArgs& A, hipStream_t st) {
         static SmemCache cache;
