@@ -13,6 +13,8 @@
 // the summed index start from zero, smallest products first, and are added to the sum by fp32 additions that round to nearest.
 // An infinity times a part that is 0 makes a NaN that fp32 would not: a tile with a NaN in it is computed again in fp32, from the
 // tensors themselves.
+#include <type_traits>
+
 #include "kernels.h"
 #include "linear_big.h"
 #include "linear_tile.h"
@@ -69,20 +71,27 @@ struct Stage {
             }
         }
     }
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    __device__ __forceinline__ u32x4 resource(int64_t advance) const {
+        const uint64_t a = (uint64_t)(corner + advance);
+        u32x4 r;
+        r.x = __builtin_amdgcn_readfirstlane((uint32_t)a);
+        r.y = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) & 0xffffu;
+        r.z = 0xffffffffu;
+        r.w = 0x00020000u;
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t wave_base(uint32_t lds) { return __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024); }
+    __device__ __forceinline__ void load_one(int j, uint32_t base, u32x4 rsrc) const {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(base + j * THREADS * 16), "v"(voff[j]), "s"(rsrc)
+                     : "memory");
+    }
     // all of BR lies inside the operand
     __device__ __forceinline__ void load_full(uint32_t lds, int64_t advance) const {
-        const uint64_t a = (uint64_t)(corner + advance);
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        u32x4 rsrc;
-        rsrc.x = __builtin_amdgcn_readfirstlane((uint32_t)a);
-        rsrc.y = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) & 0xffffu;
-        rsrc.z = 0xffffffffu;
-        rsrc.w = 0x00020000u;
-        const uint32_t base = __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024);
+        const u32x4 rsrc = resource(advance);
+        const uint32_t base = wave_base(lds);
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(base + j * THREADS * 16), "v"(voff[j]), "s"(rsrc)
-                         : "memory");
+        for (int j = 0; j < LOADS; ++j) load_one(j, base, rsrc);
     }
     // `left` of the summed index remain: what lies beyond reads zeros
     __device__ __forceinline__ void load_part(uint32_t lds, int64_t advance, int64_t left) const {
@@ -101,26 +110,27 @@ struct Stage {
         const int r = g * 8 + i / 4, c = base + i % 4 * 4;                 // the first four of a lane group's eight rows
         return r * (B * 2) + (((c >> 3) ^ swizzle(r)) << 4) + (c & 4) * 2;
     }
-    // ... of the i-th 16 from there on (i * 16 < 128), in the k-th 32.  Along: 16 rows keep the swizzle, k flips bit 2 of the group.  Down:
-    // 16 columns are 2 groups, and i flips bits of the group like the swizzle does; 32 rows keep it.
-    static __device__ __forceinline__ int frag(int first, int i, int k) {
-        return ALONG ? (first ^ k << 6) + i * 16 * BR * 2 : (first ^ i << 5) + k * 32 * B * 2;
+    // The i-th 16 from there on (i * 16 < 128), in the k-th 32, of the tile at `lds` (a multiple of 256): from(lds, first, k), then read(from, i,
+    // k).  Along: 16 rows keep the swizzle, k flips bit 2 of the group.  Down: 16 columns are 2 groups, and i flips bits of the group like
+    // the swizzle does; 32 rows keep it, and 4 rows too (bit 2 of the row is in no swizzle).  Steps of 32: k counts tiles that follow.
+    static __device__ __forceinline__ uint32_t from(uint32_t lds, int first, int k) {
+        uint32_t a = lds + (ALONG ? first ^ k << 6 : first);
+        asm("" : "+v"(a));                      // one register that all reads share, what is constant goes into their offsets
+        return a;
+    }
+    template <typename E> static __device__ __forceinline__ typename E8<E>::t read(uint32_t from, int i, int k) {
+        if constexpr (ALONG) return *(const __attribute__((address_space(3))) typename E8<E>::t*)(uintptr_t)(from + i * 16 * BR * 2 + (BR == 32 ? k * BYTES : 0));
+        else {
+            typedef __attribute__((address_space(3))) s16x4* p4;
+            const uint32_t at = (from ^ i << 5) + k * 32 * B * 2;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(uintptr_t)at);
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(uintptr_t)(at + B * 8));
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            const s16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(typename E8<E>::t, v);
+        }
     }
 };
-
-template <typename E, int B, bool ALONG, int THREADS>
-__device__ __forceinline__ typename E8<E>::t read_frag(uint32_t lds, int off) {
-    if constexpr (ALONG) return *(const __attribute__((address_space(3))) typename E8<E>::t*)(uintptr_t)(lds + off);
-    else {
-        // rows +4: bit 2 of the row is in no swizzle, so the address is B * 8 bytes further
-        typedef __attribute__((address_space(3))) s16x4* p4;
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(uintptr_t)(lds + off));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(uintptr_t)(lds + off + B * 8));
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-        return __builtin_bit_cast(typename E8<E>::t, v);
-    }
-}
 
 // LDS of a block: `buffers` of a step, and in the end 128 rows of sums (4 words of padding keep a column off one bank)
 static constexpr int big_lds(int buffers, int step_bytes, int btq) {
@@ -262,34 +272,57 @@ __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, 
         else sq.load_part(at + SP::BYTES, s * sq.step, lq);
     };
     v8 p0[FP], q0[FQ], p1[FP], q1[FQ];          // fragments of the first and the second 32 of a step
-    auto read = [&](v8 (&p)[FP], v8 (&q)[FQ], int s, int k) {
+    struct From { uint32_t p, q; };
+    auto from = [&](int s, int k) {
         const uint32_t at = lds0 + s % BUFS * BUF;
+        return From{SP::from(at, op, k), SQ::from(at, oq, k)};
+    };
+    auto read_one = [&](v8 (&p)[FP], v8 (&q)[FQ], const From& f, int k, int i) {
+        if (i < FQ) q[i] = SQ::template read<T>(f.q, i, k);
+        else p[i - FQ] = SP::template read<T>(f.p, i - FQ, k);
+    };
+    auto read = [&](v8 (&p)[FP], v8 (&q)[FQ], int s, int k) {
+        const From f = from(s, k);
 #pragma unroll
-        for (int j = 0; j < FQ; ++j) q[j] = read_frag<T, BT, QA, THREADS>(at, SQ::frag(oq, j, k));
-#pragma unroll
-        for (int i = 0; i < FP; ++i) p[i] = read_frag<T, BT, PA, THREADS>(at, SP::frag(op, i, k));
+        for (int i = 0; i < FP + FQ; ++i) read_one(p, q, f, k, i);
     };
     f32x4 acc[FP][FQ];
 #pragma unroll
     for (int i = 0; i < FP; ++i)
 #pragma unroll
         for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // 32 of the summed index multiplied, the next 32 read (k of step s) and, if `next` says so, step `fill` loaded.  Reads and loads stand between
+    // the products, so that the matrix cores wait for neither's queue: with the loads of a step in a row the waves of a block stand
+    // in front of the address unit together.
+    auto half = [&](const v8 (&p)[FP], const v8 (&q)[FQ], v8 (&pn)[FP], v8 (&qn)[FQ], int s, int k, auto next, int fill) {
+        constexpr bool LOAD = decltype(next)::value;
+        constexpr int READS = FP + FQ, PER = (READS + FP - 3) / (FP - 2), PER_L = (LOADS + FP - 1) / FP;
+        const From f = from(s, k);
+        typename SP::u32x4 rp = {}, rq = {};
+        uint32_t bp = 0, bq = 0;
+        if (LOAD) {
+            rp = sp.resource(fill * sp.step), rq = sq.resource(fill * sq.step);
+            bp = SP::wave_base(lds0 + fill % BUFS * BUF), bq = SQ::wave_base(lds0 + fill % BUFS * BUF + SP::BYTES);
+        }
+#pragma unroll
+        for (int i = 0; i < FP; ++i) {
+            if (LOAD)
+#pragma unroll
+                for (int j = i * PER_L; j < (i + 1) * PER_L && j < LOADS; ++j)
+                    if (j < SP::LOADS) sp.load_one(j, bp, rp);
+                    else sq.load_one(j - SP::LOADS, bq, rq);
+#pragma unroll
+            for (int j = i * PER; j < (i + 1) * PER && j < READS; ++j) read_one(pn, qn, f, k, j);
+#pragma unroll
+            for (int j = 0; j < FQ; ++j) acc[i][j] = mma(q[j], p[i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
     auto multiply = [&](const v8 (&p)[FP], const v8 (&q)[FQ]) {
 #pragma unroll
         for (int i = 0; i < FP; ++i)
 #pragma unroll
             for (int j = 0; j < FQ; ++j) acc[i][j] = mma(q[j], p[i], acc[i][j]);
-    };
-    // the reads of one half between the products of the other: the matrix cores wait for neither LDS nor its queue
-    auto interleave = [&] {
-        constexpr int READS = FP * (PA ? 1 : 2) + FQ * (QA ? 1 : 2), PER = FP * FQ / READS, REST = FP * FQ - READS * PER;
-#pragma unroll
-        for (int i = 0; i < READS; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, REST, 0);
-        __builtin_amdgcn_sched_barrier(0);
     };
 
     const bool touch = G.splits == 1 && A.res;
@@ -299,18 +332,21 @@ __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, 
         else wait_loads<0>();
         block_barrier();
         read(p0, q0, 0, 0);
-        for (int s = 0; s + 1 < steps; ++s) {
-            read(p1, q1, s, 1);
-            multiply(p0, q0);
-            interleave();
+        int s = 0;
+        for (; s + BUFS + 1 < steps; ++s) {         // (step s + BUFS is not the last one, so it is whole)
+            half(p0, q0, p1, q1, s, 1, std::false_type(), 0);
+            wait_loads<(BUFS - 2) * LOADS>();
+            block_barrier();                    // the next step's operands are in LDS, and all of this one's have been read
+            half(p1, q1, p0, q0, s + 1, 0, std::true_type(), s + BUFS);
+        }
+        for (; s + 1 < steps; ++s) {
+            half(p0, q0, p1, q1, s, 1, std::false_type(), 0);
             if (s + BUFS <= steps) wait_loads<(BUFS - 2) * LOADS>();
             else wait_loads<0>();
-            block_barrier();                    // the next step's operands are in LDS, and all of this one's have been read
+            block_barrier();
             if (s + BUFS < steps) load(s + BUFS);
             if (EPI == EPI_FWD && s + 2 == steps && touch) touch_residual<T, BT, BT, THREADS>(G, A, at0, lds0 + big_lds(BUFS, BUF, BT));
-            read(p0, q0, s + 1, 0);
-            multiply(p1, q1);
-            interleave();
+            half(p1, q1, p0, q0, s + 1, 0, std::false_type(), 0);
         }
         read(p1, q1, steps - 1, 1);
         multiply(p0, q0);
@@ -358,16 +394,16 @@ __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A
         for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     bf16x8 p[3][4], q[2][3][2];                 // parts of the P fragments; parts of the Q fragments, two columns of tiles at a time
     auto read_p = [&](int s, int k) {
-        const uint32_t at = lds0 + s % BUFS * BUF + k * SP::BYTES;
+        const uint32_t from = SP::from(lds0 + s % BUFS * BUF, op, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[k][i] = read_frag<bf16_t, BTP, PA, THREADS>(at, SP::frag(op, i, 0));
+        for (int i = 0; i < 4; ++i) p[k][i] = SP::template read<bf16_t>(from, i, k);
     };
     auto read_q = [&](int s, int half) {
-        const uint32_t at = lds0 + s % BUFS * BUF;
+        const uint32_t from = SQ::from(lds0 + s % BUFS * BUF, oq, 0);
 #pragma unroll
         for (int k = 0; k < 3; ++k)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) q[half][k][j] = read_frag<bf16_t, BTQ, QA, THREADS>(at + k * SQ::BYTES, SQ::frag(oq, half * 2 + j, 0));
+            for (int j = 0; j < 2; ++j) q[half][k][j] = SQ::template read<bf16_t>(from, half * 2 + j, k);
     };
     f32x4 c[4][2];
     auto product = [&](int half, int kp, int kq, bool first) {
