@@ -435,25 +435,54 @@ __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A
             __builtin_amdgcn_sched_barrier(0);
         };
         float sign = 1.f;                       // (a split starts at a multiple of 64)
-        for (int s = 0; s + 1 < steps; ++s) {
-            first_half(s, sign);
-            if (s + BUFS <= steps) wait_loads<(BUFS - 2) * LOADS>();
-            else wait_loads<0>();
-            block_barrier();                    // the next step's operands are in LDS, and all of this one's have been read
-            if (s + BUFS < steps) load(s + BUFS);
-            if (EPI == EPI_FWD && s + 2 == steps && touch) touch_residual<float, BTP, BTQ, THREADS>(G, A, at0, lds0 + big_lds(BUFS, BUF, BTQ));
+        // LOAD: step `fill` is loaded, piece by piece between the products.  The next step's P takes each part's registers as soon as its last
+        // product is issued.
+        auto second_half = [&](int s, float sign, auto what, int fill) {
+            auto part = [&](int n, int kp, int kq) {          // the n-th of six products of the half
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (decltype(what)::value) {
+#pragma unroll
+                        for (int j = ((n * 4 + i) * LOADS + 23) / 24; j < ((n * 4 + i + 1) * LOADS + 23) / 24; ++j) {
+                            const int k = j / (LOADS / 3), at = j % (LOADS / 3);
+                            const uint32_t to = lds0 + fill % BUFS * BUF;
+                            if (at < SP::LOADS) sp.load_one(at, SP::wave_base(to + k * SP::BYTES), sp.resource(k * G.P.plane * 2 + fill * sp.step));
+                            else sq.load_one(at - SP::LOADS, SQ::wave_base(to + 3 * SP::BYTES + k * SQ::BYTES), sq.resource(k * G.Q.plane * 2 + fill * sq.step));
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) c[i][j] = mma(q[1][kq][j], p[kp][i], n == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : c[i][j]);
+                    if (decltype(what)::value) __builtin_amdgcn_sched_barrier(0);
+                }
+            };
             read_q(s + 1, 0);
-            // the next step's P takes each part's registers as soon as its last product is issued
-            product(1, 0, 2, true), product(1, 2, 0, false);
+            part(0, 0, 2), part(1, 2, 0);
             __builtin_amdgcn_sched_barrier(0);
             read_p(s + 1, 2);
-            product(1, 1, 1, false), product(1, 1, 0, false);
+            part(2, 1, 1), part(3, 1, 0);
             __builtin_amdgcn_sched_barrier(0);
             read_p(s + 1, 1);
-            product(1, 0, 1, false), product(1, 0, 0, false);
+            part(4, 0, 1), part(5, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
             read_p(s + 1, 0);
             add(1, sign);
+        };
+        int s = 0;
+        for (; s + BUFS + 1 < steps; ++s) {         // (step s + BUFS is not the last one, so it is whole)
+            first_half(s, sign);
+            wait_loads<(BUFS - 2) * LOADS>();
+            block_barrier();                    // the next step's operands are in LDS, and all of this one's have been read
+            second_half(s, sign, std::true_type(), s + BUFS);
+            sign = -sign;
+        }
+        for (; s + 1 < steps; ++s) {
+            first_half(s, sign);
+            if (s + BUFS <= steps) wait_loads<(BUFS - 2) * LOADS>();
+            else wait_loads<0>();
+            block_barrier();
+            if (s + BUFS < steps) load(s + BUFS);
+            if (EPI == EPI_FWD && s + 2 == steps && touch) touch_residual<float, BTP, BTQ, THREADS>(G, A, at0, lds0 + big_lds(BUFS, BUF, BTQ));
+            second_half(s, sign, std::false_type(), 0);
             sign = -sign;
         }
         first_half(steps - 1, sign);
