@@ -18,6 +18,7 @@ struct DropArgs {
     uint32_t k0, k1;
     uint64_t offset;
     const int64_t* offset_dev; // or null; added to offset
+    bool past;                 // y is stored past the caches
 };
 
 // high and low half of a * m from ONE wide multiply (v_mad_u64_u32)
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(256) void k_dropout(DropArgs A) {
                 x[g * 4 + j] = A.residual ? r[g * 4 + j] + v : v;
             }
         }
-        store_some<T>((T*)A.y + e, left, x);
+        store_some<T>((T*)A.y + e, left, x, A.past);
     }
 }
 
@@ -78,6 +79,7 @@ hipError_t launch_dropout(int dtype, int64_t n, const void* x, const void* resid
     A.scale = A.all ? 0.f : (float)(1.0 / (1.0 - p));
     A.k0 = (uint32_t)seed; A.k1 = (uint32_t)(seed >> 32);
     A.offset = offset; A.offset_dev = offset_dev;
+    A.past = past_caches(n, dtype);
     const int per = dtype == IVAE_F32 ? 4 : 8;
     int64_t blocks = ((n + per - 1) / per + 255) / 256;
     if (blocks > 8192) blocks = 8192;

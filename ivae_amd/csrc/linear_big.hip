@@ -308,9 +308,10 @@ __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, 
         for (int i = 0; i < FP; ++i) {
             if (LOAD)
 #pragma unroll
-                for (int j = i * PER_L; j < (i + 1) * PER_L && j < LOADS; ++j)
+                for (int j = i * PER_L; j < (i + 1) * PER_L && j < LOADS; ++j) {
                     if (j < SP::LOADS) sp.load_one(j, bp, rp);
                     else sq.load_one(j - SP::LOADS, bq, rq);
+                }
 #pragma unroll
             for (int j = i * PER; j < (i + 1) * PER && j < READS; ++j) read_one(pn, qn, f, k, j);
 #pragma unroll

@@ -16,6 +16,7 @@ struct NormArgs {
     int64_t rows, ldx, lddy, ldr;
     int D, w_f32;
     float eps;
+    bool past;                                 // y is stored past the caches
 };
 
 __device__ __forceinline__ float wload(const void* w, int w_f32, int i, bool half_is_bf16) {
@@ -71,11 +72,11 @@ template <typename T, int TPR, int E, bool TAIL> struct Row {
         }
     }
 };
-template <typename T, int TPR, bool TAIL, int C, int N> __device__ __forceinline__ void store_row(T* row, int t, int D, const float (&o)[C][N]) {
+template <typename T, int TPR, bool TAIL, int C, int N> __device__ __forceinline__ void store_row(T* row, int t, int D, const float (&o)[C][N], bool past) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int e = (c * TPR + t) * N;
-        if (TAIL ? e + N <= D : e < D) store_wide<T>(row + e, o[c]);
+        if (TAIL ? e + N <= D : e < D) store_wide<T>(row + e, o[c], past);
         else if (TAIL && e < D) store_part<T>(row + e, D - e, o[c]);
     }
 }
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs A) 
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int j = 0; j < N; ++j) v[c][j] = v[c][j] * r * g[c][j] + b[c][j];
-        store_row<T, TPR, TAIL>((T*)A.y + row * A.D, t, A.D, v);
+        store_row<T, TPR, TAIL>((T*)A.y + row * A.D, t, A.D, v, A.past);
     }
 }
 
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs A) 
                 d[c][j] = rr * (d[c][j] - m1 - xh[c][j] * m2);
                 if (A.residual) d[c][j] += to_f(add.v[c].e[j]);
             }
-        store_row<T, TPR, TAIL>((T*)A.y + row * A.D, t, A.D, d);
+        store_row<T, TPR, TAIL>((T*)A.y + row * A.D, t, A.D, d, A.past);
     }
     if (!A.part) return;
     float* part = A.part + (int64_t)blockIdx.x * 2 * A.D;
@@ -409,6 +410,7 @@ hipError_t launch_layer_norm(const IvaeNorm& N, const void* x, const void* w, co
     NormArgs A = {};
     A.x = x; A.w = w; A.b = b; A.y = y; A.stats = stats;
     A.rows = N.rows; A.ldx = N.ldx; A.D = N.width; A.w_f32 = N.weight_f32 || N.dtype == IVAE_F32; A.eps = N.eps;
+    A.past = past_caches(N.rows * N.width, N.dtype);
     if (N.dtype == IVAE_F32) norm_fwd<float>(A, st);
     else if (N.dtype == IVAE_BF16) norm_fwd<bf16_t>(A, st);
     else norm_fwd<f16_t>(A, st);
@@ -437,6 +439,7 @@ hipError_t launch_layer_norm_backward(const IvaeNorm& N, const void* dy, const v
     NormArgs A = {};
     A.x = x; A.dy = dy; A.w = w; A.residual = residual; A.y = dx; A.cstats = stats; A.part = dg || dc ? ws : nullptr;
     A.rows = N.rows; A.ldx = N.ldx; A.lddy = N.lddy; A.ldr = N.ld_residual; A.D = N.width; A.w_f32 = N.weight_f32 || N.dtype == IVAE_F32;
+    A.past = past_caches(N.rows * N.width, N.dtype);
     const int blocks = norm_blocks(N.rows, N.width, N.dtype);
     if (N.dtype == IVAE_F32) norm_bwd<float>(A, blocks, dg, dc, st);
     else if (N.dtype == IVAE_BF16) norm_bwd<bf16_t>(A, blocks, dg, dc, st);

@@ -26,12 +26,18 @@ template <typename T, int N> __device__ __forceinline__ void load_wide(const T* 
 #pragma unroll
     for (int j = 0; j < N; ++j) out[j] = to_f(v.e[j]);
 }
-template <typename T, int N> __device__ __forceinline__ void store_wide(T* p, const float (&in)[N]) {
+// `past`: past the caches
+template <typename T, int N> __device__ __forceinline__ void store_wide(T* p, const float (&in)[N], bool past = false) {
     static_assert(N == Wide<T>::N, "one 16-byte store");
     Vec<T> v;
 #pragma unroll
     for (int j = 0; j < N; ++j) v.e[j] = from_f<T>(in[j]);
-    *reinterpret_cast<Vec<T>*>(p) = v;
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+    if (past) {
+        asm volatile("");                                // (without these, both stores become one that goes through the caches)
+        __builtin_nontemporal_store(__builtin_bit_cast(u4, v), reinterpret_cast<u4*>(p));
+        asm volatile("");
+    } else *reinterpret_cast<Vec<T>*>(p) = v;
 }
 // the first `n` (0 < n < N) of them
 template <typename T, int N> __device__ __forceinline__ void load_part(const T* p, int n, float (&out)[N]) {
@@ -47,9 +53,14 @@ template <typename T, int N> __device__ __forceinline__ void load_some(const T* 
     if (n >= N) load_wide<T>(p, out);
     else load_part<T>(p, n, out);
 }
-template <typename T, int N> __device__ __forceinline__ void store_some(T* p, int n, const float (&in)[N]) {
-    if (n >= N) store_wide<T>(p, in);
+template <typename T, int N> __device__ __forceinline__ void store_some(T* p, int n, const float (&in)[N], bool past = false) {
+    if (n >= N) store_wide<T>(p, in, past);
     else store_part<T>(p, n, in);
 }
+
+// Elementwise results from 96 MB on are stored past the caches: together with its operands such a tensor does not stay in the 256 MB cache
+// for its reader anyway, and then leaves the operands there.  (layer_norm, dropout with residual and both gradients, one after the other,
+// us, through | past the caches: tensors of 32 MB 78 | 83, 64 MB 136 | 143, 128 MB bf16 295 | 258, 128 MB fp32 273 | 242, 256 MB 582 | 532.)
+static inline bool past_caches(int64_t elements, int dt) { return elements * (int64_t)(dt == IVAE_F32 ? 4 : 2) >= (int64_t)96 << 20; }
 
 static inline size_t dtype_size(int dt) { return dt == IVAE_F32 ? 4 : 2; }

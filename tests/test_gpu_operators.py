@@ -415,6 +415,32 @@ def test_layer_norm_refuses_what_it_does_not_serve():
             call()
 
 
+@pytest.mark.parametrize("dt", R.DTYPES)
+@pytest.mark.parametrize("d", [1031, 2048])
+def test_results_beyond_the_cache(dt, d):
+    """Results of 96 MB and more are stored another way; their rows, and their elements, are those of the two halves."""
+    m = 2 * (((100 << 20) // (d * torch.finfo(dt).bits // 8) + 1) // 2)
+    g = torch.Generator(device=dev()).manual_seed(d)
+    x, dy, r = (torch.randn(m, d, device=dev(), generator=g).to(dt) for _ in range(3))
+    w = torch.randn(d, device=dev(), generator=g).to(dt)
+    parts = slice(0, m // 2), slice(m // 2, m)
+    y, stats = ops.layer_norm(x, w, w, save=True)
+    dx = ops.layer_norm_backward(dy, x, stats, w, residual=r)[0]
+    z = ops.dropout(x, .25, 7, 1, residual=r)
+    keep = ops.dropout(torch.ones_like(x), .25, 7, 1) != 0
+    assert abs(float(keep.float().mean()) - .75) < 1e-3
+    for i, p in enumerate(parts):
+        yp, sp = ops.layer_norm(x[p], w, w, save=True)
+        assert torch.equal(y[p], yp) and torch.equal(stats[:, p], sp)
+        assert torch.equal(dx[p], ops.layer_norm_backward(dy[p], x[p], sp, w, residual=r[p])[0])
+    n = m // 2 * d
+    assert torch.equal(z.view(-1)[:n], ops.dropout(x.view(-1)[:n], .25, 7, 1, residual=r.view(-1)[:n]))
+    v = torch.where(keep, x.float() * (4 / 3), 0.) + r.float()
+    # 4 / 3, the product and the sum are rounded to 24 bits on each side, the result to its type
+    bound = R.u(dt) * v.abs() + R.tiny(dt) + 8 * R.U32 * (v.abs() + r.float().abs())
+    assert bool(((z.float() - v).abs() <= bound).all())
+
+
 # ---- dropout ------------------------------------------------------------------------------------------------------------
 
 
