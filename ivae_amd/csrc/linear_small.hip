@@ -30,16 +30,26 @@ __global__ __launch_bounds__(256) void k_linear_bwd(LinArgs A, LinSplit X, LinSp
     }
 }
 
-// 8 neighbouring sums of `splits` parts of n values
+// 8 neighbouring sums of `splits` parts of n values, four parts under way at a time
 __device__ __forceinline__ void join8(const float* part, int splits, int64_t n, int64_t i, int left, float (&v)[8]) {
-    Raw8<float> u;
-    u.load(part + i, left);
+    Raw8<float> u[4];
+    u[0].load(part + i, left);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = u.at(e);
-    for (int k = 1; k < splits; ++k) {
-        u.load(part + k * n + i, left);
+    for (int e = 0; e < 8; ++e) v[e] = u[0].at(e);
+    int k = 1;
+    if (left == 8)
+        for (; k + 4 <= splits; k += 4) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += u.at(e);
+            for (int j = 0; j < 4; ++j) u[j].load(part + (k + j) * n + i, 8);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += u[j].at(e);
+        }
+    for (; k < splits; ++k) {
+        u[0].load(part + k * n + i, left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += u[0].at(e);
     }
 }
 template <typename T>
@@ -98,13 +108,19 @@ __global__ __launch_bounds__(256) void k_linear_join_bwd(LinArgs A, LinParts J) 
     }
 }
 
-static LinSplit split_of(int64_t P, int64_t Q, int64_t R) {
+// A part sums over 128 (two steps of a tile) or more, where R is `from` or more: in the backward pass a step takes 1.3 to 3.5 us (16 bits without
+// an activation; fp32, xtanh), less in the forward pass, and a join takes 4 us and a launch.  Gradients of 1024 x 96 x 72 in fp32 with xtanh
+// and their join: parts of 256 28 us, of 128 18 us; 300 x 300 x 300: one part 28 us, two 23 us; 256 rows: no difference,
+// unless the other gradient is joined anyway.
+static const int SPLIT_FORWARD = 512, SPLIT_BACKWARD = 257;
+static LinSplit split_of(int64_t P, int64_t Q, int64_t R, int from) {
     LinSplit S;
     S.tp = (P + TP - 1) / TP;
     S.tq = (Q + TQ - 1) / TQ;
-    const int64_t tiles = S.tp * S.tq, most = R / 256;          // a part sums over 256 or more
-    int64_t s = tiles > 0 && tiles < 256 ? 512 / tiles : 1;
-    if (s > most) s = most;
+    const int64_t tiles = S.tp * S.tq;
+    auto parts = [&](int64_t blocks, int64_t len) { return blocks / tiles < R / len ? blocks / tiles : R / len; };
+    // up to one block a CU in parts of 128 or more, up to two in parts of 256 or more
+    int64_t s = tiles == 0 || tiles >= 256 || R < from ? 1 : parts(256, 128) > parts(512, 256) ? parts(256, 128) : parts(512, 256);
     if (s > 64) s = 64;
     if (s < 1) s = 1;
     S.len = ((R + s - 1) / s + TR - 1) / TR * TR;
@@ -115,8 +131,10 @@ static LinSplit split_of(int64_t P, int64_t Q, int64_t R) {
 struct BwdPlan { LinSplit X, W; int64_t off_w, off_b, floats; };
 static BwdPlan plan_bwd(const LinArgs& A) {
     BwdPlan p;
-    p.X = split_of(A.M, A.K, A.N);
-    p.W = split_of(A.N, A.K, A.M);
+    p.X = split_of(A.M, A.K, A.N, SPLIT_BACKWARD);
+    p.W = split_of(A.N, A.K, A.M, SPLIT_BACKWARD);
+    if (p.X.splits > 1 && A.dx) p.W = split_of(A.N, A.K, A.M, 0);
+    else if (p.W.splits > 1 && A.dw) p.X = split_of(A.M, A.K, A.N, 0);
     if (!A.dx) p.X.tp = 0;
     if (!A.dw) p.W.tq = A.db ? 1 : 0;                           // db alone: the first column of tiles sums it
     const int64_t nx = A.dx && p.X.splits > 1 ? p.X.splits * A.M * A.K : 0;
@@ -128,7 +146,7 @@ static BwdPlan plan_bwd(const LinArgs& A) {
 }
 size_t linear_small_ws(const LinArgs& A, bool backward) {
     if (!backward) {
-        const LinSplit S = split_of(A.M, A.N, A.K);
+        const LinSplit S = split_of(A.M, A.N, A.K, SPLIT_FORWARD);
         return S.splits > 1 ? (size_t)S.splits * A.M * A.N * 4 : 0;
     }
     return (size_t)plan_bwd(A).floats * 4;
@@ -159,7 +177,7 @@ hipError_t linear_join_backward(const LinArgs& A, const LinParts& J0, int dtype,
     return hipGetLastError();
 }
 template <typename T> static void fwd(const LinArgs& A, hipStream_t st) {
-    const LinSplit S = split_of(A.M, A.N, A.K);
+    const LinSplit S = split_of(A.M, A.N, A.K, SPLIT_FORWARD);
     hipLaunchKernelGGL(k_linear_fwd<T>, dim3(cap(S.tp * S.tq * S.splits)), dim3(256), 0, st, A, S);
 }
 hipError_t linear_small_forward(const LinArgs& A, int dtype, hipStream_t st) {
@@ -167,7 +185,7 @@ hipError_t linear_small_forward(const LinArgs& A, int dtype, hipStream_t st) {
     else if (dtype == IVAE_BF16) fwd<bf16_t>(A, st);
     else fwd<f16_t>(A, st);
     const hipError_t e = hipGetLastError();
-    return e != hipSuccess ? e : linear_join_forward(A, split_of(A.M, A.N, A.K).splits, dtype, st);
+    return e != hipSuccess ? e : linear_join_forward(A, split_of(A.M, A.N, A.K, SPLIT_FORWARD).splits, dtype, st);
 }
 template <typename T> static void bwd(const LinArgs& A, const BwdPlan& p, float* pw, float* pb, hipStream_t st) {
     const int64_t tiles = p.X.tp * p.X.tq * p.X.splits + p.W.tp * p.W.tq * p.W.splits;
