@@ -79,7 +79,7 @@ hipError_t launch_dropout(int dtype, int64_t n, const void* x, const void* resid
     A.scale = A.all ? 0.f : (float)(1.0 / (1.0 - p));
     A.k0 = (uint32_t)seed; A.k1 = (uint32_t)(seed >> 32);
     A.offset = offset; A.offset_dev = offset_dev;
-    A.past = past_caches(n, dtype);
+    A.past = past_caches((double)n, dtype);
     const int per = dtype == IVAE_F32 ? 4 : 8;
     int64_t blocks = ((n + per - 1) / per + 255) / 256;
     if (blocks > 8192) blocks = 8192;

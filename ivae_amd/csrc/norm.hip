@@ -410,7 +410,7 @@ hipError_t launch_layer_norm(const IvaeNorm& N, const void* x, const void* w, co
     NormArgs A = {};
     A.x = x; A.w = w; A.b = b; A.y = y; A.stats = stats;
     A.rows = N.rows; A.ldx = N.ldx; A.D = N.width; A.w_f32 = N.weight_f32 || N.dtype == IVAE_F32; A.eps = N.eps;
-    A.past = past_caches(N.rows * N.width, N.dtype);
+    A.past = past_caches((double)N.rows * N.width, N.dtype);
     if (N.dtype == IVAE_F32) norm_fwd<float>(A, st);
     else if (N.dtype == IVAE_BF16) norm_fwd<bf16_t>(A, st);
     else norm_fwd<f16_t>(A, st);
@@ -439,7 +439,7 @@ hipError_t launch_layer_norm_backward(const IvaeNorm& N, const void* dy, const v
     NormArgs A = {};
     A.x = x; A.dy = dy; A.w = w; A.residual = residual; A.y = dx; A.cstats = stats; A.part = dg || dc ? ws : nullptr;
     A.rows = N.rows; A.ldx = N.ldx; A.lddy = N.lddy; A.ldr = N.ld_residual; A.D = N.width; A.w_f32 = N.weight_f32 || N.dtype == IVAE_F32;
-    A.past = past_caches(N.rows * N.width, N.dtype);
+    A.past = past_caches((double)N.rows * N.width, N.dtype);
     const int blocks = norm_blocks(N.rows, N.width, N.dtype);
     if (N.dtype == IVAE_F32) norm_bwd<float>(A, blocks, dg, dc, st);
     else if (N.dtype == IVAE_BF16) norm_bwd<bf16_t>(A, blocks, dg, dc, st);

@@ -61,6 +61,6 @@ template <typename T, int N> __device__ __forceinline__ void store_some(T* p, in
 // Elementwise results from 96 MB on are stored past the caches: together with its operands such a tensor does not stay in the 256 MB cache
 // for its reader anyway, and then leaves the operands there.  (layer_norm, dropout with residual and both gradients, one after the other,
 // us, through | past the caches: tensors of 32 MB 78 | 83, 64 MB 136 | 143, 128 MB bf16 295 | 258, 128 MB fp32 273 | 242, 256 MB 582 | 532.)
-static inline bool past_caches(int64_t elements, int dt) { return elements * (int64_t)(dt == IVAE_F32 ? 4 : 2) >= (int64_t)96 << 20; }
+static inline bool past_caches(double elements, int dt) { return elements * (dt == IVAE_F32 ? 4 : 2) >= 96 * 1048576.0; }
 
 static inline size_t dtype_size(int dt) { return dt == IVAE_F32 ? 4 : 2; }
