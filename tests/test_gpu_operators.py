@@ -394,6 +394,20 @@ def test_layer_norm_constant_rows_and_parts():
     assert y.shape == dx.shape == (0, 9) and float(dw.abs().sum()) == 0 and float(db.abs().sum()) == 0
 
 
+@pytest.mark.parametrize("dt", R.DTYPES)
+@pytest.mark.parametrize("m,d", [(1, 8), (24, 64), (25, 64), (23, 50), (6, 2048), (3, 1037), (2, 16384), (3, 16381)])
+def test_layer_norm_few_rows(dt, m, d):
+    """Up to six rows of a block's share of threads are one block's, which writes the weight's gradients itself."""
+    for wdtype in (dt, F32):
+        X, D, stats, full = run_norm(dt, m, d, wdtype=wdtype, seed=m + d, residual=True)
+        w = torch.ones(d, device=dev(), dtype=wdtype)
+        one = ops.layer_norm_backward(D, X, stats, w)
+        for need in ((True, False, False), (False, True, False), (False, False, True), (False, False, False)):
+            part = ops.layer_norm_backward(D, X, stats, w, need=need)
+            assert all((b is None) if not n else torch.equal(a, b) for a, b, n in zip(one, part, need))
+        assert all(torch.equal(a, b) for a, b in zip(one[1:], full[1:]))          # (they do not depend on the weight)
+
+
 def test_layer_norm_nan_stays_in_its_row():
     g = torch.Generator().manual_seed(7)
     x = normal(g, 20, 300).to(dev())
