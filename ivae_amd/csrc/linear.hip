@@ -169,13 +169,13 @@ static hipError_t big_backward(const LinArgs& A, int dtype, void* ws, hipStream_
 // ---- which kernel -----------------------------------------------------------------------------------------------------
 static bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
 // The large kernels from the size on from which they take less time, all their launches together (us, small | large):
-//   16 bits, forward    2048 x 512 x 1024 14 | 16, 1024 x 1024 x 1024 19 | 25, 2048 x 1024 x 1024 26 | 21, 128 x 4096 x 4096 33 | 22;
-//                       1531 x 1001 x 777 34 | 31
-//   16 bits, backward   128 x 512 x 512 18 | 17, 1024 x 512 x 512 28 | 22, 1024 x 1024 x 1024 66 | 29 (but the small kernel does not round
-//                       act' dy: it keeps what it loses little by)
-//   fp32, forward       1024 x 1024 x 1024 30 | 42, 2048 x 1024 x 1024 48 | 55, 300 x 4096 x 2048 80 | 76, 128 x 4096 x 4096 51 | 74
-//                       (cutting the weight in three costs as much as a product with 128 rows); 1531 x 1001 x 777 65 | 50
-//   fp32, backward      512 x 512 x 512 27 | 29, 1024 x 512 x 512 35 | 33, 1024 x 1024 x 1024 96 | 52
+//   16 bits, forward    2048 x 512 x 1024 14 | 15, 1024 x 1024 x 1024 20 | 27, 2048 x 1024 x 1024 26 | 19, 128 x 4096 x 4096 34 | 23;
+//                       1531 x 1001 x 777 34 | 29
+//   16 bits, backward   1024 x 256 x 256 15 | 17, 512 x 512 x 512 20 | 18, 1024 x 512 x 512 27 | 21, 1024 x 1024 x 1024 66 | 28 (but the small
+//                       kernel does not round act' dy: it keeps what it loses little by)
+//   fp32, forward       1024 x 1024 x 1024 31 | 40, 2048 x 1024 x 1024 48 | 54, 300 x 4096 x 2048 81 | 75, 128 x 4096 x 4096 51 | 75
+//                       (cutting the weight in three costs as much as a product with 128 rows); 1531 x 1001 x 777 65 | 47
+//   fp32, backward      512 x 512 x 512 25 | 27, 1024 x 512 x 512 36 | 30, 1024 x 1024 x 1024 96 | 47
 // Forward, rows that do not start on 16 bytes cost the small kernel twice the loads, the large one only its packing.
 static bool big_by_size(const LinArgs& A, int dtype, bool backward) {
     const int64_t lds[] = {A.ldx, A.lddy, A.K, A.N};
@@ -186,7 +186,7 @@ static bool big_by_size(const LinArgs& A, int dtype, bool backward) {
     const double flops = 2.0 * (double)A.M * (double)A.N * (double)A.K;
     const bool ragged = A.K % (dtype == IVAE_F32 ? 4 : 8) != 0;
     if (dtype == IVAE_F32) return backward ? flops >= 5e8 : flops >= (ragged ? 2e9 : 5e9) && A.M >= 256;
-    return flops >= (backward ? 1e8 : ragged ? 2e9 : 3e9);
+    return flops >= (backward ? 2e8 : ragged ? 2e9 : 3e9);
 }
 // a matrix that would be loaded in place has to start on 16 bytes
 static bool big_in_place(const void* p, int64_t cols, int64_t ld, int dtype) { return dtype == IVAE_F32 || ld % 8 || cols % 8 || aligned(p); }
