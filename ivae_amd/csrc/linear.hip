@@ -17,27 +17,28 @@ static const int64_t BIG_MAX_LD = 1 << 21;              // 32-bit byte offsets i
 
 static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 static int64_t tiles_of(const BigProduct& B, int tp, int tq) { return ((B.p_end + tp - 1) / tp) * ((B.q_end + tq - 1) / tq); }
-// Tiles and splits of the products of one launch: the choice for which a simple model of its time is least.  A block takes `start` us and
-// `per` ns for each of its summed index (measured: a 256 x 256 tile of 16-bit values 27 ns, bound by the matrix cores; a 128 x 128
-// tile 17 ns, bound by the latency of its loads; split fp32 82 and 60 ns); blocks beyond one a CU queue up; split sums are written,
-// read and joined at 4 TB/s and one more launch.
-struct BigModel { int tile_p, tile_q; double start, per; int slots; };
+// Tiles and splits of the products of one launch: the choice for which a simple model of its time is least.  A round of 256 blocks, one a
+// CU, takes `start` us (those after the first `again` of it) and `per` ns for each of its summed index (fitted to products of one to four
+// rounds: 16 bits, 256 x 256 and 128 x 128 tiles, the small ones two a CU; split fp32, 256 x 128 and 128 x 128); split sums cost a launch
+// and are joined at 6 TB/s.  What it decides between (us, forward, 256-wide | 128-wide): fp16 4096 x 4096 x 4096 114 | 136,
+// 4096 x 2048 x 2048 53 | 42, 8192 x 1024 x 1024 36 | 26; fp32 4096 x 1024 x 4096 197 | 216, 2048 x 2048 x 2048 118 | 109.
+struct BigModel { int tile_p, tile_q; double start, again, per; };
 static double big_time(BigProduct** B, int n, const BigModel& m, const int64_t* s) {
-    double work = 0, longest = 0, join = 0;
+    double load = 0, longest = 0, join = 0;
     int64_t blocks = 0;
     for (int i = 0; i < n; ++i) {
-        const int64_t tiles = tiles_of(*B[i], m.tile_p, m.tile_q) * s[i];
-        const double t = m.start + 1e-3 * m.per * (double)((B[i]->R + s[i] - 1) / s[i]);
-        work += (double)tiles * t;
+        const int64_t tiles = tiles_of(*B[i], m.tile_p, m.tile_q) * s[i], len = (B[i]->R + s[i] - 1) / s[i];
+        load += (double)tiles * (double)len;
         blocks += tiles;
-        if (t > longest) longest = t;
-        if (s[i] > 1) join += 3.0 + (double)(2 * s[i] + 1) * (double)B[i]->p_end * (double)B[i]->q_end * 4 / 4e6;
+        if ((double)len > longest) longest = (double)len;
+        if (s[i] > 1) join += 4.0 + ((double)s[i] + 0.5) * (double)B[i]->p_end * (double)B[i]->q_end * 4 / 6e6;
     }
-    return (blocks <= m.slots ? longest : work / m.slots + 0.5 * longest) + join;
+    const double rounds = (double)((blocks + 255) / 256), each = blocks ? rounds * load / (double)blocks : 0;
+    return m.start * (1 + m.again * (rounds - 1)) + 1e-3 * m.per * (each > longest ? each : longest) + join;
 }
 static void big_geometry(BigProduct** B, int n, int dtype) {
-    static const BigModel m16[2] = {{256, 256, 10.0, 27.0, 256}, {128, 128, 4.0, 17.0, 256}};
-    static const BigModel m32[2] = {{256, 128, 10.0, 82.0, 256}, {128, 128, 5.0, 60.0, 256}};
+    static const BigModel m16[2] = {{256, 256, 15.0, 0.3, 24.5}, {128, 128, 10.0, 0.1, 7.6}};
+    static const BigModel m32[2] = {{256, 128, 20.0, 0.5, 72.0}, {128, 128, 14.0, 0.5, 41.0}};
     double best = 1e30;
     for (const BigModel& m : dtype == IVAE_F32 ? m32 : m16)
         for (int64_t s0 = 1; s0 <= 16; s0 *= 2)

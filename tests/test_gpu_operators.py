@@ -108,7 +108,7 @@ def test_linear_large(dt, m, k, n):
 
 
 @pytest.mark.parametrize("m,k,n", SIZES + BIG + [(64, 60000, 256), (4096, 200, 264), (8200, 1032, 136), (8192, 512, 4096), (3000, 2000, 2001),
-                                                       (256, 4096, 8200), (20000, 256, 200), (24, 264, 8200), (50, 72, 8195)])
+                                                       (256, 4096, 8200), (20000, 256, 200), (24, 264, 8200), (50, 72, 8195), (2500, 2500, 2500), (8192, 1024, 1024)])
 @pytest.mark.parametrize("dt", R.DTYPES)
 def test_linear_integers_are_exact(dt, m, k, n):
     """Small whole numbers: every product and sum is one too, below 2^24, so each result is the exact one, rounded once to its type."""
