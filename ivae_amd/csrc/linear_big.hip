@@ -170,7 +170,7 @@ __device__ __forceinline__ void touch_residual(const BigProduct& G, const LinArg
     constexpr int E = 64 / sizeof(T), PER_ROW = BTQ / E, LOADS = BTP * PER_ROW / THREADS;
     const uint32_t base = __builtin_amdgcn_readfirstlane(at + threadIdx.x / 64 * 256);
     int64_t q = at0.q0 + threadIdx.x % PER_ROW * E;
-    if (q >= G.q_end) q = G.q_end - 1;
+    if (q > G.q_end - 4 / (int)sizeof(T)) q = G.q_end - 4 / (int)sizeof(T);          // (4 bytes inside the row; there are 64 columns at least)
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
         int64_t p = at0.p0 + threadIdx.x / PER_ROW + j * (THREADS / PER_ROW);
