@@ -247,7 +247,7 @@ int ivae_corr_batched(const float* x, const float* y, int64_t n_blocks, int64_t 
 /* y = act(x w^T + b) + residual;  x (rows, in_features), w (out_features, in_features), b (out_features) or NULL,
  * residual (rows, out_features) or NULL, y (rows, out_features).
  * saved: NULL, or (rows, out_features) values that the backward pass of an activation other than IVAE_ACT_NONE needs: the
- * pre-activation in fp32, or for IVAE_BF16 in fp16 (clamped to fp16's range, its sign kept).
+ * pre-activation, in fp32 for every type.
  * ivae_linear_backward: dy (rows, out_features) -> dx (rows, in_features), dw (like w), db (out_features); any of them may be
  * NULL.  The gradient of the residual is dy itself.  In large products act'(s) dy is rounded to the element type first.
  * Limits: in_features, out_features <= 2^24, rows <= 2^40: IVAE_E_TOOLARGE. */

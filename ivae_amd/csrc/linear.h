@@ -4,8 +4,8 @@
 
 struct LinArgs {
     const void* x; const void* w; const void* b; const void* res;
-    void* y; void* pre;                    // forward
-    const void* dy; const void* cpre;      // backward
+    void* y; float* pre;                   // forward; pre: or null, the pre-activations in 32 bits for the backward pass
+    const void* dy; const float* cpre;     // backward
     void* dx; void* dw; void* db;
     int64_t M, ldx, ldr, lddy;
     int K, N;
@@ -17,19 +17,6 @@ struct LinArgs {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
-
-// What the forward pass keeps of the pre-activation s for the backward pass's act'(s): 32 bits, but for bf16 operands fp16 --
-// act' is a function of moderate s, where fp16 has 3 bits more than the gradients around it.  |s| beyond fp16's range is clamped
-// (act' has reached its limit there) and a positive s never becomes 0, so lrelu's side is kept.  (For fp16 operands fp16 would
-// add an error as large as that of rounding a gradient: x 1.5 together where 32 bits stay at x 1.41.)
-template <typename T> struct Pre { typedef float t; };
-template <> struct Pre<bf16_t> { typedef f16_t t; };
-__device__ __forceinline__ float pre_pack(float s, float) { return s; }
-__device__ __forceinline__ f16_t pre_pack(float s, f16_t) {
-    if (s != s) return (f16_t)s;
-    const f16_t h = (f16_t)fminf(fmaxf(s, -65504.f), 65504.f);
-    return s > 0.f && h == (f16_t)0.f ? (f16_t)5.9604645e-8f : h;
-}
 
 // Activations of 16-bit results from the hardware's exp2 and reciprocal (1 unit in the last place of 32 bits each): their errors are
 // at most 2e-7 next to steps of 2^-11 and more, and an epilogue of 128 values a lane costs a third of what the exact forms do.
@@ -120,18 +107,7 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int n, const 
 // What follows the sums of 8 neighbouring results (bias included, n of them inside the matrix, the first at element `at` of y).
 template <typename T>
 __device__ __forceinline__ void forward_store8(const LinArgs& A, int64_t at, int n, float (&v)[8], const Raw8<T>* res) {
-    typedef typename Pre<T>::t pre_t;
-    if (A.pre && n) {
-        struct __attribute__((packed, aligned(sizeof(pre_t)))) { pre_t e[8]; } s;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s.e[e] = pre_pack(v[e], pre_t());
-        pre_t* to = (pre_t*)A.pre + at;
-        if (n == 8) *(decltype(s)*)to = s;
-        else
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < n) to[e] = s.e[e];
-    }
+    if (A.pre && n) store8(A.pre + at, n, v);
     lin_act_all<T>(A.act, A.slope, v);
     if (res)
 #pragma unroll
@@ -142,7 +118,7 @@ __device__ __forceinline__ void forward_store8(const LinArgs& A, int64_t at, int
 template <typename T>
 __device__ __forceinline__ void forward_store(const LinArgs& A, int64_t m, int n, float s) {
     if (A.b) s += to_f(((const T*)A.b)[n]);
-    if (A.pre) ((typename Pre<T>::t*)A.pre)[m * A.N + n] = pre_pack(s, typename Pre<T>::t());
+    if (A.pre) A.pre[m * A.N + n] = s;
     s = lin_act<T>(A.act, A.slope, s);
     if (A.res) s += to_f(((const T*)A.res)[m * A.ldr + n]);
     ((T*)A.y)[m * A.N + n] = from_f<T>(s);

@@ -206,7 +206,7 @@ size_t linear_ws_bytes(const IvaeLinear& L, bool backward) {
 hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, const void* b, const void* residual, void* y, void* saved,
                          void* ws, hipStream_t st) {
     LinArgs A = lin_args(L);
-    A.x = x; A.w = w; A.b = b; A.res = residual; A.y = y; A.pre = saved; A.part = (float*)ws;
+    A.x = x; A.w = w; A.b = b; A.res = residual; A.y = y; A.pre = (float*)saved; A.part = (float*)ws;
     if (A.M <= ROWS_MAX) return linear_rows_forward(A, L.dtype, st);
     if (big_by_size(A, L.dtype, false) && big_in_place(x, A.K, A.ldx, L.dtype) && big_in_place(w, A.K, A.K, L.dtype) && aligned(ws))
         return big_forward(A, L.dtype, ws, st);
@@ -215,7 +215,7 @@ hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, cons
 hipError_t launch_linear_backward(const IvaeLinear& L, const void* dy, const void* x, const void* w, const void* saved, void* dx, void* dw,
                                   void* db, void* ws, hipStream_t st) {
     LinArgs A = lin_args(L);
-    A.x = x; A.w = w; A.dy = dy; A.cpre = saved; A.dx = dx; A.dw = dw; A.db = db; A.part = (float*)ws;
+    A.x = x; A.w = w; A.dy = dy; A.cpre = (const float*)saved; A.dx = dx; A.dw = dw; A.db = db; A.part = (float*)ws;
     if (big_by_size(A, L.dtype, true) && (A.act != IVAE_ACT_NONE || big_in_place(dy, A.N, A.lddy, L.dtype)) && (!dw || big_in_place(x, A.K, A.ldx, L.dtype)) &&
         (!dx || big_in_place(w, A.K, A.K, L.dtype)) && aligned(ws))
         return big_backward(A, L.dtype, ws, st);

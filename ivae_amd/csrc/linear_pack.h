@@ -6,7 +6,7 @@ enum { FLIP_NONE, FLIP_ROWS, FLIP_COLS };
 
 struct PackArgs {
     const void* src;            // (rows, cols), row stride ld
-    const void* pre;            // or null: (rows, cols) saved pre-activations; the values become act'(pre) src
+    const float* pre;           // or null: (rows, cols) saved pre-activations; the values become act'(pre) src
     void* out;                  // or null: (rows, ldo) of the same type, or for fp32 three bf16 matrices `plane` elements apart, each in
                                 // columns of 32 values and `rows` rows (linear_big.h)
     float* colsum;              // or null: (row blocks, cols) sums over the rows

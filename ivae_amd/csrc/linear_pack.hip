@@ -22,7 +22,6 @@ __device__ __forceinline__ void cut(float x, bf16_t (&o)[3]) {
 struct PackJobs { PackArgs job[3]; };
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack(PackJobs J) {
-    typedef typename Pre<T>::t pre_t;
     int block = blockIdx.x, k = 0;
     while (block >= J.job[k].blocks) block -= J.job[k++].blocks;
     const PackArgs& A = J.job[k];
@@ -44,15 +43,14 @@ __global__ __launch_bounds__(256) void k_pack(PackJobs J) {
             for (int j = 0; j < N; ++j) v[h * N + j] = u[j];
         }
         if (A.pre) {
-            const pre_t* q = (const pre_t*)A.pre + r * A.cols + col;
-            constexpr int NP = Wide<pre_t>::N;
+            const float* q = A.pre + r * A.cols + col;
 #pragma unroll
-            for (int h = 0; h < 8 / NP; ++h) {
-                float u[NP];
-                if (left - h * NP >= NP) load_wide<pre_t>(q + h * NP, u);
-                else load_part<pre_t>(q + h * NP, left - h * NP, u);
+            for (int h = 0; h < 8; h += 4) {
+                float u[4];
+                if (left - h >= 4) load_wide<float>(q + h, u);
+                else load_part<float>(q + h, left - h, u);
 #pragma unroll
-                for (int j = 0; j < NP; ++j) s[h * NP + j] = u[j];
+                for (int j = 0; j < 4; ++j) s[h + j] = u[j];
             }
             lin_act_slope_all<T>(A.act, A.slope, s, v);
         }

@@ -152,8 +152,6 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
     const T* x = (const T*)A.x;
     const T* w = (const T*)A.w;
     const T* dy = (const T*)A.dy;
-    typedef typename Pre<T>::t pre_t;
-    const pre_t* pre = (const pre_t*)A.cpre;
 
     float vp[2][8], vq[2][8], sum[8] = {};
     auto fetch = [&](int64_t r0) {
@@ -165,7 +163,7 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
             fetch_tile<T, RC>(t, dy, A.lddy, p0, P, r0, rb, vp);
             if (A.act != IVAE_ACT_NONE) {
                 float s[2][8];
-                fetch_tile<pre_t, RC>(t, pre, A.N, p0, P, r0, rb, s);
+                fetch_tile<float, RC>(t, A.cpre, A.N, p0, P, r0, rb, s);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) lin_act_slope_all<T>(A.act, A.slope, s[h], vp[h]);
             }

@@ -387,7 +387,6 @@ def train_steps(shape, coef, params, exp_avg, exp_avg_sq, x_data, u_data, batch_
 # allocate their outputs, and raise on anything they do not serve.  All of them can be captured into a graph.
 
 DTYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_SAVED = (torch.float32, torch.float16, torch.float32)       # of linear's pre-activation, by type id
 
 
 def _dtype_id(t, name):
@@ -482,7 +481,7 @@ def _linear_shapes(x, weight, activation):
 def linear(x, weight, bias=None, activation="none", slope=.1, residual=None, save=False):
     """ivae_linear: act(x weight^T + bias) + residual, for x (..., in), weight (out, in), bias (out,), residual (..., out) of one
     type; activation: none, lrelu (slope), xtanh (tanh(s) + slope s), sigmoid, gelu (the erf form), silu.
-    -> y, or with save=True (y, saved): saved is what linear_backward needs of the pre-activation, None for 'none'."""
+    -> y, or with save=True (y, saved): saved (like y, float32) is the pre-activation, which linear_backward needs; None for 'none'."""
     dt, act, rows, k, n = _linear_shapes(x, weight, activation)
     out = (rows, n) if x.dim() == 2 else (*x.shape[:-1], n)
     if bias is not None:
@@ -495,7 +494,7 @@ def linear(x, weight, bias=None, activation="none", slope=.1, residual=None, sav
     dev = x.device
     lin, nb = _linear_plan(rows, k, n, dt, act, float(slope), ldx, ldr, 0, 0)
     y = x.new_empty(out)
-    saved = _empty(x, out, _SAVED[dt]) if save and act else None
+    saved = _empty(x, out, torch.float32) if save and act else None
     ws = _empty(x, nb, torch.uint8) if nb else None
     _call(dev, _lib.lib().ivae_linear, "ivae_linear", lin, x.data_ptr(), weight.data_ptr(), _opt(bias), _opt(residual), y.data_ptr(), _opt(saved),
           _opt(ws), nb)
@@ -511,7 +510,7 @@ def linear_backward(dy, x, weight, saved=None, activation="none", slope=.1, need
     if act:
         if saved is None:
             raise ValueError("the backward pass of an activation needs linear's `saved` (save=True)")
-        saved = _dense(_like(saved, x, "saved", out, _SAVED[dt]))
+        saved = _dense(_like(saved, x, "saved", out, torch.float32))
     else:
         saved = None
     shape = x.shape
