@@ -510,8 +510,8 @@ __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A
         wait_loads<0>();
         __syncthreads();
         for (int u = group; u < SUBS; u += GROUPS)
-            tile_product<float, MODE>(threadIdx.x % 256, B, S, at0.split, at0.p0 + u / (BTQ / 64) * 64, at0.q0 + u % (BTQ / 64) * 64, G.part, nullptr,
-                                      smem + group * tile_lds<float>(true));
+            tile_product<float, float, MODE>(threadIdx.x % 256, B, S, at0.split, at0.p0 + u / (BTQ / 64) * 64, at0.q0 + u % (BTQ / 64) * 64, G.part, nullptr,
+                                      smem + group * tile_lds<float>());
         return;
     }
     finish<float, BTP, BTQ, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
@@ -564,7 +564,7 @@ template <typename T, int BT, int WP, int WQ, int BUFS> struct Big16 {
 };
 template <int BTP, int BTQ, int BUFS> struct Big32 {
     static constexpr int THREADS = BTP * BTQ / 64, LDS = big_lds(BUFS, 3 * (BTP + BTQ) * 32 * 2, BTQ) + THREADS * 4;
-    static_assert(LDS >= THREADS / 256 * tile_lds<float>(true), "a tile with a NaN is computed again here");
+    static_assert(LDS >= THREADS / 256 * tile_lds<float>(), "a tile with a NaN is computed again here");
     static hipError_t fwd(const BigProduct& B, const LinArgs& A, hipStream_t st) {
         static SmemCache cache;
         return go(k_split_fwd<BTP, BTQ, BUFS>, LDS, THREADS, cache, blocks_of(B), st, B, A);

@@ -12,21 +12,21 @@ __device__ __forceinline__ At at_of(const LinSplit& S, int64_t b) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_linear_fwd(LinArgs A, LinSplit S) {
-    __shared__ __attribute__((aligned(16))) char smem[tile_lds<T>(false)];
+    __shared__ __attribute__((aligned(16))) char smem[tile_lds<T>()];
     const int64_t tiles = S.tp * S.tq * S.splits;
     for (int64_t b = blockIdx.x; b < tiles; b += gridDim.x) {
         const At at = at_of(S, b);
-        tile_product<T, MODE_FWD>(threadIdx.x, A, S, at.split, at.p0, at.q0, A.part, nullptr, smem);
+        tile_product<T, T, MODE_FWD>(threadIdx.x, A, S, at.split, at.p0, at.q0, A.part, nullptr, smem);
     }
 }
-template <typename T>
+template <typename T, typename C>
 __global__ __launch_bounds__(256) void k_linear_bwd(LinArgs A, LinSplit X, LinSplit W, float* part_w, float* part_b) {
-    __shared__ __attribute__((aligned(16))) char smem[tile_lds<T>(true)];
+    __shared__ __attribute__((aligned(16))) char smem[tile_lds<C>()];
     const int64_t nx = X.tp * X.tq * X.splits, tiles = nx + W.tp * W.tq * W.splits;
     for (int64_t b = blockIdx.x; b < tiles; b += gridDim.x) {
         const At at = b < nx ? at_of(X, b) : at_of(W, b - nx);
-        if (b < nx) tile_product<T, MODE_DX>(threadIdx.x, A, X, at.split, at.p0, at.q0, A.part, nullptr, smem);
-        else tile_product<T, MODE_DW>(threadIdx.x, A, W, at.split, at.p0, at.q0, part_w, part_b, smem);
+        if (b < nx) tile_product<T, C, MODE_DX>(threadIdx.x, A, X, at.split, at.p0, at.q0, A.part, nullptr, smem);
+        else tile_product<T, C, MODE_DW>(threadIdx.x, A, W, at.split, at.p0, at.q0, part_w, part_b, smem);
     }
 }
 
@@ -189,7 +189,10 @@ hipError_t linear_small_forward(const LinArgs& A, int dtype, hipStream_t st) {
 }
 template <typename T> static void bwd(const LinArgs& A, const BwdPlan& p, float* pw, float* pb, hipStream_t st) {
     const int64_t tiles = p.X.tp * p.X.tq * p.X.splits + p.W.tp * p.W.tq * p.W.splits;
-    if (tiles) hipLaunchKernelGGL(k_linear_bwd<T>, dim3(cap(tiles)), dim3(256), 0, st, A, p.X, p.W, pw, pb);
+    if (tiles == 0) return;
+    const dim3 g(cap(tiles)), b(256);
+    if (A.act == IVAE_ACT_NONE) hipLaunchKernelGGL((k_linear_bwd<T, T>), g, b, 0, st, A, p.X, p.W, pw, pb);
+    else hipLaunchKernelGGL((k_linear_bwd<T, float>), g, b, 0, st, A, p.X, p.W, pw, pb);
 }
 hipError_t linear_small_backward(const LinArgs& A, int dtype, hipStream_t st) {
     const BwdPlan p = plan_bwd(A);

@@ -5,9 +5,11 @@
 //   dx       P = m, Q = k, R = n     dx[m,k] = sum_n ds[m,n] w[n,k]
 //   dw       P = n, Q = k, R = m     dw[n,k] = sum_m ds[m,n] x[m,k]        (db[n] = sum_m ds[m,n] on the way)
 // The Q operand is the matrix instruction's first one, so that a lane ends up with 4 neighbouring columns of one row.
-// In the 16-bit types the gradient of the pre-activation, act'(s) dy, enters as the sum of two numbers of the type (the second is
-// the first's rounding error), one more matrix instruction each: these sizes wait for memory and launches, and the products then
-// have no rounding but their result's.
+// T: of the tensors, C: of the products' operands, T or float.  With an activation the gradient of the pre-activation, act'(s) dy, is a
+// number of 32 bits that the 16-bit types cannot hold (fp16 neither its range), so the backward pass then multiplies in fp32: these sizes
+// wait for memory and launches, and the products have no rounding but their result's.  (fp16, gelu, gradients of 64 x 50 x 50 8.1 us,
+// of 256 x 256 x 256 16.6 us; as two numbers of the type, which lose fp16's smallest and largest gradients and make a NaN where
+// an infinity meets a second number of 0, 7.4 and 13.8 us.)
 #pragma once
 #include "linear.h"
 
@@ -52,19 +54,15 @@ __device__ __forceinline__ void fetch_tile(int t, const T* base, int64_t ld, int
     }
 }
 // ... into LDS as they lie in memory, 16 bytes at a time: [row of the tile][summed index] (RC) or [summed index][column of the tile].
-// ERR: what rounding to T leaves of them
-template <typename T, bool RC, bool ERR = false>
-__device__ __forceinline__ void put_tile(int t, T* lds, const float (&u)[2][8]) {
-    constexpr int LD = Lds<T>::LD;
-    struct __attribute__((aligned(16))) V { T e[8]; };
+template <typename C, bool RC>
+__device__ __forceinline__ void put_tile(int t, C* lds, const float (&u)[2][8]) {
+    constexpr int LD = Lds<C>::LD;
+    struct __attribute__((aligned(16))) V { C e[8]; };
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         V v;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float r = to_f(from_f<T>(u[h][j]));
-            v.e[j] = from_f<T>(!ERR ? u[h][j] : fabsf(r) < __builtin_inff() ? u[h][j] - r : 0.f);      // (infinities and NaN are whole in the first number)
-        }
+        for (int j = 0; j < 8; ++j) v.e[j] = from_f<C>(u[h][j]);
         *(V*)(lds + (RC ? (t / 4) * LD + h * 32 + t % 4 * 8 : (h * 32 + t / 8) * LD + t % 8 * 8)) = v;
     }
 }
@@ -102,17 +100,17 @@ template <bool RC> __device__ __forceinline__ f32x4 fragment32(int l, const floa
 }
 
 // one TR-long step of a wave's 32 x 32 part
-template <typename T, bool PRC, bool QRC>
-__device__ __forceinline__ void tile_mma(int t, const T* lp, const T* lq, f32x4 (&acc)[2][2]) {
+template <typename C, bool PRC, bool QRC>
+__device__ __forceinline__ void tile_mma(int t, const C* lp, const C* lq, f32x4 (&acc)[2][2]) {
     const int l = t % 64, w = t / 64;
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(C) == 2) {
 #pragma unroll
         for (int b = 0; b < TR; b += 32) {
-            typename V8<T>::t p[2], q[2];
+            typename V8<C>::t p[2], q[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                p[i] = fragment<T, PRC>(l, lp, w / 2 * 32 + i * 16, b);
-                q[i] = fragment<T, QRC>(l, lq, w % 2 * 32 + i * 16, b);
+                p[i] = fragment<C, PRC>(l, lp, w / 2 * 32 + i * 16, b);
+                q[i] = fragment<C, QRC>(l, lq, w % 2 * 32 + i * 16, b);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -141,12 +139,11 @@ __device__ __forceinline__ void tile_mma(int t, const T* lp, const T* lq, f32x4 
 
 // The tile at (p0, q0), whole or (S.splits > 1) its part over a split of R.  256 threads, numbered t; several such groups of a block may run
 // together if they all walk the same R.  A tile outside the matrix stores nothing.
-template <typename T, int MODE>
+template <typename T, typename C, int MODE>
 __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinSplit& S, int64_t split, int64_t p0, int64_t q0, float* part, float* part_db,
                                              char* smem) {
-    T* lp = (T*)smem;
-    T* lq = lp + TP * Lds<T>::LD;
-    T* le = lq + TQ * Lds<T>::LD;                   // (16-bit types, backward)
+    C* lp = (C*)smem;
+    C* lq = lp + TP * Lds<C>::LD;
     const int64_t P = MODE == MODE_DW ? A.N : A.M, Q = MODE == MODE_FWD ? A.N : A.K, R = MODE == MODE_FWD ? A.K : MODE == MODE_DX ? A.N : A.M;
     const int64_t ra = split * S.len, rb = ra + S.len < R ? ra + S.len : R;
     const T* x = (const T*)A.x;
@@ -178,15 +175,11 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
     if (ra < rb) fetch(ra);
     for (int64_t r = ra; r < rb; r += TR) {
         __syncthreads();
-        put_tile<T, MODE != MODE_DW>(t, lp, vp);
-        put_tile<T, MODE == MODE_FWD>(t, lq, vq);
-        const bool two = sizeof(T) == 2 && MODE != MODE_FWD && A.act != IVAE_ACT_NONE;
-        if (two) put_tile<T, MODE != MODE_DW, true>(t, le, vp);
+        put_tile<C, MODE != MODE_DW>(t, lp, vp);
+        put_tile<C, MODE == MODE_FWD>(t, lq, vq);
         __syncthreads();
         if (r + TR < rb) fetch(r + TR);
-        tile_mma<T, MODE != MODE_DW, MODE == MODE_FWD>(t, lp, lq, acc);
-        if constexpr (sizeof(T) == 2 && MODE != MODE_FWD)
-            if (two) tile_mma<T, MODE != MODE_DW, false>(t, le, lq, acc);
+        tile_mma<C, MODE != MODE_DW, MODE == MODE_FWD>(t, lp, lq, acc);
     }
     // the sums go through LDS, so that what follows runs along rows, 8 columns a thread
     constexpr int LD = TQ + 4;
@@ -242,5 +235,5 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
     __syncthreads();                                // the tiles are free for the next round
 }
 // LDS of one group of 256 threads: the tiles, then the sums
-template <typename T> static constexpr int tile_lds(bool backward) { return (sizeof(T) == 2 && backward ? 3 : 2) * TP * Lds<T>::LD * (int)sizeof(T); }
-static_assert(tile_lds<f16_t>(false) >= TP * (TQ + 4) * 4, "the sums fit");
+template <typename C> static constexpr int tile_lds() { return 2 * TP * Lds<C>::LD * (int)sizeof(C); }
+static_assert(tile_lds<f16_t>() >= TP * (TQ + 4) * 4, "the sums fit");

@@ -8,8 +8,8 @@ from tests import operator_ref as R
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
-# one product that the 64 x 64 kernel takes, one that the large kernels take, and one of odd sizes
-SIZES = [(96, 120, 104), (1024, 768, 520), (1003, 777, 531)]
+# (rows, in, out) that the 64 x 64 kernels take
+SIZES = [(96, 120, 104), (300, 33, 77)]
 GRADS = ("dx", "dw", "db")
 
 
@@ -55,6 +55,19 @@ def gradients(x, w, b, act, dy, slope=R.SLOPE):
     return dict(zip(GRADS, ops.linear_backward(D, X, W, saved, act, slope))), saved
 
 
+@pytest.mark.parametrize("m,k,n", SIZES)
+@pytest.mark.parametrize("act", R.ACTS)
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_gradients_are_rounded_once(dt, act, m, k, n):
+    g = torch.Generator().manual_seed(m + n)
+    x, w, b, dy = normal(g, m, k, dtype=dt), normal(g, n, k, scale=k ** -0.5, dtype=dt), normal(g, n, scale=.3, dtype=dt), normal(g, m, n, dtype=dt)
+    if act == "lrelu":          # no pre-activation near the kink, where the order of a sum decides the side
+        b = torch.where(b >= 0, 1.0, -1.0).to(dt) * 8
+    want, (got, _) = formula(x, w, b, act, dy), gradients(x, w, b, act, dy)
+    for name in GRADS:
+        only_rounded(got[name], want[name], dt, (name, act))
+
+
 @pytest.mark.parametrize("dt", R.DTYPES)
 def test_saved_holds_32_bits(dt):
     """The pre-activation that the backward pass takes act' of, in the tail of gelu's slope: there s off by 2^-9 (half a step of fp16) moves act' by
@@ -66,3 +79,73 @@ def test_saved_holds_32_bits(dt):
     assert saved.dtype == F32 and bool(((saved.cpu().double() - want["s"]).abs() <= R.U32 * 4.25).all())
     err = (got["dx"].cpu().double() - want["dx"]).abs()
     assert bool((err <= (R.u(dt) + 2.0 ** -10) * want["dx"].abs() + R.tiny(dt)).all()), float((err / want["dx"].abs()).max())
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
+@pytest.mark.parametrize("scale", [2.0 ** -17, 2.0 ** -20])
+def test_small_fp16_gradients_keep_their_digits(scale, m, k, n):
+    """dy among fp16's subnormal numbers, and products that the type holds: act'(s) dy has 32 bits on its way into them."""
+    g = torch.Generator().manual_seed(5)
+    x, w = normal(g, m, k, scale=2.0 ** 6, dtype=F16), normal(g, n, k, scale=2.0 ** 8, dtype=F16)
+    dy = normal(g, m, n, scale=scale, dtype=F16)
+    b = normal(g, n, scale=.3, dtype=F16)
+    x[:, 1:] = 0                                # (so that s stays moderate: one product of 2^-8 and 2^8)
+    x[:, 0] = normal(g, m, scale=2.0 ** -8, dtype=F16)
+    want, (got, _) = formula(x, w, b, "gelu", dy), gradients(x, w, b, "gelu", dy)
+    assert float(want["dx"].abs().mean()) > 2.0 ** -13
+    only_rounded(got["dx"], want["dx"], F16, "dx")
+    x = normal(g, m, k, scale=2.0 ** 12, dtype=F16)
+    w = normal(g, n, k, scale=2.0 ** -12 * k ** -0.5, dtype=F16)
+    want, (got, _) = formula(x, w, b, "gelu", dy), gradients(x, w, b, "gelu", dy)
+    # (s is a sum in 32 bits: relative 2^-24 sqrt(k) of numbers of order 1)
+    only_rounded(got["dw"], want["dw"], F16, "dw")
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
+@pytest.mark.parametrize("act,slope", [("gelu", .1), ("lrelu", 2.0), ("lrelu", 1000.0), ("xtanh", 30.0), ("silu", .1)])
+def test_large_fp16_gradients_stay_finite(act, slope, m, k, n):
+    """act'(s) dy beyond 65504, in products that the type holds."""
+    g = torch.Generator().manual_seed(6)
+    x, w = normal(g, m, k, scale=2.0 ** -9, dtype=F16), normal(g, n, k, scale=2.0 ** -8, dtype=F16)
+    b = torch.full((n,), 1.4 if act != "lrelu" else -1.4, dtype=F16)
+    dy = (torch.where(torch.rand(m, n, generator=g) < .5, 1.0, -1.0) * 60000 * (1 - torch.rand(m, n, generator=g) / 16)).to(F16)
+    if slope > 2:
+        dy = (dy.float() / slope * 2).to(F16)
+    want, (got, _) = formula(x, w, b, act, dy, slope), gradients(x, w, b, act, dy, slope)
+    for name in ("dx", "dw"):
+        assert float(want[name].abs().max()) < 65000
+        only_rounded(got[name], want[name], F16, (name, act))
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_infinities_in_gradients_with_an_activation(dt, m, k, n):
+    """x or w infinite where act'(s) dy is a number that the type holds: each product is that infinity, not 0 times it."""
+    g = torch.Generator().manual_seed(7)
+    x, w, dy = normal(g, m, k, dtype=dt), normal(g, n, k, scale=.03, dtype=dt), normal(g, m, n, dtype=dt)
+    dy[dy == 0] = 1
+    b = normal(g, n, dtype=dt)
+    X, W, D = x.to(dev()), w.to(dev()), dy.to(dev())
+    _, saved = ops.linear(X, W, b.to(dev()), "lrelu", 0.5, save=True)
+    clean = ops.linear_backward(D, X, W, saved, "lrelu", 0.5)
+    ds = dy.double() * torch.where(saved.cpu() > 0, 1.0, 0.5)        # half a value is a value of the type
+    X[3, 5], W[7, 2] = float("inf"), -float("inf")
+    dx, dw, db = ops.linear_backward(D, X, W, saved, "lrelu", 0.5)
+    assert torch.equal(dw[:, 5].cpu().double(), torch.sign(ds[3]) * float("inf"))
+    assert torch.equal(dx[:, 2].cpu().double(), -torch.sign(ds[:, 7]) * float("inf"))
+    cols, ok = [j for j in range(k) if j != 5], [j for j in range(k) if j != 2]
+    want = {"dx": ds @ w.double(), "dw": ds.t() @ x.double()}
+    for name, t, keep in (("dx", dx, ok), ("dw", dw, cols)):
+        if dt == F32:
+            mag = ds.abs() @ w.double().abs() if name == "dx" else ds.abs().t() @ x.double().abs()
+            R.close(t[:, keep], (want[name][:, keep], (R.U32 * ((m if name == "dw" else n) + 16) * mag)[:, keep]), name)
+        else:
+            only_rounded(t[:, keep], want[name][:, keep], dt, name)
+    assert torch.equal(db, clean[2])
+    # ... and an infinite gradient
+    D[4, 6] = float("inf")
+    X[3, 5], W[7, 2] = x[3, 5], w[7, 2]
+    dx, dw, db = ops.linear_backward(D, X, W, saved, "lrelu", 0.5)
+    assert torch.equal(dx[4].cpu().double(), torch.sign(w[6].double()) * float("inf"))
+    assert torch.equal(dw[6].cpu().double(), torch.sign(x[4].double()) * float("inf")) and float(db[6]) == float("inf")
+    assert torch.isfinite(dx[:4]).all() and torch.isfinite(dx[5:]).all() and torch.isfinite(dw[:6]).all() and torch.isfinite(dw[7:]).all()
