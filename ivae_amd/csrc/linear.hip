@@ -1,4 +1,6 @@
 // Dispatch of the linear operator (ivae_linear, ivae_linear_backward) to its kernels.
+#include <math.h>
+
 #include "kernels.h"
 #include "linear_big.h"
 #include "linear_pack.h"
@@ -27,7 +29,7 @@ static double big_time(BigProduct** B, int n, const BigModel& m, const int64_t* 
     double load = 0, longest = 0, join = 0;
     int64_t blocks = 0;
     for (int i = 0; i < n; ++i) {
-        const int64_t tiles = tiles_of(*B[i], m.tile_p, m.tile_q) * s[i], len = (B[i]->R + s[i] - 1) / s[i];
+        const int64_t tiles = tiles_of(*B[i], m.tile_p, m.tile_q) * s[i], len = (B[i]->R + s[i] - 1) / s[i] * (B[i]->pair ? 2 : 1);
         load += (double)tiles * (double)len;
         blocks += tiles;
         if ((double)len > longest) longest = (double)len;
@@ -69,17 +71,17 @@ struct Bytes {                                          // a workspace, handed o
 
 // A matrix as an operand: in place where its rows are 16-byte groups already, packed otherwise (fp32 always)
 struct Packed { BigOperand O; PackArgs P; bool needed; };
-static Packed pack_of(const void* src, int64_t rows, int cols, int64_t ld, int dtype, Bytes& ws, bool must = false) {
+static Packed pack_of(const void* src, int64_t rows, int cols, int64_t ld, int dtype, Bytes& ws, bool pair = false) {
     Packed r = {};
-    r.needed = must || dtype == IVAE_F32 || ld % 8 != 0 || cols % 8 != 0;
+    r.needed = pair || dtype == IVAE_F32 || ld % 8 != 0 || cols % 8 != 0;
     if (!r.needed) {
         r.O = {src, ld, 0, 0, 0, false};
         r.P.ldo = cols;
         return r;
     }
     const int64_t ldo = up(cols, 64), plane = rows * ldo;           // (fp32: columns of 32, `rows` long each)
-    void* out = ws.take<uint16_t>(plane * (dtype == IVAE_F32 ? 3 : 1));
-    r.P.src = src; r.P.out = out; r.P.rows = rows; r.P.cols = cols; r.P.ld = ld; r.P.ldo = ldo; r.P.plane = plane;
+    void* out = ws.take<uint16_t>(plane * (dtype == IVAE_F32 ? 3 : pair ? 2 : 1));
+    r.P.src = src; r.P.out = out; r.P.rows = rows; r.P.cols = cols; r.P.ld = ld; r.P.ldo = ldo; r.P.plane = plane; r.P.pair = pair;
     r.O = {out, dtype == IVAE_F32 ? rows : ldo, 0, 0, plane, false};
     return r;
 }
@@ -123,11 +125,31 @@ static hipError_t big_forward(LinArgs A, int dtype, void* ws, hipStream_t st) {
     return e;
 }
 
+// |act'(s)| <= 2^shift (0 at least).  fp16 pairs serve up to SHIFT_MAX: each more costs the smallest gradients a bit.
+static const int SHIFT_MAX = 4;
+static float slope_bound(int act, float slope) {
+    switch (act) {
+        case IVAE_ACT_LRELU: return fmaxf(1.f, fabsf(slope));
+        case IVAE_ACT_XTANH: return fmaxf(fabsf(slope), fabsf(1.f + slope));
+        case IVAE_ACT_GELU: return 1.13f;
+        case IVAE_ACT_SILU: return 1.1f;
+        default: return 1.f;
+    }
+}
+static int slope_shift(int act, float slope) {
+    const float c = slope_bound(act, slope);
+    int e = 0;
+    while (e < SHIFT_MAX && c > (float)(1 << e)) ++e;
+    return e;
+}
 struct BigBackward { Packed ds, x, w; BigProduct X, W; float* colsum; int kb; size_t bytes; };
 static BigBackward plan_big_backward(const LinArgs& A, int dtype, void* ws) {
     BigBackward f = {};
     Bytes m = {(char*)ws, 0};
-    f.ds = pack_of(A.dy, A.M, A.N, A.lddy, dtype, m, A.act != IVAE_ACT_NONE);
+    const bool pair = dtype != IVAE_F32 && A.act != IVAE_ACT_NONE;
+    f.ds = pack_of(A.dy, A.M, A.N, A.lddy, dtype, m, pair);
+    const int shift = dtype == IVAE_F16 ? slope_shift(A.act, A.slope) : 0;
+    f.ds.P.scale = ldexpf(1.f, -shift); f.ds.P.up = dtype == IVAE_F16 ? 2048.f : 1.f;
     f.ds.P.pre = A.act != IVAE_ACT_NONE ? A.cpre : nullptr;
     f.ds.P.act = A.act; f.ds.P.slope = A.slope;
     if (!f.ds.needed) {                                 // dy itself; only its column sums are taken
@@ -149,6 +171,7 @@ static BigBackward plan_big_backward(const LinArgs& A, int dtype, void* ws) {
     W.p_end = A.N; W.q_end = A.K; W.R = A.M;
     W.out = A.dw;
     BigProduct* both[2] = {&X, &W};
+    for (BigProduct* B : both) B->pair = pair, B->scale = ldexpf(1.f, shift), B->low = 1.f / f.ds.P.up;
     big_geometry(both, 2, dtype);
     for (BigProduct* B : both) {
         if (B->splits > 1) B->part = m.take<float>(B->splits * B->p_end * B->q_end);
@@ -172,8 +195,9 @@ static bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
 // The large kernels from the size on from which they take less time, all their launches together (us, small | large):
 //   16 bits, forward    2048 x 512 x 1024 14 | 15, 1024 x 1024 x 1024 20 | 27, 2048 x 1024 x 1024 26 | 19, 128 x 4096 x 4096 34 | 23;
 //                       1531 x 1001 x 777 34 | 29
-//   16 bits, backward   1024 x 256 x 256 15 | 17, 512 x 512 x 512 20 | 18, 1024 x 512 x 512 27 | 21, 1024 x 1024 x 1024 66 | 28 (but the small
-//                       kernel does not round act' dy: it keeps what it loses little by)
+//   16 bits, backward   no activation 1024 x 256 x 256 11 | 14, 512 x 512 x 512 13 | 14, 1003 x 777 x 531 28 | 25, 768 x 768 x 768 24 | 17
+//                       gelu (the small kernel in fp32, the large one in pairs) 512 x 512 x 512 20 | 22, 300 x 1001 x 777 34 | 23,
+//                       1024 x 512 x 512 31 | 27, 1024 x 1024 x 1024 84 | 36
 //   fp32, forward       1024 x 1024 x 1024 31 | 40, 2048 x 1024 x 1024 48 | 54, 300 x 4096 x 2048 81 | 75, 128 x 4096 x 4096 51 | 75
 //                       (cutting the weight in three costs as much as a product with 128 rows); 1531 x 1001 x 777 65 | 47
 //   fp32, backward      512 x 512 x 512 25 | 27, 1024 x 512 x 512 36 | 30, 1024 x 1024 x 1024 96 | 47
@@ -184,10 +208,11 @@ static bool big_by_size(const LinArgs& A, int dtype, bool backward) {
         if (ld > BIG_MAX_LD) return false;
     // (blocks are counted, and bytes inside a tile of fp32 columns offset, in 32 bits)
     if (A.M < 64 || A.N < 64 || A.K < 64 || A.M >= (dtype == IVAE_F32 ? 1 << 22 : 1 << 29)) return false;
+    if (backward && dtype == IVAE_F16 && !(isfinite(A.slope) && slope_bound(A.act, A.slope) <= (float)(1 << SHIFT_MAX))) return false;
     const double flops = 2.0 * (double)A.M * (double)A.N * (double)A.K;
     const bool ragged = A.K % (dtype == IVAE_F32 ? 4 : 8) != 0;
     if (dtype == IVAE_F32) return backward ? flops >= 5e8 : flops >= (ragged ? 2e9 : 5e9) && A.M >= 256;
-    return flops >= (backward ? 2e8 : ragged ? 2e9 : 3e9);
+    return flops >= (backward ? A.act == IVAE_ACT_NONE ? 2e8 : 3e8 : ragged ? 2e9 : 3e9);
 }
 // a matrix that would be loaded in place has to start on 16 bytes
 static bool big_in_place(const void* p, int64_t cols, int64_t ld, int dtype) { return dtype == IVAE_F32 || ld % 8 || cols % 8 || aligned(p); }

@@ -7,7 +7,8 @@
 // Rows start at multiples of 16 bytes and hold whole 16-byte groups.  Split fp32 is stored in columns of 32 values, ld rows each
 // (value (r, c) at (c / 32 * ld + r) * 32 + c % 32): what a step loads of a tile lies in one piece, or (down) in pieces of 2 KB, where
 // rows of 64 bytes out of a row-major matrix would use half of each cache line.  `limit` is the end of the stored values along R (a multiple
-// of 8 where `along`; values between R and limit are 0).  Split fp32: of every second 32 along R, Q has its sign turned.  `plane`: elements between the three parts of split fp32 values.
+// of 8 where `along`; values between R and limit are 0).  Split fp32: of every second 32 along R, Q has its sign turned.  `plane`: elements between the three parts of split fp32 values,
+// or the two numbers of a pair.
 struct BigOperand {
     const void* base;
     int64_t ld, extent, limit, plane;
@@ -24,6 +25,8 @@ struct BigProduct {
     int tile_p, tile_q;         // 16-bit types: 256 x 256 or 128 x 128; fp32: 256 x 128 or 128 x 128
     int splits;
     int64_t len;                // R of a split, a multiple of 64
+    bool pair;                  // 16-bit types: P's values are scale (first + low second), two numbers of the type
+    float scale, low;           // powers of two
 };
 
 int64_t big_tiles(const BigProduct& B);

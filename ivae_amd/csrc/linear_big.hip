@@ -7,6 +7,13 @@
 // LDS rows cannot be padded (a load fills them in lane order), so the 16-byte groups of a row are permuted instead, by an XOR with
 // bits of the row number that puts every 16 lanes (along) or every 8 groups of 32 bytes (down) on distinct banks.
 //
+// 16-bit types with an activation, backward: act'(s) dy has 32 bits and enters as a pair of numbers of the type, P = scale (first + low
+// second), the whole sum over the second before the one over the first, in the same registers.  bf16: the second is what rounding left
+// (2^-16 of the value remains).  fp16: values are divided by a bound of act', so that dy's range fits, and what rounding left is multiplied by
+// 2^11: 2^-22 of the value remains, or 2^-36 among the smallest.  The products cost twice the time (8192 x 4096 x 4096 bf16, gelu: 446 -> 826 us); with one
+// number the results had 1.4 times the error of their own rounding, and fp16 lost gradients of 1e-6 and those beyond 65504.  A second number of 0 makes a NaN of an infinity: tiles with a NaN
+// are computed again in fp32, as below.
+//
 // fp32 (k_split_*): x = x0 + x1 + x2 with bf16 parts cut off after 8 bits each (exact), and x y = x0 y0 + x0 y1 + x1 y0 + x1 y1 + x0 y2 +
 // x2 y0 up to 2^-23 |x y|: six products at 16 times the rate of the fp32 matrix instructions.  The running sum of the bf16 matrix
 // instructions drifts downwards, by little but always the same way, and a column sum over such results would add that up; so every 32 of
@@ -242,6 +249,31 @@ __device__ __forceinline__ void finish(const BigProduct& G, const LinArgs& A, co
     }
 }
 
+// A tile with a NaN in it is computed again in fp32 from the tensors, 64 x 64 at a time by every 256 threads.  -> whether it was.
+template <typename T, int BTP, int BTQ, int THREADS, int MODE, int FP, int FQ>
+__device__ __forceinline__ bool again_if_nan(const BigProduct& G, const LinArgs& A, const Place& at0, const f32x4 (&acc)[FP][FQ], char* smem) {
+    int nan = 0;
+#pragma unroll
+    for (int i = 0; i < FP; ++i)
+#pragma unroll
+        for (int j = 0; j < FQ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) nan |= acc[i][j][e] != acc[i][j][e];
+    if (!__syncthreads_or(nan)) return false;
+    constexpr int GROUPS = THREADS / 256, SUBS = (BTP / 64) * (BTQ / 64);
+    static_assert(SUBS % GROUPS == 0, "the groups meet the same barriers");
+    const LinSplit S = {0, 0, G.splits, G.len};
+    LinArgs B = A;
+    B.db = nullptr;                         // (its sums are fp32 already)
+    const int group = threadIdx.x / 256;
+    wait_loads<0>();
+    __syncthreads();
+    for (int u = group; u < SUBS; u += GROUPS)
+        tile_product<T, float, MODE>(threadIdx.x % 256, B, S, at0.split, at0.p0 + u / (BTQ / 64) * 64, at0.q0 + u % (BTQ / 64) * 64, G.part, nullptr,
+                                     smem + group * tile_lds<float>());
+    return true;
+}
+
 // 16-bit types.  BT x BT tiles, WP x WQ waves, 64 of the summed index a step, BUFS buffers.
 template <typename T, int BT, int WP, int WQ, int BUFS, bool PA, bool QA, int EPI>
 __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, int block, char* smem) {
@@ -328,7 +360,24 @@ __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, 
     };
 
     const bool touch = G.splits == 1 && A.res;
-    if (steps > 0) {
+    auto scaled = [&](float by) {
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] *= by;
+    };
+    const bool pair = EPI == EPI_STORE && G.pair;
+    if (pair) sp.corner += G.P.plane * 2;           // the second numbers first
+#pragma unroll 1
+    for (int pass = pair ? 2 : 1; pass > 0 && steps > 0; --pass) {
+        if (pair && pass == 1) {
+            wait_loads<0>();
+            block_barrier();                        // all of the last step has been read
+            sp.corner -= G.P.plane * 2;
+            scaled(G.low);
+        }
         for (int s = 0; s < BUFS && s < steps; ++s) load(s);
         if (steps >= BUFS) wait_loads<(BUFS - 1) * LOADS>();
         else wait_loads<0>();
@@ -353,6 +402,10 @@ __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, 
         read(p1, q1, steps - 1, 1);
         multiply(p0, q0);
         multiply(p1, q1);
+    }
+    if (pair) {
+        scaled(G.scale);
+        if (again_if_nan<T, BT, BT, THREADS, PA ? MODE_DX : MODE_DW>(G, A, at0, acc, smem)) return;
     }
     finish<T, BT, BT, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
 }
@@ -492,28 +545,7 @@ __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A
         add(1, sign);
     }
 
-    int nan = 0;                                // is there a NaN in what will be stored?
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) nan |= acc[i][j][e] != acc[i][j][e];
-    nan = __syncthreads_or(nan);
-    if (nan) {                                  // 64 x 64 at a time by every 256 threads
-        constexpr int GROUPS = THREADS / 256, SUBS = (BTP / 64) * (BTQ / 64), MODE = EPI == EPI_FWD ? MODE_FWD : PA ? MODE_DX : MODE_DW;
-        static_assert(SUBS % GROUPS == 0, "the groups meet the same barriers");
-        const LinSplit S = {0, 0, G.splits, G.len};
-        LinArgs B = A;
-        B.db = nullptr;                         // (its sums are fp32 already)
-        const int group = threadIdx.x / 256;
-        wait_loads<0>();
-        __syncthreads();
-        for (int u = group; u < SUBS; u += GROUPS)
-            tile_product<float, float, MODE>(threadIdx.x % 256, B, S, at0.split, at0.p0 + u / (BTQ / 64) * 64, at0.q0 + u % (BTQ / 64) * 64, G.part, nullptr,
-                                      smem + group * tile_lds<float>());
-        return;
-    }
+    if (again_if_nan<float, BTP, BTQ, THREADS, EPI == EPI_FWD ? MODE_FWD : PA ? MODE_DX : MODE_DW>(G, A, at0, acc, smem)) return;
     finish<float, BTP, BTQ, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
 }
 

@@ -9,6 +9,8 @@ struct PackArgs {
     const float* pre;           // or null: (rows, cols) saved pre-activations; the values become act'(pre) src
     void* out;                  // or null: (rows, ldo) of the same type, or for fp32 three bf16 matrices `plane` elements apart, each in
                                 // columns of 32 values and `rows` rows (linear_big.h)
+    bool pair;                  // 16-bit types: two matrices `plane` elements apart, values times `scale` rounded, and what that rounding left times `up`
+    float scale, up;
     float* colsum;              // or null: (row blocks, cols) sums over the rows
     int64_t rows, ld, ldo, plane;
     int cols;

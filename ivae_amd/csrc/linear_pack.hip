@@ -1,7 +1,7 @@
 // What a large product needs done to a matrix before it can be loaded 16 bytes at a time: rows brought to 16-byte boundaries,
-// fp32 cut into three bf16 parts, and in the backward pass the gradient of the pre-activation, ds = act'(s) dy, with its column
-// sums (db) taken on the way.  One read and one write of the matrix; a thread takes 8 neighbouring values of every row that its
-// group walks.
+// fp32 cut into three bf16 parts, and in the backward pass the gradient of the pre-activation, ds = act'(s) dy, for 16-bit types as
+// two numbers of the type, with its column sums (db) taken on the way.  One read and one write of the matrix; a thread takes 8
+// neighbouring values of every row that its group walks.
 #include "kernels.h"
 #include "linear_pack.h"
 
@@ -17,6 +17,15 @@ __device__ __forceinline__ void cut(float x, bf16_t (&o)[3]) {
     o[0] = __builtin_bit_cast(bf16_t, (uint16_t)(h0 >> 16));
     o[1] = __builtin_bit_cast(bf16_t, (uint16_t)(u1 >> 16));
     o[2] = __builtin_bit_cast(bf16_t, (uint16_t)(__builtin_bit_cast(uint32_t, r2) >> 16));
+}
+
+// scale v = hi + lo / up, both of type T.  A finite value stays finite; infinities and NaN are whole in hi.
+template <typename T> struct Largest { static constexpr float v = 65504.f; };
+template <> struct Largest<bf16_t> { static constexpr float v = 3.3895313892515355e38f; };
+template <typename T> __device__ __forceinline__ void halve(float v, float up, float& hi, float& lo) {
+    hi = to_f(from_f<T>(v));
+    if (fabsf(hi) == __builtin_inff() && fabsf(v) < __builtin_inff()) hi = copysignf(Largest<T>::v, v);
+    lo = fabsf(hi) < __builtin_inff() ? (v - hi) * up : 0.f;
 }
 
 struct PackJobs { PackArgs job[3]; };
@@ -58,7 +67,14 @@ __global__ __launch_bounds__(256) void k_pack(PackJobs J) {
         for (int j = 0; j < 8; ++j) sum[j] += v[j];
         if (!A.out) continue;
         if constexpr (sizeof(T) == 2) {
-            store_wide<T>((T*)A.out + r * A.ldo + col, v);
+            T* to = (T*)A.out + r * A.ldo + col;
+            if (A.pair) {
+                float lo[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) halve<T>(v[j] * A.scale, A.up, v[j], lo[j]);
+                store_wide<T>(to + A.plane, lo);
+            }
+            store_wide<T>(to, v);
         } else {
             const int64_t at = (col / 32 * A.rows + r) * 32 + col % 32;
             if (A.flip != FLIP_NONE && ((A.flip == FLIP_ROWS ? (int)(r >> 5) : col >> 5) & 1))

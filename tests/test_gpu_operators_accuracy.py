@@ -8,8 +8,8 @@ from tests import operator_ref as R
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
-# (rows, in, out) that the 64 x 64 kernels take
-SIZES = [(96, 120, 104), (300, 33, 77)]
+# (rows, in, out) that the 64 x 64 kernels take, and such that the large kernels' backward passes take
+SIZES = [(96, 120, 104), (300, 33, 77), (1024, 768, 520), (1003, 777, 531)]
 GRADS = ("dx", "dw", "db")
 
 
