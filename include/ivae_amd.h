@@ -249,7 +249,7 @@ int ivae_corr_batched(const float* x, const float* y, int64_t n_blocks, int64_t 
  * saved: NULL, or (rows, out_features) values that the backward pass of an activation other than IVAE_ACT_NONE needs: the
  * pre-activation, in fp32 for every type.
  * ivae_linear_backward: dy (rows, out_features) -> dx (rows, in_features), dw (like w), db (out_features); any of them may be
- * NULL.  The gradient of the residual is dy itself.  act'(s) dy keeps 16 bits or more, and any finite value, on its way into the products.
+ * NULL, and then so may w without dx, and x without dw.  The gradient of the residual is dy itself.  act'(s) dy keeps 16 bits or more, and any finite value, on its way into the products.
  * Limits: in_features, out_features <= 2^24, rows <= 2^40: IVAE_E_TOOLARGE. */
 typedef struct IvaeLinear {
     int64_t rows;

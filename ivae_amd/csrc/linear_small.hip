@@ -138,10 +138,11 @@ static BwdPlan plan_bwd(const LinArgs& A) {
     if (!A.dx) p.X.tp = 0;
     if (!A.dw) p.W.tq = A.db ? 1 : 0;                           // db alone: the first column of tiles sums it
     const int64_t nx = A.dx && p.X.splits > 1 ? p.X.splits * A.M * A.K : 0;
-    const int64_t nw = p.W.tq && p.W.splits > 1 ? (int64_t)p.W.splits * A.N * A.K : 0;
+    const bool split_w = p.W.tq && p.W.splits > 1;
+    const int64_t nw = A.dw && split_w ? (int64_t)p.W.splits * A.N * A.K : 0;
     p.off_w = nx;
     p.off_b = nx + nw;
-    p.floats = nx + nw + (nw ? (int64_t)p.W.splits * A.N : 0);
+    p.floats = nx + nw + (split_w ? (int64_t)p.W.splits * A.N : 0);
     return p;
 }
 size_t linear_small_ws(const LinArgs& A, bool backward) {

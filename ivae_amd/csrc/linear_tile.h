@@ -150,6 +150,7 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
     const T* w = (const T*)A.w;
     const T* dy = (const T*)A.dy;
 
+    const bool product = MODE != MODE_DW || A.dw;   // (db alone: the column sums of ds; x may be null)
     float vp[2][8], vq[2][8], sum[8] = {};
     auto fetch = [&](int64_t r0) {
         if constexpr (MODE == MODE_FWD) {
@@ -168,12 +169,16 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum[j] += vp[0][j] + vp[1][j];
             if (MODE == MODE_DX) fetch_tile<T, false>(t, w, A.K, q0, Q, r0, rb, vq);
-            else fetch_tile<T, false>(t, x, A.ldx, q0, Q, r0, rb, vq);
+            else if (product) fetch_tile<T, false>(t, x, A.ldx, q0, Q, r0, rb, vq);
         }
     };
     f32x4 acc[2][2] = {};
     if (ra < rb) fetch(ra);
     for (int64_t r = ra; r < rb; r += TR) {
+        if (!product) {
+            if (r + TR < rb) fetch(r + TR);
+            continue;
+        }
         __syncthreads();
         put_tile<C, MODE != MODE_DW>(t, lp, vp);
         put_tile<C, MODE == MODE_FWD>(t, lq, vq);
@@ -213,10 +218,10 @@ __device__ __forceinline__ void tile_product(int t, const LinArgs& A, const LinS
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = from[e] + (fwd && A.b ? bias.at(e) : 0.f);
         if (fwd) forward_store8<T>(A, at, m, v, A.res ? &res[h] : nullptr);
-        else if (m) {
+        else if (m && product) {
             if (S.splits > 1) store8(part + split * P * Q + at, m, v);
             else if (MODE == MODE_DX) store8((T*)A.dx + at, m, v);
-            else if (A.dw) store8((T*)A.dw + at, m, v);
+            else store8((T*)A.dw + at, m, v);
         }
     }
     if (MODE == MODE_DW && A.db && q0 == 0) {       // thread t holds the sums of 8 columns over every 32nd row: 32 threads hold each column

@@ -149,3 +149,25 @@ def test_infinities_in_gradients_with_an_activation(dt, m, k, n):
     assert torch.equal(dx[4].cpu().double(), torch.sign(w[6].double()) * float("inf"))
     assert torch.equal(dw[6].cpu().double(), torch.sign(x[4].double()) * float("inf")) and float(db[6]) == float("inf")
     assert torch.isfinite(dx[:4]).all() and torch.isfinite(dx[5:]).all() and torch.isfinite(dw[:6]).all() and torch.isfinite(dw[7:]).all()
+
+
+@pytest.mark.parametrize("m,k,n", SIZES + [(64, 50, 50), (6000, 17, 19)])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_gradients_without_the_operands_that_they_do_not_need(dt, act, m, k, n):
+    """The bias gradient needs neither x nor w, dx no x, dw no w: the C entry takes NULL for them, and the gradients are the same."""
+    from ivae_amd import _lib
+    g = torch.Generator().manual_seed(8)
+    X, W, D = (t.to(dev()) for t in (normal(g, m, k, dtype=dt), normal(g, n, k, scale=k ** -0.5, dtype=dt), normal(g, m, n, dtype=dt)))
+    _, saved = ops.linear(X, W, None, act, save=True)
+    want = ops.linear_backward(D, X, W, saved, act)
+    lin, nb = ops._linear_plan(m, k, n, ops.DTYPE_IDS[dt], _lib.LINEAR_ACT_IDS[act], R.SLOPE, k, 0, n, 1)
+    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=dev())
+    for need in ((False, False, True), (True, False, True), (False, True, True), (True, False, False), (False, True, False)):
+        out = [torch.full_like(t, 7.0) if w else None for t, w in zip(want, need)]
+        rc = _lib.lib().ivae_linear_backward(lin, D.data_ptr(), X.data_ptr() if need[1] else None, W.data_ptr() if need[0] else None,
+                                             saved.data_ptr() if saved is not None else None, *[t.data_ptr() if t is not None else None for t in out],
+                                             ws.data_ptr(), nb, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        for name, a, b in zip(GRADS, want, out):
+            assert b is None or torch.equal(a, b), (name, need)
