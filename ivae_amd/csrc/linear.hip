@@ -69,6 +69,11 @@ struct Bytes {                                          // a workspace, handed o
     }
 };
 
+// (a job's blocks, with column sums or without)
+static int max_ranges(int64_t rows, int64_t ldo) {
+    const int a = pack_blocks(rows, ldo, false, IVAE_F32), b = pack_blocks(rows, ldo, true, IVAE_F32);
+    return a > b ? a : b;
+}
 // A matrix as an operand: in place where its rows are 16-byte groups already, packed otherwise (fp32 always)
 struct Packed { BigOperand O; PackArgs P; bool needed; };
 static Packed pack_of(const void* src, int64_t rows, int cols, int64_t ld, int dtype, Bytes& ws, bool pair = false) {
@@ -83,19 +88,24 @@ static Packed pack_of(const void* src, int64_t rows, int cols, int64_t ld, int d
     void* out = ws.take<uint16_t>(plane * (dtype == IVAE_F32 ? 3 : pair ? 2 : 1));
     r.P.src = src; r.P.out = out; r.P.rows = rows; r.P.cols = cols; r.P.ld = ld; r.P.ldo = ldo; r.P.plane = plane; r.P.pair = pair;
     r.O = {out, dtype == IVAE_F32 ? rows : ldo, 0, 0, plane, false};
+    if (dtype == IVAE_F32) r.P.range = ws.take<uint2>(max_ranges(rows, ldo));
     return r;
 }
 // rows are what the product has as rows or columns, the summed index runs along them / down the rows
 static BigOperand along(const Packed& p, int64_t rows) {
     BigOperand o = p.O;
     o.along = true; o.extent = rows; o.limit = p.P.ldo;
+    o.range = p.P.range;
     return o;
 }
 static BigOperand down(const Packed& p, int64_t rows) {
     BigOperand o = p.O;
     o.along = false; o.extent = p.P.ldo; o.limit = rows;
+    o.range = p.P.range;
     return o;
 }
+
+static int ranges_of(const Packed& p, int dtype) { return dtype == IVAE_F32 ? pack_blocks(p.P.rows, p.P.ldo, p.P.colsum != nullptr, dtype) : 0; }
 
 struct BigForward { Packed x, w; BigProduct B; size_t bytes; };
 static BigForward plan_big_forward(const LinArgs& A, int dtype, void* ws) {
@@ -115,8 +125,9 @@ static BigForward plan_big_forward(const LinArgs& A, int dtype, void* ws) {
     return f;
 }
 static hipError_t big_forward(LinArgs A, int dtype, void* ws, hipStream_t st) {
-    const BigForward f = plan_big_forward(A, dtype, ws);
+    BigForward f = plan_big_forward(A, dtype, ws);
     hipError_t e = hipSuccess;
+    f.B.P.ranges = ranges_of(f.x, dtype), f.B.Q.ranges = ranges_of(f.w, dtype);
     const PackArgs* packs[2] = {f.x.needed ? &f.x.P : nullptr, f.w.needed ? &f.w.P : nullptr};
     e = launch_packs(packs, 2, dtype, st);
     if (e == hipSuccess) e = big_forward_launch(f.B, A, dtype, st);
@@ -183,6 +194,8 @@ static hipError_t big_backward(const LinArgs& A, int dtype, void* ws, hipStream_
     BigBackward f = plan_big_backward(A, dtype, ws);
     hipError_t e = hipSuccess;
     f.ds.P.colsum = A.db ? f.colsum : nullptr;
+    f.X.P.ranges = f.W.P.ranges = ranges_of(f.ds, dtype);
+    f.X.Q.ranges = ranges_of(f.w, dtype), f.W.Q.ranges = ranges_of(f.x, dtype);
     const PackArgs* packs[3] = {f.ds.needed || A.db ? &f.ds.P : nullptr, A.dx && f.w.needed ? &f.w.P : nullptr, A.dw && f.x.needed ? &f.x.P : nullptr};
     e = launch_packs(packs, 3, dtype, st);
     if (e == hipSuccess) e = big_backward_launch(f.X, f.W, A, dtype, st);

@@ -7,12 +7,14 @@
 // Rows start at multiples of 16 bytes and hold whole 16-byte groups.  Split fp32 is stored in columns of 32 values, ld rows each
 // (value (r, c) at (c / 32 * ld + r) * 32 + c % 32): what a step loads of a tile lies in one piece, or (down) in pieces of 2 KB, where
 // rows of 64 bytes out of a row-major matrix would use half of each cache line.  `limit` is the end of the stored values along R (a multiple
-// of 8 where `along`; values between R and limit are 0).  Split fp32: of every second 32 along R, Q has its sign turned.  `plane`: elements between the three parts of split fp32 values,
-// or the two numbers of a pair.
+// of 8 where `along`; values between R and limit are 0).  Split fp32: of every second 32 along R, Q has its sign turned.
+// `plane`: elements between the three parts of split fp32 values, or the two numbers of a pair.  `range`: PackArgs' of split fp32.
 struct BigOperand {
     const void* base;
     int64_t ld, extent, limit, plane;
     bool along;
+    const uint2* range;
+    int ranges;
 };
 
 enum { EPI_FWD, EPI_STORE };    // what follows the sums: forward_store's, or a store of the result type

@@ -14,12 +14,12 @@
 // number the results had 1.4 times the error of their own rounding, and fp16 lost gradients of 1e-6 and those beyond 65504.  A second number of 0 makes a NaN of an infinity: tiles with a NaN
 // are computed again in fp32, as below.
 //
-// fp32 (k_split_*): x = x0 + x1 + x2 with bf16 parts cut off after 8 bits each (exact), and x y = x0 y0 + x0 y1 + x1 y0 + x1 y1 + x0 y2 +
+// fp32 (k_split_*): x = x0 + x1 + x2 with bf16 parts cut off after 8 bits each (exact from 2^-110 on), and x y = x0 y0 + x0 y1 + x1 y0 + x1 y1 + x0 y2 +
 // x2 y0 up to 2^-23 |x y|: six products at 16 times the rate of the fp32 matrix instructions.  The running sum of the bf16 matrix
 // instructions drifts downwards, by little but always the same way, and a column sum over such results would add that up; so every 32 of
 // the summed index start from zero, smallest products first, and are added to the sum by fp32 additions that round to nearest.
 // An infinity times a part that is 0 makes a NaN that fp32 would not: a tile with a NaN in it is computed again in fp32, from the
-// tensors themselves.
+// tensors themselves.  So is one with a result of which the bits that smaller values lost can be more than 2^-25.
 #include <type_traits>
 
 #include "kernels.h"
@@ -249,9 +249,32 @@ __device__ __forceinline__ void finish(const BigProduct& G, const LinArgs& A, co
     }
 }
 
-// A tile with a NaN in it is computed again in fp32 from the tensors, 64 x 64 at a time by every 256 threads.  -> whether it was.
+// Split fp32: cutting drops bits under 2^-133 of values below 2^-110, so a sum over R terms is off by at most R 2^-133 (the largest |P| and
+// the largest |Q|).  Has a block that cut an operand seen such a value? (four blocks' answers under way at a time)
+template <int THREADS> __device__ __forceinline__ uint32_t lost_bits(const BigOperand& O) {
+    uint32_t lost = 0;
+    for (int i = threadIdx.x; i < O.ranges; i += 4 * THREADS) {
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = O.range[min(i + j * THREADS, O.ranges - 1)].x;
+        lost |= v[0] | v[1] | v[2] | v[3];
+    }
+    return lost;
+}
+__device__ __forceinline__ float largest(const BigOperand& O) {             // by every wave for itself
+    uint32_t most = 0;
+    for (int i = threadIdx.x % 64; i < O.ranges; i += 64) most = max(most, O.range[i].y);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
+    return __builtin_bit_cast(float, most);
+}
+// A tile with a NaN in it, or with a result of which lost bits can be more than 2^-25, is computed again in fp32 from the tensors, 64 x 64 at a
+// time by every 256 threads.  -> whether it was.
 template <typename T, int BTP, int BTQ, int THREADS, int MODE, int FP, int FQ>
-__device__ __forceinline__ bool again_if_nan(const BigProduct& G, const LinArgs& A, const Place& at0, const f32x4 (&acc)[FP][FQ], char* smem) {
+__device__ __forceinline__ bool again_if_needed(const BigProduct& G, const LinArgs& A, const Place& at0, const f32x4 (&acc)[FP][FQ], char* smem) {
+    constexpr bool CUT = sizeof(T) == 4;
+    uint32_t lost = 0;
+    if (CUT) lost = lost_bits<THREADS>(G.P) | lost_bits<THREADS>(G.Q);
     int nan = 0;
 #pragma unroll
     for (int i = 0; i < FP; ++i)
@@ -259,7 +282,17 @@ __device__ __forceinline__ bool again_if_nan(const BigProduct& G, const LinArgs&
         for (int j = 0; j < FQ; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) nan |= acc[i][j][e] != acc[i][j][e];
-    if (!__syncthreads_or(nan)) return false;
+    if (!__syncthreads_or(nan | (int)lost)) return false;
+    if (CUT) {
+        const float scale = 0x1p-108f * (float)G.len, least = scale * largest(G.P) + scale * largest(G.Q);
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) nan |= fabsf(acc[i][j][e]) < least;
+        if (!__syncthreads_or(nan)) return false;
+    }
     constexpr int GROUPS = THREADS / 256, SUBS = (BTP / 64) * (BTQ / 64);
     static_assert(SUBS % GROUPS == 0, "the groups meet the same barriers");
     const LinSplit S = {0, 0, G.splits, G.len};
@@ -405,7 +438,7 @@ __device__ __forceinline__ void big_tile(const BigProduct& G, const LinArgs& A, 
     }
     if (pair) {
         scaled(G.scale);
-        if (again_if_nan<T, BT, BT, THREADS, PA ? MODE_DX : MODE_DW>(G, A, at0, acc, smem)) return;
+        if (again_if_needed<T, BT, BT, THREADS, PA ? MODE_DX : MODE_DW>(G, A, at0, acc, smem)) return;
     }
     finish<T, BT, BT, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
 }
@@ -545,7 +578,7 @@ __device__ __forceinline__ void split_tile(const BigProduct& G, const LinArgs& A
         add(1, sign);
     }
 
-    if (again_if_nan<float, BTP, BTQ, THREADS, EPI == EPI_FWD ? MODE_FWD : PA ? MODE_DX : MODE_DW>(G, A, at0, acc, smem)) return;
+    if (again_if_needed<float, BTP, BTQ, THREADS, EPI == EPI_FWD ? MODE_FWD : PA ? MODE_DX : MODE_DW>(G, A, at0, acc, smem)) return;
     finish<float, BTP, BTQ, WP, WQ, EPI>(G, A, at0, acc, (float*)smem);
 }
 

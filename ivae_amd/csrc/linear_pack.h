@@ -11,6 +11,7 @@ struct PackArgs {
                                 // columns of 32 values and `rows` rows (linear_big.h)
     bool pair;                  // 16-bit types: two matrices `plane` elements apart, values times `scale` rounded, and what that rounding left times `up`
     float scale, up;
+    uint2* range;               // fp32: of each block, whether the parts of a value of it lost bits, and the largest finite magnitude (its bits)
     float* colsum;              // or null: (row blocks, cols) sums over the rows
     int64_t rows, ld, ldo, plane;
     int cols;
@@ -20,4 +21,5 @@ struct PackArgs {
     int group, blocks_x, blocks;    // set by the launcher
 };
 int pack_row_blocks(int64_t rows, int64_t width, bool colsum, int dtype);  // of a job with ldo = width: rows of its colsum
+int pack_blocks(int64_t rows, int64_t width, bool colsum, int dtype);      // ... and all of its blocks
 hipError_t launch_packs(const PackArgs* const* P, int n, int dtype, hipStream_t st);    // up to three in one launch; null: none

@@ -6,8 +6,8 @@
 #include "linear_pack.h"
 
 // x = x0 + x1 + x2, 8 bits each, cut off rather than rounded: every part has x's sign and the first never overflows.  Infinities and
-// NaN are whole in the first part.
-__device__ __forceinline__ void cut(float x, bf16_t (&o)[3]) {
+// NaN are whole in the first part.  -> what is lost, as bits that are not 0: below 2^-110 x has bits under 2^-133, the smallest that bf16 holds.
+__device__ __forceinline__ uint32_t cut(float x, bf16_t (&o)[3]) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x);
     const bool finite = (u & 0x7f800000u) != 0x7f800000u;
     const uint32_t h0 = finite || (u & 0x007fffffu) == 0 ? u & 0xffff0000u : u | 0x00400000u;
@@ -17,6 +17,7 @@ __device__ __forceinline__ void cut(float x, bf16_t (&o)[3]) {
     o[0] = __builtin_bit_cast(bf16_t, (uint16_t)(h0 >> 16));
     o[1] = __builtin_bit_cast(bf16_t, (uint16_t)(u1 >> 16));
     o[2] = __builtin_bit_cast(bf16_t, (uint16_t)(__builtin_bit_cast(uint32_t, r2) >> 16));
+    return __builtin_bit_cast(uint32_t, r2) << 16;
 }
 
 // scale v = hi + lo / up, both of type T.  A finite value stays finite; infinities and NaN are whole in hi.
@@ -38,6 +39,7 @@ __global__ __launch_bounds__(256) void k_pack(PackJobs J) {
     const int group = A.group;                          // threads that share a row of 8 * group values
     const int col = (bx * group + threadIdx.x % group) * 8, sub = threadIdx.x / group, subs = 256 / group;
     float sum[8] = {};
+    uint32_t lost = 0, most = 0;
     const int left = A.cols - col;                      // <= 0: beyond the last value (the padding is zeros)
     for (int64_t r = (int64_t)by * subs + sub; r < A.rows && col < A.ldo; r += (int64_t)rows_of_blocks * subs) {
         float v[8], s[8];
@@ -84,13 +86,23 @@ __global__ __launch_bounds__(256) void k_pack(PackJobs J) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 bf16_t o[3];
-                cut(v[j], o);
+                lost |= cut(v[j], o);
+                const uint32_t size = __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu;
+                if (size < 0x7f800000u && size > most) most = size;
 #pragma unroll
                 for (int k = 0; k < 3; ++k) part[k].e[j] = o[k];
             }
 #pragma unroll
             for (int k = 0; k < 3; ++k) *(V*)((bf16_t*)A.out + k * A.plane + at) = part[k];
         }
+    }
+    if (sizeof(T) == 4 && A.out) {
+        __shared__ uint32_t waves[4];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
+        if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = most;
+        const int any = __syncthreads_or(lost != 0);
+        if (threadIdx.x == 0) A.range[block] = uint2{any ? 1u : 0u, max(max(waves[0], waves[1]), max(waves[2], waves[3]))};
     }
     if (!A.colsum) return;
     __shared__ float fold[256][9];
@@ -122,6 +134,10 @@ int pack_row_blocks(int64_t rows, int64_t width, bool colsum, int dtype) {
     if (y > most) y = most;
     return (int)(y < 1 ? 1 : y);
 }
+int pack_blocks(int64_t rows, int64_t width, bool colsum, int dtype) {
+    const int g = group_of(width, dtype);
+    return (int)((width + g * 8 - 1) / (g * 8)) * pack_row_blocks(rows, width, colsum, dtype);
+}
 hipError_t launch_packs(const PackArgs* const* P, int n, int dtype, hipStream_t st) {
     PackJobs J = {};
     int jobs = 0, blocks = 0;
@@ -130,7 +146,7 @@ hipError_t launch_packs(const PackArgs* const* P, int n, int dtype, hipStream_t 
         PackArgs& A = J.job[jobs++] = *P[i];
         A.group = group_of(A.ldo, dtype);
         A.blocks_x = (int)((A.ldo + A.group * 8 - 1) / (A.group * 8));
-        A.blocks = A.blocks_x * pack_row_blocks(A.rows, A.ldo, A.colsum != nullptr, dtype);
+        A.blocks = pack_blocks(A.rows, A.ldo, A.colsum != nullptr, dtype);
         blocks += A.blocks;
     }
     if (blocks == 0) return hipSuccess;

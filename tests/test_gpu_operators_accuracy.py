@@ -171,3 +171,39 @@ def test_gradients_without_the_operands_that_they_do_not_need(dt, act, m, k, n):
         assert rc == 0
         for name, a, b in zip(GRADS, want, out):
             assert b is None or torch.equal(a, b), (name, need)
+
+
+# products that the 64 x 64 kernel takes, and such that the split kernels take (forward pass: 5e9 operations and more, odd sizes 2e9)
+@pytest.mark.parametrize("m,k,n", [(96, 120, 104), (1024, 2048, 1300), (1100, 1501, 1003)])
+@pytest.mark.parametrize("ex,ew", [(0, 0), (-60, -50), (-112, 100), (-118, 100), (-121, 100), (100, -125), (-130, 110), (-118, 0), (0, -122)])
+def test_fp32_keeps_its_digits_down_to_the_smallest_numbers(m, k, n, ex, ew):
+    """x 2^ex and w 2^ew of unit values, the gradient at x's scale: a sum of n products of 24-bit numbers is off by a walk of sqrt(n) half steps
+    or less.  Numbers below 2^-126 have fewer bits themselves; the formula takes them as they are.  db and results below 2^-126 are left out."""
+    g = torch.Generator().manual_seed(m)
+    x, w, dy = (torch.ldexp(normal(g, *s), torch.tensor(e)) for s, e in (((m, k), ex), ((n, k), ew), ((m, n), ex)))
+    got = {"y": ops.linear(x.to(dev()), w.to(dev()))}
+    got["dx"], got["dw"], _ = ops.linear_backward(dy.to(dev()), x.to(dev()), w.to(dev()))
+    up = lambda t, e: torch.ldexp(t.double(), torch.tensor(-e))  # noqa: E731
+    X, W, D = up(x, ex), up(w, ew), up(dy, ex)
+    for name, want, e, terms in (("y", X @ W.t(), ex + ew, k), ("dx", D @ W, ex + ew, n), ("dw", D.t() @ X, 2 * ex, m)):
+        if -120 < e < 110:
+            rms = float((up(got[name].cpu(), e) - want).square().mean().sqrt() / want.square().mean().sqrt())
+            assert rms <= R.U32 * terms ** 0.5, (name, rms)
+
+
+def test_fp32_tiny_rows_among_ordinary_ones():
+    """Rows whose values have bits that a bf16 number cannot hold, among rows of unit scale and rows of zeros: each is right by itself."""
+    g = torch.Generator().manual_seed(9)
+    m, k, n = 1100, 1501, 1003
+    x, w = normal(g, m, k), torch.ldexp(normal(g, n, k), torch.tensor(20))
+    x[300:310] = torch.ldexp(x[300:310], torch.tensor(-120))
+    x[700:800] = 0
+    w[5] = torch.ldexp(w[5], torch.tensor(-140))
+    y = ops.linear(x.to(dev()), w.to(dev())).cpu().double()
+    want, mag = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+    assert bool(((y - want).abs() <= (k + 16) * R.U32 * mag + 2.0 ** -149 * k).all())
+    for rows, cols in ((slice(300, 310), slice(6, n)), (slice(0, 300), slice(5, 6)), (slice(0, 300), slice(6, n))):
+        a, b = y[rows, cols], want[rows, cols]
+        a, b = a / b.abs().max(), b / b.abs().max()
+        assert float((a - b).square().mean().sqrt() / b.square().mean().sqrt()) <= R.U32 * k ** 0.5, (rows, cols)
+    assert float(y[700:800].abs().max()) == 0
