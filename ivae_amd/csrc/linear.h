@@ -41,7 +41,7 @@ __device__ __forceinline__ float lin_act(int act, float slope, float s) {
         case IVAE_ACT_LRELU: return s > 0.f ? s : slope * s;
         case IVAE_ACT_XTANH: return (fast ? fast_tanh(s) : tanhf(s)) + slope * s;
         case IVAE_ACT_SIGMOID: return fast ? fast_sigmoid(s) : 1.f / (1.f + expf(-s));
-        case IVAE_ACT_GELU: return 0.5f * s * (fast ? fast_cdf2(s) : 1.f + erff(s * 0.70710678118654752f));
+        case IVAE_ACT_GELU: return 0.5f * s * (fast ? fast_cdf2(s) : erfcf(s * -0.70710678118654752f));     // (1 + erf would cancel below 0)
         case IVAE_ACT_SILU: return fast ? s * fast_sigmoid(s) : s / (1.f + expf(-s));
         default: return s;
     }
@@ -54,7 +54,7 @@ __device__ __forceinline__ float lin_act_slope(int act, float slope, float s) {
         case IVAE_ACT_XTANH: { const float t = fast ? fast_tanh(s) : tanhf(s); return (1.f - t * t) + slope; }
         case IVAE_ACT_SIGMOID: { const float t = fast ? fast_sigmoid(s) : 1.f / (1.f + expf(-s)); return t * (1.f - t); }
         case IVAE_ACT_GELU:
-            return 0.5f * (fast ? fast_cdf2(s) : 1.f + erff(s * 0.70710678118654752f)) +
+            return 0.5f * (fast ? fast_cdf2(s) : erfcf(s * -0.70710678118654752f)) +
                    s * (fast ? fast_exp(-0.5f * s * s) : expf(-0.5f * s * s)) * 0.39894228040143268f;
         case IVAE_ACT_SILU: { const float t = fast ? fast_sigmoid(s) : 1.f / (1.f + expf(-s)); return t * (1.f + s * (1.f - t)); }
         default: return 1.f;

@@ -207,3 +207,40 @@ def test_fp32_tiny_rows_among_ordinary_ones():
         a, b = a / b.abs().max(), b / b.abs().max()
         assert float((a - b).square().mean().sqrt() / b.square().mean().sqrt()) <= R.U32 * k ** 0.5, (rows, cols)
     assert float(y[700:800].abs().max()) == 0
+
+
+def tails(dt, act, slope=0.0):
+    """act and act' where they are small next to 1, one value a row: -> ((y, its value, the sum of its terms' magnitudes), the same of act')."""
+    s = torch.linspace(-12.5, 12.5, 6001).to(dt)[:, None]
+    one = torch.ones(1, 1, dtype=dt)
+    y = ops.linear(s.to(dev()), one.to(dev()), None, act, slope).cpu().double()
+    got, _ = gradients(s, one, None, act, torch.ones_like(s), slope)
+    S = s.double()
+    sig, sig_ = torch.special.expit(S), torch.special.expit(-S)
+    if act == "gelu":
+        cdf, pdf = torch.special.erfc(-S / 2 ** 0.5) / 2, torch.exp(-S * S / 2) / (2 * torch.pi) ** 0.5
+        v, d, mag = S * cdf, cdf + S * pdf, cdf + S.abs() * pdf
+    elif act == "sigmoid":
+        v, d, mag = sig, sig * sig_, sig * sig_
+    elif act == "silu":
+        v, d, mag = S * sig, sig * (1 + S * sig_), sig * (1 + S.abs() * sig_)
+    else:
+        d = 4 * torch.exp(-2 * S.abs()) / (1 + torch.exp(-2 * S.abs())) ** 2
+        v, mag = torch.tanh(S), d
+    return S, (y, v, v.abs()), (got["dx"].cpu().double(), d, mag)
+
+
+def check_tails(dt, act, rel):
+    """rel(s): the relative error that the evaluation may have; the result's own rounding comes on top."""
+    S, *both = tails(dt, act)
+    for name, (got, want, mag) in zip(("y", "slope"), both):
+        bound = R.u(dt) * want.abs() + rel(S) * mag + R.tiny(dt) + 2.0 ** -126
+        err = (got - want).abs()
+        assert bool((err <= bound).all()), (name, float((err / bound).max()), float(S[(err / bound).argmax()]))
+
+
+# exp's argument is rounded, which moves the result by |argument| half steps for each of its roundings; 16 half steps for the rest
+@pytest.mark.parametrize("dt", [F32])
+def test_gelu_keeps_its_digits_in_the_tail(dt):
+    """exp(-s^2 / 2) and erfc(-s / sqrt 2), whose argument is rounded twice and counts twice: 3 s^2 half steps."""
+    check_tails(dt, "gelu", lambda s: (16 + 3 * s * s) * R.U32)
