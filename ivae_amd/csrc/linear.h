@@ -46,13 +46,18 @@ __device__ __forceinline__ float lin_act(int act, float slope, float s) {
         default: return s;
     }
 }
+// sigmoid'(s) = e / (1 + e)^2, e = exp(-s), for s >= 0 (it is even): sigmoid (1 - sigmoid) would lose the digits of what is left of 1
+template <bool FAST> __device__ __forceinline__ float logistic_slope(float s) {
+    const float e = FAST ? fast_exp(-s) : expf(-s), r = FAST ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);
+    return e * r * r;
+}
 template <typename T>
 __device__ __forceinline__ float lin_act_slope(int act, float slope, float s) {
     constexpr bool fast = sizeof(T) == 2;
     switch (act) {
         case IVAE_ACT_LRELU: return s > 0.f ? 1.f : slope;
-        case IVAE_ACT_XTANH: { const float t = fast ? fast_tanh(s) : tanhf(s); return (1.f - t * t) + slope; }
-        case IVAE_ACT_SIGMOID: { const float t = fast ? fast_sigmoid(s) : 1.f / (1.f + expf(-s)); return t * (1.f - t); }
+        case IVAE_ACT_XTANH: return 4.f * logistic_slope<fast>(2.f * fabsf(s)) + slope;          // 1 - tanh^2
+        case IVAE_ACT_SIGMOID: return logistic_slope<fast>(fabsf(s));
         case IVAE_ACT_GELU:
             return 0.5f * (fast ? fast_cdf2(s) : erfcf(s * -0.70710678118654752f)) +
                    s * (fast ? fast_exp(-0.5f * s * s) : expf(-0.5f * s * s)) * 0.39894228040143268f;

@@ -244,3 +244,10 @@ def check_tails(dt, act, rel):
 def test_gelu_keeps_its_digits_in_the_tail(dt):
     """exp(-s^2 / 2) and erfc(-s / sqrt 2), whose argument is rounded twice and counts twice: 3 s^2 half steps."""
     check_tails(dt, "gelu", lambda s: (16 + 3 * s * s) * R.U32)
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "xtanh", "silu"])
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_slopes_keep_their_digits_in_the_tails(dt, act):
+    """exp(-s) and exp(-2 |s|): 2 |s| half steps, twice (argument and constant)."""
+    check_tails(dt, act, lambda s: (16 + 4 * s.abs()) * R.U32 + (2.0 ** -18 if act == "xtanh" and dt != F32 else 0.0))
