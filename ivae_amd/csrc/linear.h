@@ -18,8 +18,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 
-// Activations of 16-bit results from the hardware's exp2 and reciprocal (1 unit in the last place of 32 bits each): their errors are
-// at most 2e-7 next to steps of 2^-11 and more, and an epilogue of 128 values a lane costs a third of what the exact forms do.
+// Activations of 16-bit results from the hardware's exp2 and reciprocal (1 unit in the last place of 32 bits each): relative errors of a
+// few 2^-24, and for each factor exp(-x) x 2^-23 more (2^-16 at gelu's smallest bf16 results), next to half steps of 2^-12 and 2^-9 relative to
+// the result; an epilogue of 128 values a lane costs a third of what the exact forms do.
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 __device__ __forceinline__ float fast_sigmoid(float s) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-s)); }
 __device__ __forceinline__ float fast_tanh(float s) {
@@ -28,10 +29,13 @@ __device__ __forceinline__ float fast_tanh(float s) {
     const float far = copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(1.f + fast_exp(2.f * a)), s);
     return a < 0.1f ? near : far;
 }
-// 1 + erf(x / sqrt 2) (twice the normal distribution): Abramowitz and Stegun 7.1.26, |error| <= 1.5e-7
+// 1 + erf(s / sqrt 2) (twice the normal distribution): erfc(a) exp(a^2) = t P(t), t = 1 / (1 + 0.42 a), P fitted to the least relative error
+// over 0 <= a <= 9.6, 1.8e-7, so that what is left of the tail below 0 keeps its digits; in 32 bits 5e-7 near 0, 8e-6 at the end, from exp
 __device__ __forceinline__ float fast_cdf2(float s) {
-    const float a = fabsf(s) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * a);
-    const float tail = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * fast_exp(-a * a);
+    const float a = fabsf(s) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.f + 0.42f * a);
+    const float p = 0.23682660f + t * (0.23955022f + t * (0.19494417f + t * (0.26803513f + t * (-0.12920924f + t * (0.43926111f + t * (-0.31944717f +
+                    t * 0.070038993f))))));
+    const float tail = t * p * fast_exp(-a * a);
     return s < 0.f ? tail : 2.f - tail;
 }
 template <typename T>
