@@ -128,6 +128,8 @@ class MLP(nn.Module):
     them the forward and backward passes run in the library's kernels (``ops.linear``, ``ops.layer_norm``, ``ops.dropout``) and need
     a ROCm device; fp32, bf16 and fp16 parameters, and the activations 'gelu' and 'silu' besides the others."""
 
+    operators = False           # of an MLP that was pickled before there were these options
+
     def __init__(self, input_dim, output_dim, hidden_dim, n_layers, activation='none', slope=.1, device='cpu', layer_norm=False,
                  residual=False, dropout=0.):
         super().__init__()
