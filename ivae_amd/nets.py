@@ -53,13 +53,14 @@ def _no_capture(*tensors):
         raise RuntimeError('autograd through MLP operators cannot be captured into a graph: capture ivae_amd.ops calls instead')
 
 
+# The operators go through these Functions without gradients as well: forward mode and tracing know nothing of what runs outside of one,
+# and would drop it in silence.  Inside a Function its caller's grad mode is not to be seen, so `grad` says whether to keep anything.
 class _LinearFn(torch.autograd.Function):
     """ops.linear with its gradients."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, activation, slope, residual):
-        save = any(ctx.needs_input_grad[:3])
-        if not save:
+    def forward(ctx, x, weight, bias, activation, slope, residual, grad):
+        if not (grad and any(ctx.needs_input_grad[:3])):
             return ops.linear(x, weight, bias, activation, slope, residual)
         _no_capture(x)
         y, pre = ops.linear(x, weight, bias, activation, slope, residual, save=True)
@@ -76,15 +77,15 @@ class _LinearFn(torch.autograd.Function):
         if any(need[:3]):
             x, weight, pre = ctx.saved_tensors
             dx, dw, db = ops.linear_backward(dy, x, weight, pre, *ctx.act, need=need[:3])
-        return dx, dw, db, None, None, dy if need[5] else None
+        return dx, dw, db, None, None, dy if need[5] else None, None
 
 
 class _LayerNormFn(torch.autograd.Function):
     """ops.layer_norm with its gradients."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        if not any(ctx.needs_input_grad[:3]):
+    def forward(ctx, x, weight, bias, eps, grad):
+        if not (grad and any(ctx.needs_input_grad[:3])):
             return ops.layer_norm(x, weight, bias, eps)
         _no_capture(x)
         y, stats = ops.layer_norm(x, weight, bias, eps, save=True)
@@ -96,15 +97,15 @@ class _LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         _no_capture(dy)
         x, weight, stats = ctx.saved_tensors
-        return (*ops.layer_norm_backward(dy, x, stats, weight, need=ctx.needs_input_grad[:3]), None)
+        return (*ops.layer_norm_backward(dy, x, stats, weight, need=ctx.needs_input_grad[:3]), None, None)
 
 
 class _DropoutFn(torch.autograd.Function):
     """ops.dropout with its gradients; the mask is drawn again in the backward pass."""
 
     @staticmethod
-    def forward(ctx, x, p, seed, offset, residual):
-        if any(ctx.needs_input_grad):
+    def forward(ctx, x, p, seed, offset, residual, grad):
+        if grad and any(ctx.needs_input_grad):
             _no_capture(x)
         ctx.draw = p, seed, offset
         return ops.dropout(x, p, seed, offset, residual)
@@ -114,7 +115,7 @@ class _DropoutFn(torch.autograd.Function):
     def backward(ctx, dy):
         _no_capture(dy)
         need = ctx.needs_input_grad
-        return ops.dropout_backward(dy, *ctx.draw) if need[0] else None, None, None, None, dy if need[4] else None
+        return ops.dropout_backward(dy, *ctx.draw) if need[0] else None, None, None, None, dy if need[4] else None, None
 
 
 class MLP(nn.Module):
@@ -184,25 +185,24 @@ class MLP(nn.Module):
         if drop:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('a captured MLP would draw the same dropout mask at every replay: call eval() first')
+            if torch.jit.is_tracing():
+                raise RuntimeError('a traced MLP would draw the same dropout mask at every call: call eval() first')
             seed = int(torch.randint(2 ** 63 - 1, ()))
-        # (inside a Function the grad mode of its caller is not to be seen: without one nothing needs to be saved)
         grad = torch.is_grad_enabled()
-        linear, layer_norm, drop_out = ((_LinearFn.apply, _LayerNormFn.apply, _DropoutFn.apply) if grad else
-                                        (ops.linear, ops.layer_norm, ops.dropout))
         h = x
         for c, fc in enumerate(self.fc):
             t = h
             if self.norm is not None and c:
                 n = self.norm[c - 1]
-                t = layer_norm(t, n.weight, n.bias, n.eps)
+                t = _LayerNormFn.apply(t, n.weight, n.bias, n.eps, grad)
             if c == self.n_layers - 1:
-                return linear(t, fc.weight, fc.bias, 'none', self.slope, None)
+                return _LinearFn.apply(t, fc.weight, fc.bias, 'none', self.slope, None, grad)
             add = h if self.residual and fc.in_features == fc.out_features else None
             if drop:
-                t = linear(t, fc.weight, fc.bias, self.activation[c], self.slope, None)
-                h = drop_out(t, drop, seed, c, add)
+                t = _LinearFn.apply(t, fc.weight, fc.bias, self.activation[c], self.slope, None, grad)
+                h = _DropoutFn.apply(t, drop, seed, c, add, grad)
             else:
-                h = linear(t, fc.weight, fc.bias, self.activation[c], self.slope, add)
+                h = _LinearFn.apply(t, fc.weight, fc.bias, self.activation[c], self.slope, add, grad)
         return h
 
     def forward(self, x):
