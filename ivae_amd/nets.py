@@ -118,6 +118,25 @@ class _DropoutFn(torch.autograd.Function):
         return ops.dropout_backward(dy, *ctx.draw) if need[0] else None, None, None, None, dy if need[4] else None, None
 
 
+class _OperatorLinear(nn.Linear):
+    """nn.Linear on ops.linear, with the activation and the residual that its caller passes fused into it."""
+
+    def forward(self, x, activation='none', slope=.1, residual=None):
+        return _LinearFn.apply(x, self.weight, self.bias, activation, slope, residual, torch.is_grad_enabled())
+
+
+class _OperatorNorm(nn.LayerNorm):
+    """nn.LayerNorm over the last dimension on ops.layer_norm."""
+
+    def forward(self, x):
+        return _LayerNormFn.apply(x, self.weight, self.bias, self.eps, torch.is_grad_enabled())
+
+
+def _fuses(fc):
+    """Whether what follows fc may run inside it: it is this module's own, and nobody asked for its output or its gradients."""
+    return isinstance(fc, _OperatorLinear) and not (fc._forward_hooks or fc._backward_hooks or fc._backward_pre_hooks)
+
+
 class MLP(nn.Module):
     """Container with the reference's constructor and ``fc`` ModuleList (nets.py:66-107).
     Inside the fused models only its parameters are used; its own ``forward`` (plain torch
@@ -127,7 +146,9 @@ class MLP(nn.Module):
     ``h + dropout(act(fc(norm(h))))``: every layer but the first normalises its input (``norm.<layer - 1>``), the sum is taken where a
     hidden layer's two widths agree, and dropout acts in training mode, its seed drawn from torch's CPU generator.  With any of
     them the forward and backward passes run in the library's kernels (``ops.linear``, ``ops.layer_norm``, ``ops.dropout``) and need
-    a ROCm device; fp32, bf16 and fp16 parameters, and the activations 'gelu' and 'silu' besides the others."""
+    a ROCm device; fp32, bf16 and fp16 parameters, and the activations 'gelu' and 'silu' besides the others.  ``fc`` and ``norm`` hold
+    modules that are called, so hooks run, and what rebuilds a weight before a call (weight norm, spectral norm, pruning) acts; where an
+    ``fc`` has forward or backward hooks or was replaced, its activation and the sum run in torch, outside of it."""
 
     operators = False           # of an MLP that was pickled before there were these options
 
@@ -160,8 +181,9 @@ class MLP(nn.Module):
             if act not in (ops.LINEAR_ACT_IDS if self.operators else ops.ACT_IDS):
                 raise ValueError('Incorrect activation: {}'.format(act))
         dims = [self.input_dim] + list(self.hidden_dim[:self.n_layers - 1]) + [self.output_dim]
-        self.fc = nn.ModuleList([nn.Linear(dims[i], dims[i + 1]) for i in range(self.n_layers)])
-        self.norm = nn.ModuleList([nn.LayerNorm(d) for d in dims[1:-1]]) if layer_norm else None
+        linear = _OperatorLinear if self.operators else nn.Linear
+        self.fc = nn.ModuleList([linear(dims[i], dims[i + 1]) for i in range(self.n_layers)])
+        self.norm = nn.ModuleList([_OperatorNorm(d) for d in dims[1:-1]]) if layer_norm else None
         self.to(self.device)
 
     @staticmethod
@@ -175,6 +197,10 @@ class MLP(nn.Module):
             return self.xtanh(h, alpha=self.slope)
         if kind == 'sigmoid':
             return torch.sigmoid(h)
+        if kind == 'gelu':
+            return F.gelu(h)
+        if kind == 'silu':
+            return F.silu(h)
         return h
 
     def _forward_operators(self, x):
@@ -188,21 +214,24 @@ class MLP(nn.Module):
             if torch.jit.is_tracing():
                 raise RuntimeError('a traced MLP would draw the same dropout mask at every call: call eval() first')
             seed = int(torch.randint(2 ** 63 - 1, ()))
-        grad = torch.is_grad_enabled()
         h = x
         for c, fc in enumerate(self.fc):
-            t = h
-            if self.norm is not None and c:
-                n = self.norm[c - 1]
-                t = _LayerNormFn.apply(t, n.weight, n.bias, n.eps, grad)
+            t = self.norm[c - 1](h) if self.norm is not None and c else h
             if c == self.n_layers - 1:
-                return _LinearFn.apply(t, fc.weight, fc.bias, 'none', self.slope, None, grad)
-            add = h if self.residual and fc.in_features == fc.out_features else None
-            if drop:
-                t = _LinearFn.apply(t, fc.weight, fc.bias, self.activation[c], self.slope, None, grad)
-                h = _DropoutFn.apply(t, drop, seed, c, add, grad)
+                return fc(t)
+            # (the sum joins a layer whose result has its input's width)
+            fused = _fuses(fc)
+            if fused:
+                add = h if self.residual and fc.in_features == fc.out_features else None
+                t = fc(t, self.activation[c], self.slope, None if drop else add)
             else:
-                h = _LinearFn.apply(t, fc.weight, fc.bias, self.activation[c], self.slope, add, grad)
+                t = self._act(self.activation[c], fc(t))
+                add = h if self.residual and t.shape[-1] == h.shape[-1] else None
+            if drop:
+                t = _DropoutFn.apply(t, drop, seed, c, add, torch.is_grad_enabled())
+            elif add is not None and not fused:
+                t = t + add
+            h = t
         return h
 
     def forward(self, x):

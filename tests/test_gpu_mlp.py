@@ -1,6 +1,7 @@
 """What autograd and modules promise, kept by MLP's operator path."""
 import pytest
 import torch
+import torch.nn.utils.prune
 from torch.autograd import forward_ad
 
 from ivae_amd import MLP
@@ -66,3 +67,92 @@ def test_tracing_with_dropout_is_refused():
     m, x = mlp(**OPTS[-1]).train(), torch.randn(7, 12, device="cuda")
     with pytest.raises(RuntimeError, match="mask"):
         torch.jit.trace(m, x, check_trace=False)
+
+
+def reference(m, x):
+    """The same modules one after the other, with torch's operations."""
+    h = x
+    for c, fc in enumerate(m.fc):
+        t = h
+        if m.norm is not None and c:
+            t = torch.nn.functional.layer_norm(t, t.shape[-1:], m.norm[c - 1].weight, m.norm[c - 1].bias, m.norm[c - 1].eps)
+        t = torch.nn.functional.linear(t, fc.weight, fc.bias)
+        if c == m.n_layers - 1:
+            return t
+        t = torch.nn.functional.gelu(t)
+        h = t + h if m.residual and t.shape[-1] == h.shape[-1] else t
+
+
+def close(a, b):
+    """Four layers of sums of at most 80 terms in 32 bits on both sides: 4 * 80 * 2^-24 = 2e-5 of the largest magnitude each."""
+    return float((a - b).abs().max()) <= 4e-5 * float(b.abs().max())
+
+
+@pytest.mark.parametrize("opts", OPTS)
+def test_hooks_run_and_see_what_they_ask_for(opts):
+    m, x = mlp(**opts).eval(), torch.randn(9, 12, device="cuda")
+    want, seen, norms, grads = m(x), {}, [], []
+    handles = [fc.register_forward_hook(lambda mod, a, out, c=c: seen.__setitem__(c, (a[0].detach(), out.detach()))) for c, fc in enumerate(m.fc)]
+    handles += [n.register_forward_hook(lambda mod, a, out: norms.append(out)) for n in (m.norm or [])]
+    handles.append(m.fc[1].register_full_backward_hook(lambda mod, gi, go: grads.append((gi[0], go[0]))))
+    y = m(x)
+    assert close(y, want) and sorted(seen) == [0, 1, 2, 3] and len(norms) == len(m.norm or [])
+    for c, (a, out) in seen.items():                # a linear layer's output, before its activation
+        assert close(out, torch.nn.functional.linear(a, m.fc[c].weight, m.fc[c].bias))
+    y.sum().backward()
+    assert len(grads) == 1 and grads[0][0].shape == grads[0][1].shape == (9, 40)
+    # a hook's return value replaces the output
+    for h in handles:
+        h.remove()
+    m.fc[1].register_forward_hook(lambda mod, a, out: torch.zeros_like(out))
+    zeroed = mlp(**opts).eval()
+    with torch.no_grad():
+        zeroed.fc[1].weight.zero_(), zeroed.fc[1].bias.zero_()
+    assert close(m(x), zeroed(x))
+
+
+@pytest.mark.parametrize("opts", OPTS)
+@pytest.mark.parametrize("how", ["weight_norm", "spectral_norm", "prune", "parametrize"])
+def test_weights_rebuilt_before_a_call_are_used(how, opts):
+    m, x = mlp(**opts), torch.randn(9, 12, device="cuda")
+    if how == "weight_norm":
+        torch.nn.utils.weight_norm(m.fc[1])
+        with torch.no_grad():
+            m.fc[1].weight_g.mul_(2)
+    elif how == "spectral_norm":
+        torch.nn.utils.spectral_norm(m.fc[1])
+        with torch.no_grad():
+            m.fc[1].weight_orig.mul_(3)
+    elif how == "prune":
+        torch.nn.utils.prune.l1_unstructured(m.fc[1], "weight", amount=.5)
+        with torch.no_grad():
+            m.fc[1].weight_orig.mul_(2)
+    else:
+        torch.nn.utils.parametrizations.weight_norm(m.fc[1])
+        with torch.no_grad():
+            m.fc[1].parametrizations.weight.original0.mul_(2)
+    m.eval()
+    stale = m.fc[1].weight.detach().clone() if how != "parametrize" else None
+    y = m(x)
+    assert close(y, reference(m, x))                # (the call above has rebuilt the weight)
+    if how in ("weight_norm", "prune"):
+        assert not torch.equal(stale, m.fc[1].weight)
+    y.sum().backward()
+    assert all(p.grad is not None for p in m.fc[1].parameters())
+
+
+def test_replaced_layers_are_called():
+    m, x = mlp(layer_norm=True, residual=True), torch.randn(9, 12, device="cuda")
+    want = m(x)
+
+    class Twice(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, x):
+            return self.inner(x) * 1.0
+
+    m.fc[1] = Twice(m.fc[1])
+    m.fc[2] = torch.nn.Sequential(m.fc[2])
+    assert close(m(x), want)
