@@ -177,12 +177,14 @@ __device__ __forceinline__ void touch_residual(const BigProduct& G, const LinArg
     constexpr int E = 64 / sizeof(T), PER_ROW = BTQ / E, LOADS = BTP * PER_ROW / THREADS;
     const uint32_t base = __builtin_amdgcn_readfirstlane(at + threadIdx.x / 64 * 256);
     int64_t q = at0.q0 + threadIdx.x % PER_ROW * E;
-    if (q > G.q_end - 4 / (int)sizeof(T)) q = G.q_end - 4 / (int)sizeof(T);          // (4 bytes inside the row; there are 64 columns at least)
+    // (4 bytes inside the row, of 64 columns at least: at the element, or where that lies off 4 bytes at the next one)
+    constexpr int INSIDE = sizeof(T) == 2 ? 3 : 1;
+    if (q > G.q_end - INSIDE) q = G.q_end - INSIDE;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
         int64_t p = at0.p0 + threadIdx.x / PER_ROW + j * (THREADS / PER_ROW);
         if (p >= G.p_end) p = G.p_end - 1;
-        const uintptr_t a = (uintptr_t)((const T*)A.res + p * A.ldr + q) & ~(uintptr_t)3;
+        const uintptr_t a = ((uintptr_t)((const T*)A.res + p * A.ldr + q) + 3) & ~(uintptr_t)3;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(a) : "memory");
     }
 }

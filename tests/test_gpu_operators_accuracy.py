@@ -252,3 +252,19 @@ def test_gelu_keeps_its_digits_in_the_tail(dt):
 def test_slopes_keep_their_digits_in_the_tails(dt, act):
     """exp(-s) and exp(-2 |s|): 2 |s| half steps, twice (argument and constant)."""
     check_tails(dt, act, lambda s: (16 + 4 * s.abs()) * R.U32 + (2.0 ** -18 if act == "xtanh" and dt != F32 else 0.0))
+
+
+@pytest.mark.parametrize("off", [0, 1, 5])
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_residual_rows_at_any_offset_of_a_large_product(dt, off):
+    """The residual's rows start anywhere, the first and the last of them at the ends of the allocation."""
+    g = torch.Generator().manual_seed(10)
+    m, k, n = 4100, 520, 2003
+    x, w, r = (torch.randint(-3, 4, s, generator=g).to(dt).to(dev()) for s in ((m, k), (n, k), (m, n)))
+    if dt != F32:       # a large product whose sums are not split needs no workspace here; it is these that bring the residual into the cache
+        assert ops._linear_plan(m, k, n, ops.DTYPE_IDS[dt], 0, R.SLOPE, k, n, 0, 0)[1] == 0
+    for ld in (n, n + 6, n + 7):
+        flat = torch.full((off + (m - 1) * ld + n,), float("nan"), dtype=dt, device=dev())
+        view = flat[off:].as_strided((m, n), (ld, 1))
+        view.copy_(r)
+        assert torch.equal(ops.linear(x, w, residual=view), (x.double() @ w.double().t() + r.double()).to(dt))
