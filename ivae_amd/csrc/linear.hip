@@ -206,13 +206,15 @@ static hipError_t big_backward(const LinArgs& A, int dtype, void* ws, hipStream_
 // ---- which kernel -----------------------------------------------------------------------------------------------------
 static bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
 // The large kernels from the size on from which they take less time, all their launches together (us, small | large):
-//   16 bits, forward    2048 x 512 x 1024 14 | 15, 1024 x 1024 x 1024 20 | 27, 2048 x 1024 x 1024 26 | 19, 128 x 4096 x 4096 34 | 23;
-//                       1531 x 1001 x 777 34 | 29
-//   16 bits, backward   no activation 1024 x 256 x 256 11 | 14, 512 x 512 x 512 13 | 14, 1003 x 777 x 531 28 | 25, 768 x 768 x 768 24 | 17
+//   16 bits, forward    256 x 2048 x 2048 20 | 23, 1024 x 1024 x 1024 18 | 14, 65 x 4096 x 4096 31 | 18, 2048 x 1024 x 1024 24 | 14
+//                       odd sizes 701 x 701 x 701 16 | 17, 803 x 803 x 803 19 | 18, 1003 x 901 x 777 24 | 20, 65 x 4099 x 4099 51 | 35
+//                       (but 129 x 2003 x 2003 20 | 28)
+//   16 bits, backward   no activation 512 x 512 x 512 13 | 14, 1024 x 512 x 512 16 | 20, 1003 x 777 x 531 28 | 25, 768 x 768 x 768 24 | 17
 //                       gelu (the small kernel in fp32, the large one in pairs) 512 x 512 x 512 20 | 22, 300 x 1001 x 777 34 | 23,
 //                       1024 x 512 x 512 31 | 27, 1024 x 1024 x 1024 84 | 36
-//   fp32, forward       1024 x 1024 x 1024 31 | 40, 2048 x 1024 x 1024 48 | 54, 300 x 4096 x 2048 81 | 75, 128 x 4096 x 4096 51 | 75
-//                       (cutting the weight in three costs as much as a product with 128 rows); 1531 x 1001 x 777 65 | 47
+//   fp32, forward       1024 x 1024 x 1024 28 | 39, 2048 x 1024 x 1024 45 | 49, 1024 x 2048 x 1024 51 | 49, 300 x 4096 x 2048 81 | 75, 128 x
+//                       4096 x 4096 49 | 68 (cutting the weight in three costs as much as a product with 128 rows)
+//                       odd sizes 803 x 803 x 803 29 | 37, 1003 x 901 x 777 37 | 36, 1003 x 1001 x 1003 46 | 38
 //   fp32, backward      512 x 512 x 512 25 | 27, 1024 x 512 x 512 36 | 30, 1024 x 1024 x 1024 96 | 47
 // Forward, rows that do not start on 16 bytes cost the small kernel twice the loads, the large one only its packing.
 static bool big_by_size(const LinArgs& A, int dtype, bool backward) {
@@ -224,8 +226,9 @@ static bool big_by_size(const LinArgs& A, int dtype, bool backward) {
     if (backward && dtype == IVAE_F16 && !(isfinite(A.slope) && slope_bound(A.act, A.slope) <= (float)(1 << SHIFT_MAX))) return false;
     const double flops = 2.0 * (double)A.M * (double)A.N * (double)A.K;
     const bool ragged = A.K % (dtype == IVAE_F32 ? 4 : 8) != 0;
-    if (dtype == IVAE_F32) return backward ? flops >= 5e8 : flops >= (ragged ? 2e9 : 5e9) && A.M >= 256;
-    return flops >= (backward ? A.act == IVAE_ACT_NONE ? 2e8 : 3e8 : ragged ? 2e9 : 3e9);
+    if (dtype == IVAE_F32) return backward ? flops >= 5e8 : flops >= (ragged ? 1.4e9 : 5e9) && A.M >= 256;
+    if (backward) return flops >= (A.act == IVAE_ACT_NONE ? 8e8 : 3e8);
+    return flops >= (ragged ? 1e9 : 2.1e9);
 }
 // a matrix that would be loaded in place has to start on 16 bytes
 static bool big_in_place(const void* p, int64_t cols, int64_t ld, int dtype) { return dtype == IVAE_F32 || ld % 8 || cols % 8 || aligned(p); }
@@ -233,7 +236,7 @@ static bool big_in_place(const void* p, int64_t cols, int64_t ld, int dtype) { r
 size_t linear_ws_bytes(const IvaeLinear& L, bool backward) {
     LinArgs A = lin_args(L);
     A.dx = A.dw = A.db = &A;           // the size serves a call that asks for all of them
-    if (!backward && A.M <= ROWS_MAX) return rows_ws(A);
+    if (!backward && rows_serve(A, L.dtype)) return rows_ws(A);
     size_t n = linear_small_ws(A, backward);
     if (big_by_size(A, L.dtype, backward)) {
         const size_t big = backward ? plan_big_backward(A, L.dtype, nullptr).bytes : plan_big_forward(A, L.dtype, nullptr).bytes;
@@ -245,7 +248,7 @@ hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, cons
                          void* ws, hipStream_t st) {
     LinArgs A = lin_args(L);
     A.x = x; A.w = w; A.b = b; A.res = residual; A.y = y; A.pre = (float*)saved; A.part = (float*)ws;
-    if (A.M <= ROWS_MAX) return linear_rows_forward(A, L.dtype, st);
+    if (rows_serve(A, L.dtype)) return linear_rows_forward(A, L.dtype, st);
     if (big_by_size(A, L.dtype, false) && big_in_place(x, A.K, A.ldx, L.dtype) && big_in_place(w, A.K, A.K, L.dtype) && aligned(ws))
         return big_forward(A, L.dtype, ws, st);
     return linear_small_forward(A, L.dtype, st);

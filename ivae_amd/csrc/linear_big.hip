@@ -153,6 +153,7 @@ __device__ __forceinline__ void block_barrier() {
 
 // Tiles in bands of 8 rows of tiles, neighbours in a band one after the other, and a contiguous run of them for each of the 8 dies
 // (blocks go to the dies in turn): a die's cache then serves the few operand strips that its run shares.
+// (Bands of 1 | 4 | 8 | 16: fp16 2048 x 8192 x 8192 gradients 485 | 443 | 446 | 451 us, fp32 8192 x 2048 x 2048 forward 339 | 338 | 347 | 351.)
 struct Place { int64_t p0, q0, ra, rb; int split; };
 template <int BTP, int BTQ> __device__ __forceinline__ Place place(const BigProduct& G, int b) {
     const int tp = (int)((G.p_end + BTP - 1) / BTP), tq = (int)((G.q_end + BTQ - 1) / BTQ), tiles = tp * tq, blocks = tiles * G.splits;

@@ -110,7 +110,15 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_rows(LinArgs A, int len, 
     }
 }
 
-static int rows_nf(const LinArgs& A) { return A.M > 16 && A.N >= 8192 ? 2 : 1; }
+// Up to 64 rows, the most that a block's registers hold; fp32 up to 32 where blocks of 16 weight rows (below) read x too often for its slower
+// matrix instructions (us, here | on 64 x 64 tiles: fp16 64 x 1024 x 1024 6.9 | 9.5, 64 x 2048 x 8192 14 | 22, 64 x 4096 x 4096 21 | 22, 64 x 8192 x
+// 2048 24 | 22; fp32 32 x 4096 x 4096 29 | 31, 33 x 4096 x 4096 39 | 35, 64 x 4096 x 4096 46 | 31, 64 x 1024 x 1024 13 | 11, 64 x 200 x 200 6.7 | 11,
+// 64 x 2048 x 8192 30 | 31)
+bool rows_serve(const LinArgs& A, int dtype) { return A.M <= (dtype == IVAE_F32 && A.K >= 1024 && A.N <= 4096 ? 32 : 64); }
+// 32 weight rows a block, which halves what is read of x, where blocks of 16 would be more than the chip has CUs (us, 16 | 32 weight rows: fp16
+// 24 x 2048 x 4096 7.1 | 8.7, 24 x 2048 x 6000 12.5 | 9.6, 64 x 2048 x 4096 12.0 | 11.5, 64 x 2048 x 6000 22 | 14, 64 x 4096 x 16384 78 | 45; fp32
+// 24 x 2048 x 4096 13.7 | 14.8, 24 x 2048 x 6000 25.9 | 21.3, 64 x 2048 x 8192 47 | 30); up to 16 rows read little of it
+static int rows_nf(const LinArgs& A) { return A.M > 16 && A.N > 4096 ? 2 : 1; }
 RowsPlan rows_plan(const LinArgs& A) {
     RowsPlan p;
     p.nf = rows_nf(A);

@@ -382,7 +382,9 @@ static int64_t groups_of(int64_t rows, int tpr, int64_t most) {     // blocks of
     const int64_t need = (rows + rpb - 1) / rpb;
     return need < most ? need : most;
 }
-// about as many blocks as the chip holds: each keeps the weight in registers, and in the backward pass its sums
+// about as many blocks as the chip holds: each keeps the weight in registers, and in the backward pass its sums (us, forward / gradients, half as
+// many | these | twice as many blocks: 16384 x 4096 bf16 48/100 | 42/83 | 43/105, 5003 x 1037 fp32 17/30 | 13/23 | 15/28, 65536 x 256 bf16 14/29 | 13/27 |
+// 14/33, 2048 x 16384 bf16 37/91 | 36/91 | 31/121, 4096 x 8192 bf16 30/53 | 31/65 | 28/93)
 static int fwd_blocks(int64_t rows, Share h) { return (int)groups_of(rows, h.tpr, h.tpr <= 256 ? 1280 : h.tpr == 512 ? 640 : 320); }
 // blocks of the backward pass = rows of `part`.  Few rows are walked by one block, which needs neither a workspace nor a join
 // (up to 24 x 128, 6 x 2048, 4 x 4096: 11.6 us a call with the host's part, 16 with them; the kernel takes up to 10 us instead of 4 and 2.5).
