@@ -303,6 +303,10 @@ int ivae_debug_fault_inject(int32_t mask);
  * host work of the call around them (argument checks, step tables: ~20 us that events recorded by the caller include;
  * bench.py's roofline figure).  The pair is used once. */
 int ivae_debug_launch_events(void* start_event, void* stop_event);
+/* Test hook, no counterpart in the reference: what ivae_linear (backward != 0: ivae_linear_backward, all three gradients) would launch for this
+ * shape with tensors on 16-byte boundaries.  out[0]: 0 few rows, 1 the 64 x 64 tiles, 2 the large tiles; out[1]: rows of a tile (few rows: weight
+ * rows a block); out[2], out[3]: parts of the sums of y or dx, and of dw; out[4]: blocks (large tiles). */
+int ivae_debug_linear_plan(const IvaeLinear* lin, int32_t backward, int32_t out[5]);
 
 #ifdef __cplusplus
 }

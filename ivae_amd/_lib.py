@@ -51,7 +51,7 @@ EXPORTS = ["ivae_param_count", "ivae_workspace_bytes", "ivae_workspace_layout", 
            "ivae_pairwise", "ivae_pairwise_workspace_bytes", "ivae_backward", "ivae_adam_step", "ivae_elbo_adam_steps", "ivae_train_steps", "ivae_train_steps_supported", "ivae_corr_workspace_bytes", "ivae_corr", "ivae_corr_static", "ivae_corr_batched",
            "ivae_linear_workspace_bytes", "ivae_linear", "ivae_linear_backward", "ivae_layer_norm_workspace_bytes", "ivae_layer_norm",
            "ivae_layer_norm_backward", "ivae_dropout",
-           "ivae_last_hip_error", "ivae_version", "ivae_debug_fault_inject", "ivae_debug_launch_events"]
+           "ivae_last_hip_error", "ivae_version", "ivae_debug_fault_inject", "ivae_debug_launch_events", "ivae_debug_linear_plan"]
 
 _lib = None
 
@@ -88,6 +88,7 @@ def lib():
     L.ivae_corr_batched.argtypes = [vp, vp, C.c_int64, C.c_int64, C.c_int32, vp, vp]
     pl, pn = C.POINTER(IvaeLinear), C.POINTER(IvaeNorm)
     L.ivae_linear_workspace_bytes.argtypes = [pl, C.c_int32, C.POINTER(C.c_size_t)]
+    L.ivae_debug_linear_plan.argtypes = [pl, C.c_int32, C.POINTER(C.c_int32)]
     L.ivae_linear.argtypes = [pl, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
     L.ivae_linear_backward.argtypes = [pl, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
     L.ivae_layer_norm_workspace_bytes.argtypes = [pn, C.POINTER(C.c_size_t)]

@@ -343,6 +343,16 @@ int ivae_linear_workspace_bytes(const IvaeLinear* lin, int32_t backward, size_t*
     return IVAE_OK;
 }
 
+int ivae_debug_linear_plan(const IvaeLinear* lin, int32_t backward, int32_t out[5]) {
+    if (!out) return IVAE_E_NULLPTR;
+    const int rc = check_linear(lin);
+    if (rc) return rc;
+    int32_t v[5] = {};
+    linear_plan(*lin, backward != 0, v);
+    for (int i = 0; i < 5; ++i) out[i] = v[i];
+    return IVAE_OK;
+}
+
 int ivae_linear(const IvaeLinear* lin, const void* x, const void* w, const void* b, const void* residual, void* y, void* saved,
                 void* workspace, size_t workspace_bytes, void* stream) {
     const int rc = check_linear(lin);

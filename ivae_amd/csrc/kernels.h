@@ -47,6 +47,7 @@ hipError_t launch_corr_batched(const float* x, const float* y, int64_t n_blocks,
 hipError_t launch_corr_static(const float* x, const float* y, int64_t n, int d, double* cc, hipStream_t st);
 #define CORR_STATIC_MAX_D 40
 size_t linear_ws_bytes(const IvaeLinear& L, bool backward);
+void linear_plan(const IvaeLinear& L, bool backward, int32_t (&out)[5]);
 hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, const void* b, const void* residual, void* y, void* saved,
                          void* ws, hipStream_t st);
 hipError_t launch_linear_backward(const IvaeLinear& L, const void* dy, const void* x, const void* w, const void* saved, void* dx, void* dw,

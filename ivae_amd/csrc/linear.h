@@ -136,6 +136,7 @@ __device__ __forceinline__ void forward_store(const LinArgs& A, int64_t m, int n
 hipError_t linear_small_forward(const LinArgs& A, int dtype, hipStream_t st);
 hipError_t linear_small_backward(const LinArgs& A, int dtype, hipStream_t st);
 size_t linear_small_ws(const LinArgs& A, bool backward);
+void linear_small_splits(const LinArgs& A, bool backward, int32_t* splits);     // two of them: y or dx, dw
 
 // sums of split parts: kx, kw of them where there are two or more, kb where there is one (db is not written before the join)
 struct LinParts { const float* x; const float* w; const float* b; int kx, kw, kb; };

@@ -244,6 +244,28 @@ size_t linear_ws_bytes(const IvaeLinear& L, bool backward) {
     }
     return n;
 }
+void linear_plan(const IvaeLinear& L, bool backward, int32_t (&out)[5]) {
+    LinArgs A = lin_args(L);
+    A.dx = A.dw = A.db = &A;
+    if (!backward && rows_serve(A, L.dtype)) {
+        const RowsPlan p = rows_plan(A);
+        out[1] = 16 * p.nf;
+        out[2] = p.splits;
+    } else if (!big_by_size(A, L.dtype, backward)) {
+        out[0] = 1;
+        out[1] = 64;
+        linear_small_splits(A, backward, out + 2);
+    } else {
+        out[0] = 2;
+        const BigForward f = backward ? BigForward{} : plan_big_forward(A, L.dtype, nullptr);
+        const BigBackward g = backward ? plan_big_backward(A, L.dtype, nullptr) : BigBackward{};
+        const BigProduct& B = backward ? g.X : f.B;
+        out[1] = B.tile_p;
+        out[2] = B.splits;
+        out[3] = backward ? g.W.splits : 0;
+        out[4] = (int32_t)(big_tiles(B) * B.splits + (backward ? big_tiles(g.W) * g.W.splits : 0));
+    }
+}
 hipError_t launch_linear(const IvaeLinear& L, const void* x, const void* w, const void* b, const void* residual, void* y, void* saved,
                          void* ws, hipStream_t st) {
     LinArgs A = lin_args(L);

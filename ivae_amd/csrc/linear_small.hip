@@ -153,6 +153,16 @@ size_t linear_small_ws(const LinArgs& A, bool backward) {
     return (size_t)plan_bwd(A).floats * 4;
 }
 
+void linear_small_splits(const LinArgs& A, bool backward, int32_t* splits) {
+    if (!backward) {
+        splits[0] = split_of(A.M, A.N, A.K, SPLIT_FORWARD).splits;
+        return;
+    }
+    const BwdPlan p = plan_bwd(A);
+    splits[0] = p.X.splits;
+    splits[1] = p.W.splits;
+}
+
 static unsigned cap(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20); }
 
 hipError_t linear_join_forward(const LinArgs& A, int splits, int dtype, hipStream_t st) {
