@@ -85,6 +85,7 @@ def reference(m, x):
 
 def close(a, b):
     """Four layers of sums of at most 80 terms in 32 bits on both sides: 4 * 80 * 2^-24 = 2e-5 of the largest magnitude each."""
+    a, b = a.detach(), b.detach()
     return float((a - b).abs().max()) <= 4e-5 * float(b.abs().max())
 
 

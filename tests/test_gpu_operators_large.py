@@ -117,3 +117,18 @@ def test_replays_and_streams(dt, act):
         other = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, out, other))
+
+
+@pytest.mark.parametrize("dt", R.DTYPES)
+def test_repeated_and_overlapping_rows(dt):
+    """x one row repeated (stride 0), rows that overlap by all but one element (stride 1), x as the residual, and dy as x."""
+    g = torch.Generator().manual_seed(9)
+    m, k = 2200, 1104
+    w = whole(g, k, k, dtype=dt)
+    flat = whole(g, m + k, dtype=dt)
+    for x in (flat[:k].expand(m, k), flat.as_strided((m, k), (1, 1)), flat.as_strided((m, k), (0, 1))):
+        X, W = x.double(), w.double()
+        assert S.plan(m, k, k, ops.DTYPE_IDS[dt])[0] == S.LARGE
+        assert torch.equal(ops.linear(x, w, residual=x), (X @ W.t() + X).to(dt))
+        for got, want in zip(ops.linear_backward(x, x, w), (X @ W, X.t() @ X, X.sum(0))):
+            assert torch.equal(got, want.to(dt))
