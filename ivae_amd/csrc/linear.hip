@@ -160,7 +160,7 @@ static BigBackward plan_big_backward(const LinArgs& A, int dtype, void* ws) {
     const bool pair = dtype != IVAE_F32 && A.act != IVAE_ACT_NONE;
     f.ds = pack_of(A.dy, A.M, A.N, A.lddy, dtype, m, pair);
     const int shift = dtype == IVAE_F16 ? slope_shift(A.act, A.slope) : 0;
-    f.ds.P.scale = ldexpf(1.f, -shift); f.ds.P.up = dtype == IVAE_F16 ? 2048.f : 1.f;
+    f.ds.P.scale = ldexpf(1.f, -shift); f.ds.P.up = dtype == IVAE_F16 ? 2048.f : 128.f;
     f.ds.P.pre = A.act != IVAE_ACT_NONE ? A.cpre : nullptr;
     f.ds.P.act = A.act; f.ds.P.slope = A.slope;
     if (!f.ds.needed) {                                 // dy itself; only its column sums are taken

@@ -8,11 +8,12 @@
 // bits of the row number that puts every 16 lanes (along) or every 8 groups of 32 bytes (down) on distinct banks.
 //
 // 16-bit types with an activation, backward: act'(s) dy has 32 bits and enters as a pair of numbers of the type, P = scale (first + low
-// second), the whole sum over the second before the one over the first, in the same registers.  bf16: the second is what rounding left
-// (2^-16 of the value remains).  fp16: values are divided by a bound of act', so that dy's range fits, and what rounding left is multiplied by
-// 2^11: 2^-22 of the value remains, or 2^-36 among the smallest.  The products cost twice the time (8192 x 4096 x 4096 bf16, gelu: 446 -> 826 us); with one
-// number the results had 1.4 times the error of their own rounding, and fp16 lost gradients of 1e-6 and those beyond 65504.  A second number of 0 makes a NaN of an infinity: tiles with a NaN
-// are computed again in fp32, as below.
+// second), the whole sum over the second before the one over the first, in the same registers.  bf16: the second is what rounding left,
+// times 2^7 (half of the first at most): off by 2^-16 of the value, or 2^-141 among the smallest.  fp16: values are divided by a bound of
+// act', so that dy's range fits, and what rounding left is multiplied by 2^11: off by 2^-22 of the value, or 2^-36 times the bound among the
+// smallest.  The products cost twice the time (8192 x 4096 x 4096 bf16, gelu: 446 -> 826 us); with one number the results had 1.4 times the
+// error of their own rounding, and fp16 lost gradients of 1e-6 and those beyond 65504.  A second number of 0 makes a NaN of an infinity: tiles
+// with a NaN are computed again in fp32, as below.
 //
 // fp32 (k_split_*): x = x0 + x1 + x2 with bf16 parts cut off after 8 bits each (exact from 2^-110 on), and x y = x0 y0 + x0 y1 + x1 y0 + x1 y1 + x0 y2 +
 // x2 y0 up to 2^-23 |x y|: six products at 16 times the rate of the fp32 matrix instructions.  The running sum of the bf16 matrix

@@ -102,6 +102,19 @@ def test_small_fp16_gradients_keep_their_digits(scale, m, k, n):
 
 
 @pytest.mark.parametrize("m,k,n", SIZES)
+def test_smallest_bf16_gradients_keep_their_digits(m, k, n):
+    """dy at the end of bf16's range, where a second number at the first one's scale would have no bits left, and products far inside of it."""
+    g = torch.Generator().manual_seed(5)
+    x, w = normal(g, m, k, dtype=BF16), normal(g, n, k, scale=k ** -0.5, dtype=BF16)
+    dy = normal(g, m, n, dtype=F32).mul(2.0 ** -125).to(BF16)
+    big = torch.ldexp(x.float(), torch.tensor(60)).to(BF16)
+    _, saved = ops.linear(x.to(dev()), w.to(dev()), None, "gelu", save=True)
+    want = formula(x, w, None, "gelu", dy)["dw"] * 2.0 ** 60
+    _, got, _ = ops.linear_backward(dy.to(dev()), big.to(dev()), w.to(dev()), saved, "gelu")
+    only_rounded(got * 2.0 ** 60, want * 2.0 ** 60, BF16, "dw")
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
 @pytest.mark.parametrize("act,slope", [("gelu", .1), ("lrelu", 2.0), ("lrelu", 1000.0), ("xtanh", 30.0), ("silu", .1)])
 def test_large_fp16_gradients_stay_finite(act, slope, m, k, n):
     """act'(s) dy beyond 65504, in products that the type holds."""
