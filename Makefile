@@ -6,8 +6,8 @@ SRCS := $(wildcard $(CSRC)/*.hip)
 OBJS := $(SRCS:.hip=.o)
 HDRS := $(wildcard $(CSRC)/*.h) include/ivae_amd.h
 LIB := ivae_amd/libivae_amd.so
-# no packed fp32 instructions (v_pk_add / mul / fma_f32): some forms of them have given wrong results on these cards now and then.
-# (hipcc's host pass says that it does not know the feature; that is harmless.)  Two sources keep them: without them elbo_mfma.hip
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): a precaution, no result here was traced to them.  (hipcc's host pass says that it
+# does not know the feature; that is harmless.)  Two sources keep them: without them elbo_mfma.hip
 # contracts other products, which changes the last bits of what it computed so far, and pairwise.hip is 13 to 30 % slower at equal bits.
 NOPK := -Xclang -target-feature -Xclang -packed-fp32-ops
 CXXFLAGS := -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -Wall -Wno-unused-function

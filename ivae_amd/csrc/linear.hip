@@ -21,7 +21,7 @@ static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 static int64_t tiles_of(const BigProduct& B, int tp, int tq) { return ((B.p_end + tp - 1) / tp) * ((B.q_end + tq - 1) / tq); }
 // Tiles and splits of the products of one launch: the choice for which a simple model of its time is least.  A round of 256 blocks, one a
 // CU, takes `start` us (those after the first `again` of it) and `per` ns for each of its summed index (fitted to products of one to four
-// rounds: 16 bits, 256 x 256 and 128 x 128 tiles, the small ones two a CU; split fp32, 256 x 128 and 128 x 128); split sums cost a launch
+// rounds: 16 bits, 256 x 256 and 128 x 128 tiles, the small ones two a CU; split fp32, 256 x 128 and 128 x 128); a pair's sum is twice as long; split sums cost a launch
 // and are joined at 6 TB/s.  What it decides between (us, forward, 256-wide | 128-wide): fp16 4096 x 4096 x 4096 114 | 136,
 // 4096 x 2048 x 2048 53 | 42, 8192 x 1024 x 1024 36 | 26; fp32 4096 x 1024 x 4096 197 | 216, 2048 x 2048 x 2048 118 | 109.
 struct BigModel { int tile_p, tile_q; double start, again, per; };

@@ -90,6 +90,7 @@ struct Stage {
         return r;
     }
     static __device__ __forceinline__ uint32_t wave_base(uint32_t lds) { return __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024); }
+    // (m0 is written without the compiler's knowledge, which takes no clobber of it: nothing that it makes of these kernels uses m0)
     __device__ __forceinline__ void load_one(int j, uint32_t base, u32x4 rsrc) const {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(base + j * THREADS * 16), "v"(voff[j]), "s"(rsrc)
                      : "memory");
@@ -622,6 +623,7 @@ static hipError_t go(F fn, int bytes, int threads, SmemCache& cache, int blocks,
 }
 template <typename T, int BT, int WP, int WQ, int BUFS> struct Big16 {
     static constexpr int THREADS = WP * WQ * 64, LDS = big_lds(BUFS, 2 * BT * 64 * 2, BT) + THREADS * 4;
+    static_assert(LDS >= THREADS / 256 * tile_lds<float>(), "a tile with a NaN is computed again here");
     static hipError_t fwd(const BigProduct& B, const LinArgs& A, hipStream_t st) {
         static SmemCache cache;
         return go(k_big_fwd<T, BT, WP, WQ, BUFS>, LDS, THREADS, cache, blocks_of(B), st, B, A);
